@@ -371,6 +371,107 @@ int th_memcpy_d2h(th_ctx* ctx, void* dst, const void* src, size_t bytes);
 int th_ntt_time(th_ctx* ctx, uint64_t* dev_polys, size_t count, uint32_t limbs, int inverse, int reps,
                 float* avg_ms);
 
+/* ---------------------------------------------------------------- plain mixtures of adapters */
+/* The same adapters in the clear, for batches and prefills: a softmax gate per
+ * token, matrix products grouped by expert, and a shared projection with the
+ * low-rank adapters of many requests, each with its gradients. The reference
+ * applies one adapter to one hidden state in the clear
+ * (inference_engine.py:1234-1242) and routes by keyword step-gates
+ * (:1155-1171); batches, gates and gradients are this library's own.
+ *
+ * These calls need no context. They are queued on `stream` (a hipStream_t of
+ * the calling thread's current device; NULL is that device's default stream)
+ * and return without waiting; th_ctx_stream's stream orders them with a
+ * context's work. All arrays are device memory of the caller's, used until the
+ * work queued here has run. Workspaces are the caller's too (256-byte aligned,
+ * at least the size the matching *_workspace call gives) and hold nothing from
+ * call to call. No call allocates, so all of them can be captured into a graph.
+ * Matrices are row-major with unit column stride; strides count elements.
+ *
+ * A slot is a (token, choice) pair, number token * choices + choice. Expert
+ * and adapter numbers outside [0, n) mean "none" everywhere. */
+enum { TH_BF16 = 1, TH_F16 = 2, TH_F32 = 3 };
+
+/* Slots grouped by expert: order (tokens x choices) lists the slots of expert
+ * 0, then 1, ..., then those without one, each in rising order; offsets
+ * (n_experts + 1) says where each expert's begin. At most 1024 experts and 32
+ * choices. */
+int th_group_workspace(int64_t tokens, uint32_t experts, uint32_t choices, size_t* bytes);
+int th_group(const int32_t* experts, int64_t tokens, uint32_t n_experts, uint32_t choices, int32_t* order,
+             int32_t* offsets, void* work, size_t work_bytes, void* stream);
+
+/* Softmax gate with top-k. A token may use expert i if its mask byte is not 0
+ * (mask NULL: all; mask_ld 0: one row for every token) and its logit is above
+ * -inf. The `choices` largest logits are chosen, ties to the lowest index (NaN
+ * counts as the largest); experts[] holds them in falling order, -1 where
+ * fewer are allowed. weights = exp(l - max) / sum, the sum over the chosen
+ * (normalize != 0) or over all allowed experts; 0 for -1. Also groups the slots
+ * (th_group; its workspace). Logits bf16, f16 or f32, at most 512 experts. */
+int th_route(int dtype, const void* logits, int64_t ld, int64_t tokens, uint32_t n_experts, const uint8_t* mask,
+             int64_t mask_ld, uint32_t choices, int normalize, float* weights, int32_t* experts, int32_t* order,
+             int32_t* offsets, void* work, size_t work_bytes, void* stream);
+/* dlogits (tokens x n_experts, contiguous, of the logits' type) from the
+ * gradient of the weights and what th_route returned. */
+int th_route_backward(int dtype, const void* logits, int64_t ld, int64_t tokens, uint32_t n_experts,
+                      const uint8_t* mask, int64_t mask_ld, uint32_t choices, int normalize, const float* weights,
+                      const int32_t* experts, const float* dweights, void* dlogits, void* stream);
+
+/* Products grouped by expert: y[slot] = w[expert of slot] x[token of slot]
+ * (x_per_slot == 0: tokens rows of x) or x[slot] (tokens x choices rows); rows
+ * of slots without an expert are zero. w: experts matrices of d_out x d_in. */
+typedef struct th_grouped {
+  int dtype; /* TH_BF16 or TH_F16: x, w, y and their gradients; sums are in float */
+  int x_per_slot;
+  int64_t tokens;
+  uint32_t choices, experts, d_in, d_out;
+  const void* x;
+  const void* w;
+  int64_t ldx, ldw, ldwe; /* row strides; ldwe: from matrix to matrix */
+  const int32_t* order;   /* th_group or th_route */
+  const int32_t* offsets;
+} th_grouped;
+int th_grouped_matmul(const th_grouped* d, void* y, int64_t ldy, void* stream);
+/* dx (contiguous, as x; a token's choices summed in float) and dw
+ * (contiguous, experts x d_out x d_in) from dy (a row per slot); either may be
+ * NULL. */
+int th_grouped_matmul_backward_workspace(const th_grouped* d, size_t* bytes);
+int th_grouped_matmul_backward(const th_grouped* d, const void* dy, int64_t lddy, void* dx, void* dw, void* work,
+                               size_t work_bytes, void* stream);
+
+/* A shared projection with low-rank adapters:
+ *   y_t = weight x_t + bias + sum_j gate_tj scale_e B_e (A_e x_t), e = experts_tj.
+ * a: adapters matrices of rank x d_in; b: of d_out x rank (ranks up to 128;
+ * shorter ones are padded with zeros). gate (tokens x choices) and scale (per
+ * adapter) are floats, NULL for ones. order and offsets (th_group of
+ * `experts`), or NULL: made in the workspace. */
+typedef struct th_lora_linear_args {
+  int dtype; /* TH_BF16 or TH_F16: x, weight, bias, a, b, y and their gradients */
+  uint32_t choices;
+  int64_t tokens;
+  uint32_t d_in, d_out, rank, adapters;
+  const void* x;
+  const void* weight;
+  const void* bias; /* d_out values, or NULL */
+  const void* a;
+  const void* b;
+  int64_t ldx, ldw, lda, lda_adapter, ldb, ldb_adapter;
+  const int32_t* experts; /* tokens x choices */
+  const float* gate;
+  const float* scale;
+  const int32_t* order;
+  const int32_t* offsets;
+} th_lora_linear_args;
+/* u, if not NULL, receives A_e x_t of every slot in float (row stride: the rank
+ * rounded up to 4), which the backward pass reads. */
+int th_lora_linear_workspace(const th_lora_linear_args* d, int keep_u, size_t* bytes);
+int th_lora_linear(const th_lora_linear_args* d, void* y, int64_t ldy, float* u, void* work, size_t work_bytes,
+                   void* stream);
+/* Gradients of x, a, b (contiguous) and of the gate (tokens x choices) from
+ * dy; each may be NULL. weight and bias are frozen. */
+int th_lora_linear_backward_workspace(const th_lora_linear_args* d, size_t* bytes);
+int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const void* dy, int64_t lddy, void* dx,
+                            void* da, void* db, float* dgate, void* work, size_t work_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

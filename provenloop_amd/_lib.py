@@ -29,7 +29,26 @@ SZ = C.c_size_t
 U32 = C.c_uint32
 U64 = C.c_uint64
 I32 = C.c_int
+I64 = C.c_int64
 PVP = C.POINTER(C.c_void_p)
+
+TH_BF16, TH_F16, TH_F32 = 1, 2, 3
+
+
+class Grouped(C.Structure):
+    """th_grouped"""
+    _fields_ = [("dtype", I32), ("x_per_slot", I32), ("tokens", I64), ("choices", U32), ("experts", U32),
+                ("d_in", U32), ("d_out", U32), ("x", VP), ("w", VP), ("ldx", I64), ("ldw", I64), ("ldwe", I64),
+                ("order", VP), ("offsets", VP)]
+
+
+class LoraLinear(C.Structure):
+    """th_lora_linear_args"""
+    _fields_ = [("dtype", I32), ("choices", U32), ("tokens", I64), ("d_in", U32), ("d_out", U32), ("rank", U32),
+                ("adapters", U32), ("x", VP), ("weight", VP), ("bias", VP), ("a", VP), ("b", VP), ("ldx", I64),
+                ("ldw", I64), ("lda", I64), ("lda_adapter", I64), ("ldb", I64), ("ldb_adapter", I64),
+                ("experts", VP), ("gate", VP), ("scale", VP), ("order", VP), ("offsets", VP)]
+
 
 _SIGS = {
     "th_last_error": (C.c_char_p, []),
@@ -90,6 +109,17 @@ _SIGS = {
     "th_dev_free": (I32, [VP, VP]),
     "th_memcpy_h2d": (I32, [VP, VP, VP, SZ]),
     "th_memcpy_d2h": (I32, [VP, VP, VP, SZ]),
+    "th_group_workspace": (I32, [I64, U32, U32, C.POINTER(SZ)]),
+    "th_group": (I32, [VP, I64, U32, U32, VP, VP, VP, SZ, VP]),
+    "th_route": (I32, [I32, VP, I64, I64, U32, VP, I64, U32, I32, VP, VP, VP, VP, VP, SZ, VP]),
+    "th_route_backward": (I32, [I32, VP, I64, I64, U32, VP, I64, U32, I32, VP, VP, VP, VP, VP]),
+    "th_grouped_matmul": (I32, [C.POINTER(Grouped), VP, I64, VP]),
+    "th_grouped_matmul_backward_workspace": (I32, [C.POINTER(Grouped), C.POINTER(SZ)]),
+    "th_grouped_matmul_backward": (I32, [C.POINTER(Grouped), VP, I64, VP, VP, VP, SZ, VP]),
+    "th_lora_linear_workspace": (I32, [C.POINTER(LoraLinear), I32, C.POINTER(SZ)]),
+    "th_lora_linear": (I32, [C.POINTER(LoraLinear), VP, I64, VP, VP, SZ, VP]),
+    "th_lora_linear_backward_workspace": (I32, [C.POINTER(LoraLinear), C.POINTER(SZ)]),
+    "th_lora_linear_backward": (I32, [C.POINTER(LoraLinear), VP, VP, I64, VP, VP, VP, VP, VP, SZ, VP]),
     "th_ntt_time": (I32, [VP, VP, SZ, U32, I32, I32, C.POINTER(C.c_float)]),
 }
 

@@ -1,0 +1,41 @@
+// Rules on sizes of the plain mixture-of-adapters operators, apart from HIP so
+// that a host program can evaluate them (tests/test_mixture_rules.py).
+#pragma once
+#include <stddef.h>
+#include <stdint.h>
+
+namespace th {
+
+constexpr uint32_t MIX_MAX_EXPERTS = 1024;  // the slot counters of a workgroup: 16 wavefronts x 1025 words of LDS
+constexpr uint32_t MIX_MAX_CHOICES = 32;
+constexpr uint32_t MIX_MAX_RANK = 128;      // eight 16-row tiles of an adapter held by one workgroup
+
+constexpr uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
+
+// Tokens whose (token, choice) slots one workgroup of 1024 threads groups: up
+// to 4096 slots, fewer (from 1024) while that gives more workgroups than 128.
+// One workgroup alone needs no second launch, so up to 2048 slots stay whole.
+constexpr uint64_t group_chunk_tokens(uint64_t tokens, uint32_t k) {
+  const uint64_t slots = tokens * k;
+  uint64_t chunk = slots <= 2048 ? 2048 : ceil_div(slots, 128);
+  chunk = chunk < 1024 ? 1024 : chunk > 4096 ? 4096 : chunk;
+  const uint64_t t = chunk / k;
+  return t ? t : 1;
+}
+constexpr uint64_t group_chunks(uint64_t tokens, uint32_t k) {
+  return tokens ? ceil_div(tokens, group_chunk_tokens(tokens, k)) : 1;
+}
+
+// Slots of one partial sum of a low-rank gradient, and how many there are at
+// most: spans of 256 to 2048 slots, doubled while the launch has workgroups to
+// spare (128 columns each).
+constexpr uint32_t lowrank_span(uint64_t slots, uint32_t cols) {
+  uint32_t span = 256;
+  while (span < 2048 && ceil_div(slots, span * 2) * ceil_div(cols, 128) >= 1024) span *= 2;
+  return span;
+}
+constexpr uint64_t lowrank_spans(uint64_t slots, uint32_t E, uint32_t span) {
+  return slots / span + (E < slots ? E : slots);
+}
+
+}  // namespace th
