@@ -486,6 +486,7 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const float* u, const fl
 
 hipError_t launch_mat(MixType type, const MatArgs& a, int transposed, hipStream_t s) {
   if (a.rows == 0 || a.n == 0) return hipSuccess;
+  if (a.scan || (!transposed && th::narrow_product(a.rows, a.n, a.offsets ? a.E : 1))) return launch_narrow(type, a, s);
   return type == MIX_BF16 ? mat_typed<bf16_t>(a, transposed, s) : mat_typed<f16_t>(a, transposed, s);
 }
 

@@ -1,5 +1,6 @@
 // Shared declarations of the plain (unencrypted) mixture-of-adapters operators:
 //   route.hip     softmax gate with top-k, grouping of slots by expert
+//   narrow.hip    matrix products of few output tiles
 //   grouped.hip   matrix products of ragged groups, the shared projection with
 //                 its low-rank adapters, and their gradients
 //   mixture.hip   argument checks, workspaces and the C entry points
@@ -56,6 +57,7 @@ struct MatArgs {
   uint32_t n, k, E, div;        // outputs, contraction length
   int y_float;                  // y holds floats (a workspace)
   int aligned;                  // every row of x and w starts on 16 bytes and k (n, if transposed) is a multiple of 8
+  int scan;                     // no order or offsets: a slot's matrix is ids[slot], rows without one are not written
   // low-rank part: y_t += sum_j c_tj P[id_tj] u_tj over the token's choices
   // with P[e] = `p` + e * ldpe, n x r with row stride ldp
   const void* p;
@@ -68,6 +70,7 @@ struct MatArgs {
 };
 // w is n x k (transposed = 0: y = x w^T) or k x n (1: y = x w).
 hipError_t launch_mat(MixType type, const MatArgs& a, int transposed, hipStream_t s);
+hipError_t launch_narrow(MixType type, const MatArgs& a, hipStream_t s);  // w as n x k; launch_mat's choice
 
 // out[g] = sum over the slots s of group g of left[s] (outer) right[s / div]:
 // n x k per group, with left row s of dy (n values), right row s / div of x (k).

@@ -115,9 +115,14 @@ struct LoraWork {
   float *u = nullptr, *v = nullptr, *partial = nullptr;
   uint16_t *at = nullptr, *bt = nullptr;
 };
-LoraWork lay_groups(Pieces& p, const th_lora_linear_args* d) {
+// Few slots that nothing else needs grouped: the low-rank product finds each
+// adapter's slots by itself.
+bool scans(const th_lora_linear_args* d, bool keep_u) {
+  return !d->order && !keep_u && (uint64_t)d->tokens * d->choices <= th::NARROW_SCAN_SLOTS;
+}
+LoraWork lay_groups(Pieces& p, const th_lora_linear_args* d, bool own_lists = false) {
   LoraWork w;
-  if (!d->order) {
+  if (!d->order && !own_lists) {
     w.order = p.take<int32_t>((uint64_t)d->tokens * d->choices);
     w.offsets = p.take<int32_t>(d->adapters + 1);
     w.hist = p.take<uint32_t>(hist_words(d->tokens, d->adapters, d->choices));
@@ -125,7 +130,7 @@ LoraWork lay_groups(Pieces& p, const th_lora_linear_args* d) {
   return w;
 }
 LoraWork lay_forward(Pieces& p, const th_lora_linear_args* d, bool keep_u) {
-  LoraWork w = lay_groups(p, d);
+  LoraWork w = lay_groups(p, d, scans(d, keep_u));
   if (!keep_u) w.u = p.take<float>((uint64_t)d->tokens * d->choices * padded_rank(d->rank));
   return w;
 }
@@ -165,6 +170,8 @@ void make_groups(const th_lora_linear_args* d, LoraWork& w, hipStream_t s) {
 void shrink(const th_lora_linear_args* d, const LoraWork& w, const void* wide, int64_t ldwide, uint32_t width,
             const void* factor, int64_t ldf, int64_t ldfe, float* low, hipStream_t s) {
   MatArgs m{};
+  m.scan = w.offsets == nullptr;
+  m.ids = d->experts;
   m.x = wide;
   m.ldx = ldwide;
   m.w = factor;
@@ -389,7 +396,7 @@ int th_lora_linear(const th_lora_linear_args* d, void* y, int64_t ldy, float* u,
     if (d->tokens == 0) return;
     const hipStream_t s = (hipStream_t)stream;
     float* low = u ? u : w.u;
-    make_groups(d, w, s);
+    if (!scans(d, u != nullptr)) make_groups(d, w, s);
     shrink(d, w, d->x, d->ldx, d->d_in, d->a, d->lda, d->lda_adapter, low, s);
     MatArgs m{};
     m.x = d->x;
