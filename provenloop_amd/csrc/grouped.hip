@@ -1,248 +1,8 @@
-// Matrix products of ragged groups and of the shared projection with its
-// low-rank adapters, y = x w^T or x w, on the matrix cores.
+// Gradients of grouped weights and of low-rank factors: products whose
+// contraction runs over a group's slots.
 #include "mixture_device.h"
 
 namespace {
-
-constexpr int BK = 64;  // contraction steps of one LDS tile: 128 bytes a row
-
-// The low-rank part of one wavefront's TM x TN outputs: one pass per adapter
-// that its rows use, u (float) times the adapter's rows, as bf16 pairs.
-template <class T, int TM, int TN>
-__device__ void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, uint32_t n0, f32x4 (&acc)[TN / 16][TM / 16],
-                            uint32_t lane) {
-  constexpr int HALF = TM < 64 ? TM : 64;
-  for (int h = 0; h < TM / HALF; ++h) {
-    const int64_t row = m0 + h * HALF + lane;
-    const bool valid = lane < HALF && row < mend;
-    uint32_t done = 0;  // lane i: word i of the adapters dealt with
-    for (uint32_t j = 0; j < a.kc; ++j) {
-      const uint32_t id = valid ? (uint32_t)a.ids[row * a.kc + j] : ~0u;
-      const uint32_t word = __shfl(done, id < a.E ? id >> 5 : 0);
-      bool open = id < a.E && !((word >> (id & 31)) & 1);
-      uint64_t pending;
-      while ((pending = __ballot(open))) {
-        const uint32_t e = __builtin_amdgcn_readlane(id, __ffsll((unsigned long long)pending) - 1);
-        if (lane == e >> 5) done |= 1u << (e & 31);
-        if (id == e) open = false;
-        // the row's first choice of this adapter, and its coefficient there
-        int at = -1;
-        float c = 0;
-        if (valid)
-          for (uint32_t i = 0; i < a.kc; ++i)
-            if ((uint32_t)a.ids[row * a.kc + i] == e) {
-              if (at < 0) at = (int)i;
-              c += a.gate ? a.gate[row * a.kc + i] : 1.0f;
-            }
-        if (a.scale) c *= a.scale[e];
-        const T* pe = (const T*)a.p + (int64_t)e * a.ldpe;
-        for (uint32_t r0 = 0; r0 < a.r; r0 += 32) {
-          const int rr = (int)(r0 + lane / 16 * 8);
-          const int rv = (int)a.r - rr;
-          decltype(widen(vec8<T>())) pf[TN / 16];
-          for (int ni = 0; ni < TN / 16; ++ni) {
-            const uint32_t n = min(n0 + ni * 16 + lane % 16, a.n - 1);
-            pf[ni] = widen(load8<T>(pe + (int64_t)n * a.ldp + (rv > 0 ? rr : 0), rv));
-          }
-          for (int mi = 0; mi < HALF / 16; ++mi) {
-            const int src = mi * 16 + lane % 16;
-            const int ju = __shfl(at, src);
-            const float cu = __shfl(c, src);
-            f32x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-            if (ju >= 0) {
-              const float* u = a.u + ((m0 + h * HALF + src) * a.kc + ju) * a.ru + rr;
-              for (int i = 0; i < 8; ++i)
-                if (i < rv) v[i] = cu * u[i];
-            }
-            bf16x8 hi, lo;
-            split8(v, hi, lo);
-            for (int ni = 0; ni < TN / 16; ++ni)
-              acc[ni][h * (HALF / 16) + mi] = mfma_split(pf[ni], hi, lo, acc[ni][h * (HALF / 16) + mi]);
-          }
-        }
-      }
-    }
-  }
-}
-
-// BM x BN outputs per workgroup of WM x WN wavefronts. Tiles of x (BM rows of
-// 64 contraction steps) and of w in LDS, two of each: one is loaded while the
-// other is multiplied. w's tile is BN rows of 64 steps, or, for y = x w, 64
-// rows of BN columns read through the transposing LDS read.
-template <class T, int BM, int BN, int WM, int WN, bool TR, bool ALIGNED, bool LR>
-__global__ void __launch_bounds__(64 * WM * WN) mat_kernel(MatArgs a) {
-  constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN;
-  constexpr int AJ = BM / 8 / WAVES, BJ = BN / 8 / WAVES;  // 1 KiB loads per wavefront and tile
-  constexpr uint32_t STAGE = (BM + BN) * BK * 2;
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
-  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const uint32_t wm = wave / WN, wn = wave % WN;
-
-  // ---- which rows and columns
-  const uint32_t ntiles = (a.n + BN - 1) / BN;
-  const bool grouped = a.offsets != nullptr;
-  const uint32_t mtiles = grouped ? count_group_tiles(a.offsets, a.E, a.E + 1, a.rows, BM, lane)
-                                  : (uint32_t)((a.rows + BM - 1) / BM);
-  const uint32_t total = mtiles * ntiles;
-  if (blockIdx.x >= total) return;
-  // bands of 8 row tiles, column tiles outside, so that both stay in an L2
-  const uint32_t tile = xcd_tile(blockIdx.x, total);
-  const uint32_t band = tile / (8 * ntiles), in = tile % (8 * ntiles), height = min(8u, mtiles - band * 8);
-  const uint32_t mt = band * 8 + in % height, n0 = in / height * BN;
-  GroupTile g{0, (int64_t)mt * BM, min((int64_t)(mt + 1) * BM, a.rows)};
-  if (grouped) g = find_group_tile(a.offsets, a.E, a.E + 1, a.rows, BM, mt, lane);
-  if (g.begin >= g.end) return;
-  auto slot_of = [&](int64_t i) {  // sorted position -> row of y
-    i = min(i, g.end - 1);
-    return a.order ? min((int64_t)(uint32_t)a.order[i], a.rows - 1) : i;
-  };
-
-  f32x4 acc[TN / 16][TM / 16];
-  for (int i = 0; i < TN / 16; ++i)
-    for (int j = 0; j < TM / 16; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
-
-  if (!grouped || g.group < a.E) {
-    const T* w = (const T*)a.w + (grouped ? (int64_t)g.group * a.ldwe : 0);
-    const char* zero = (const char*)&mix_zero16;
-    // ---- this lane's 16-byte pieces of both tiles
-    const T* xp[AJ];
-    const T* wp[BJ];
-    uint32_t xk = (lane % 8) ^ (lane / 8);  // chunk of the row: chunk c of row i lies at c ^ (i % 8)
-    xk *= 8;
-    for (int j = 0; j < AJ; ++j) {
-      const int64_t s = slot_of(g.begin + (wave * AJ + j) * 8 + lane / 8);
-      xp[j] = (const T*)a.x + s / a.div * a.ldx + xk;
-    }
-    constexpr int ROWC = BN / 8;  // chunks of a row of the transposed tile
-    uint32_t wk[BJ], wc[BJ];      // contraction step, and columns left, of each piece
-    for (int j = 0; j < BJ; ++j) {
-      if (TR) {
-        const uint32_t row = (wave * BJ + j) * (64 / ROWC) + lane / ROWC;
-        const uint32_t col = n0 + ((lane % ROWC) ^ tr_swizzle<BN>(row)) * 8;
-        wk[j] = row;
-        wc[j] = col < a.n ? a.n - col : 0;
-        wp[j] = w + (int64_t)row * a.ldw + min(col, a.n - 1);
-      } else {
-        const uint32_t row = min(n0 + (wave * BJ + j) * 8 + lane / 8, a.n - 1);
-        wk[j] = xk;
-        wc[j] = 8;
-        wp[j] = w + (int64_t)row * a.ldw + xk;
-      }
-    }
-    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds));
-    vec8<T> rx[ALIGNED ? 1 : AJ], rw[ALIGNED ? 1 : BJ];
-    auto fetch = [&](uint32_t k0, uint32_t stage) {
-      if constexpr (ALIGNED) {
-        const uint32_t base = lds0 + stage * STAGE;
-        const bool whole = k0 + BK <= a.k;
-        for (int j = 0; j < AJ; ++j) {
-          const void* p = xp[j] + k0;
-          if (!whole && k0 + xk >= a.k) p = zero;
-          load_lds16(p, base + (wave * AJ + j) * 1024);
-        }
-        for (int j = 0; j < BJ; ++j) {
-          const void* p = wp[j] + (TR ? (int64_t)k0 * a.ldw : (int64_t)k0);
-          if ((!whole && k0 + wk[j] >= a.k) || (TR && wc[j] == 0)) p = zero;
-          load_lds16(p, base + BM * BK * 2 + (wave * BJ + j) * 1024);
-        }
-      } else {
-        for (int j = 0; j < AJ; ++j) {
-          const int64_t left = (int64_t)a.k - (k0 + xk);
-          rx[j] = load8<T>(left > 0 ? xp[j] + k0 : (const T*)zero, left);
-        }
-        for (int j = 0; j < BJ; ++j) {
-          const int64_t left = (int64_t)a.k - (k0 + wk[j]);
-          const T* p = wp[j] + (TR ? (int64_t)k0 * a.ldw : (int64_t)k0);
-          const int64_t valid = TR ? (left > 0 ? (int64_t)wc[j] : 0) : left;
-          rw[j] = load8<T>(valid > 0 ? p : (const T*)zero, valid);
-        }
-      }
-    };
-    auto commit = [&](uint32_t stage) {
-      if constexpr (!ALIGNED) {
-        char* base = lds + stage * STAGE + lane * 16;
-        for (int j = 0; j < AJ; ++j) *(vec8<T>*)(base + (wave * AJ + j) * 1024) = rx[j];
-        for (int j = 0; j < BJ; ++j) *(vec8<T>*)(base + BM * BK * 2 + (wave * BJ + j) * 1024) = rw[j];
-      }
-    };
-    fetch(0, 0);
-    commit(0);
-    uint32_t stage = 0;
-    for (uint32_t k0 = 0; k0 < a.k; k0 += BK, stage ^= 1) {
-      arrived_barrier();
-      const bool more = k0 + BK < a.k;
-      if (more) fetch(k0 + BK, stage ^ 1);
-      const char* xt = lds + stage * STAGE;
-      const char* wt = xt + BM * BK * 2;
-      for (int kk = 0; kk < BK / 32; ++kk) {
-        vec8<T> xf[TM / 16], wf[TN / 16];
-        const uint32_t chunk = kk * 4 + lane / 16;
-        for (int mi = 0; mi < TM / 16; ++mi) {
-          const uint32_t row = wm * TM + mi * 16 + lane % 16;
-          xf[mi] = *(const vec8<T>*)(xt + row * 128 + (chunk ^ (row & 7)) * 16);
-        }
-        for (int ni = 0; ni < TN / 16; ++ni) {
-          if (TR) {
-            wf[ni] = tr_fragment<T, BN>(wt, wn * TN + ni * 16, kk * 32, lane);
-          } else {
-            const uint32_t row = wn * TN + ni * 16 + lane % 16;
-            wf[ni] = *(const vec8<T>*)(wt + row * 128 + (chunk ^ (row & 7)) * 16);
-          }
-        }
-        for (int ni = 0; ni < TN / 16; ++ni)
-          for (int mi = 0; mi < TM / 16; ++mi) acc[ni][mi] = mfma(wf[ni], xf[mi], acc[ni][mi]);
-      }
-      if (more) commit(stage ^ 1);
-    }
-    if (LR) add_lowrank<T, TM, TN>(a, g.begin + wm * TM, g.end, n0 + wn * TN, acc, lane);
-  }
-
-  // ---- out: a lane holds 4 neighbouring columns of one row
-  for (int mi = 0; mi < TM / 16; ++mi) {
-    const int64_t i = g.begin + wm * TM + mi * 16 + lane % 16;
-    if (i >= g.end) continue;
-    const int64_t s = slot_of(i);
-    for (int ni = 0; ni < TN / 16; ++ni) {
-      const uint32_t n = n0 + wn * TN + ni * 16 + lane / 16 * 4;
-      if (n >= a.n) continue;
-      f32x4 v = acc[ni][mi];
-      if (a.bias)
-        for (int q = 0; q < 4; ++q)
-          if (n + q < a.n) v[q] += to_float(((const T*)a.bias)[n + q]);
-      if (a.y_float) {
-        float* y = (float*)a.y + s * a.ldy + n;
-        for (int q = 0; q < 4; ++q)
-          if (n + q < a.n) y[q] = v[q];
-      } else {
-        T* y = (T*)a.y + s * a.ldy + n;
-        if (n + 4 <= a.n && a.ldy % 4 == 0) {
-          T o[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
-          *(uint64_t*)y = __builtin_bit_cast(uint64_t, o);
-        } else {
-          for (int q = 0; q < 4; ++q)
-            if (n + q < a.n) y[q] = (T)v[q];
-        }
-      }
-    }
-  }
-}
-
-template <class T, int BM, int BN, int WM, int WN, bool TR, bool ALIGNED>
-hipError_t run_mat(const MatArgs& a, hipStream_t s) {
-  const uint64_t groups = a.offsets ? (uint64_t)min((int64_t)a.E + 1, a.rows) : 0;
-  const uint64_t tiles = (a.offsets ? a.rows / BM + groups : th::ceil_div(a.rows, BM)) * th::ceil_div(a.n, BN);
-  constexpr uint32_t bytes = 2 * (BM + BN) * BK * 2;
-  if (a.u) mat_kernel<T, BM, BN, WM, WN, TR, ALIGNED, true><<<(uint32_t)tiles, 64 * WM * WN, bytes, s>>>(a);
-  else mat_kernel<T, BM, BN, WM, WN, TR, ALIGNED, false><<<(uint32_t)tiles, 64 * WM * WN, bytes, s>>>(a);
-  return hipGetLastError();
-}
-
-template <class T>
-hipError_t mat_typed(const MatArgs& a, int transposed, hipStream_t s) {
-  if (a.aligned)
-    return transposed ? run_mat<T, 128, 128, 2, 2, true, true>(a, s) : run_mat<T, 128, 128, 2, 2, false, true>(a, s);
-  return transposed ? run_mat<T, 128, 128, 2, 2, true, false>(a, s) : run_mat<T, 128, 128, 2, 2, false, false>(a, s);
-}
 
 // ---------------------------------------------------------------- weight gradients
 // 128 x 128 outputs of one group: both operands are rows of slots, 64 slots a
@@ -483,12 +243,6 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const float* u, const fl
 }
 
 }  // namespace
-
-hipError_t launch_mat(MixType type, const MatArgs& a, int transposed, hipStream_t s) {
-  if (a.rows == 0 || a.n == 0) return hipSuccess;
-  if (a.scan || (!transposed && th::narrow_product(a.rows, a.n, a.offsets ? a.E : 1))) return launch_narrow(type, a, s);
-  return type == MIX_BF16 ? mat_typed<bf16_t>(a, transposed, s) : mat_typed<f16_t>(a, transposed, s);
-}
 
 hipError_t launch_outer(MixType type, const OuterArgs& a, hipStream_t s) {
   const uint64_t blocks = th::ceil_div(a.n, 128) * th::ceil_div(a.k, 128) * a.E;

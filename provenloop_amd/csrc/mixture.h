@@ -1,8 +1,8 @@
 // Shared declarations of the plain (unencrypted) mixture-of-adapters operators:
 //   route.hip     softmax gate with top-k, grouping of slots by expert
 //   narrow.hip    matrix products of few output tiles
-//   grouped.hip   matrix products of ragged groups, the shared projection with
-//                 its low-rank adapters, and their gradients
+//   wide.hip      large ones, of ragged groups or with low-rank adapters added
+//   grouped.hip   weight gradients of groups and of low-rank factors
 //   mixture.hip   argument checks, workspaces and the C entry points
 // They know nothing of a CKKS context: each call runs on the stream it is
 // given, in memory its caller owns.

@@ -53,6 +53,14 @@ constexpr bool narrow_product(uint64_t rows, uint32_t n, uint32_t groups) {
   const uint64_t each = ceil_div(rows, groups);
   return groups * ceil_div(each, 128) * ceil_div(n, 128) < 128 || each <= 32;
 }
+// The wide products' tile: 256 x 256 or 256 x 128. A CU holds one workgroup of
+// either; a square tile takes 1.75 times as long as the other (8192^3: 3.4 us
+// a 1000 steps of 2 tiles against ...), so it is better where the number of
+// rounds over the 256 CUs allows it.
+constexpr bool wide_square(uint64_t rows, uint32_t n, uint32_t groups) {
+  const uint64_t m = groups * ceil_div(ceil_div(rows, groups), 256);
+  return ceil_div(m * ceil_div(n, 256), 256) * 7 <= ceil_div(m * ceil_div(n, 128), 256) * 4;
+}
 // Slots whose adapters a workgroup of the low-rank product looks through by
 // itself, which saves the launch that would group them.
 constexpr uint32_t NARROW_SCAN_SLOTS = 2048;
