@@ -1,14 +1,160 @@
 // Gradients of grouped weights and of low-rank factors: products whose
 // contraction runs over a group's slots.
-#include "mixture_device.h"
+#include "wide_kernel.h"
+
+using namespace mix;
 
 namespace {
 
 // ---------------------------------------------------------------- weight gradients
-// 128 x 128 outputs of one group: both operands are rows of slots, 64 slots a
-// step, read through the transposing LDS read.
-template <class T, bool ALIGNED>
-__global__ void __launch_bounds__(256) outer_kernel(OuterArgs a) {
+// The group that comes n-th by its number of slots, most first (of up to 256;
+// further ones in their own order): the long contractions then start first and
+// the short ones fill the CUs that the last of them leave.
+__device__ uint32_t nth_longest(const int32_t* offsets, uint32_t E, int64_t slots, uint32_t n, uint32_t lane) {
+  if (E > 256) return n;
+  uint32_t size[4], rank[4] = {0, 0, 0, 0};
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint32_t g = c * 64 + lane;
+    size[c] = 0;
+    if (g < E) {
+      const int64_t d = group_begin(offsets, g + 1, E, slots) - group_begin(offsets, g, E, slots);
+      size[c] = d > 0 ? (uint32_t)d : 0;
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q)
+    for (uint32_t l = 0; l < 64 && q * 64 + l < E; ++l) {
+      const uint32_t other = __builtin_amdgcn_readlane(size[q], l), g = q * 64 + l;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) rank[c] += other > size[c] || (other == size[c] && g < c * 64 + lane);
+    }
+  uint32_t found = n;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const uint64_t here = __ballot(c * 64 + lane < E && rank[c] == n);
+    if (here) found = c * 64 + __ffsll((unsigned long long)here) - 1;
+  }
+  return found;
+}
+
+// B x B outputs of one group, WM x WN wavefronts: both operands are rows of
+// slots, 64 slots a tile, read through the transposing LDS read. Two tiles in
+// LDS or on their way, a tile's halves passing through registers as in the wide
+// products (wide_kernel.h); the slots' numbers are loaded a tile ahead of them.
+template <class T, int B, int WM, int WN>
+__global__ void __launch_bounds__(64 * WM * WN) outer_kernel(OuterArgs a) {
+  constexpr int WAVES = WM * WN, TM = B / WM, TN = B / WN, MI = TM / 16, NI = TN / 16;
+  constexpr int JOBS = B / 8 / WAVES;                    // 1 KiB loads of an operand per wavefront and tile
+  constexpr int CHUNKS = B / 8, PER = 64 / CHUNKS;       // 16-byte pieces of a row, rows of a load
+  constexpr uint32_t TILE = B * 128, STAGE = 2 * TILE;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const uint32_t wm = wave / WN, wn = wave % WN;
+  const uint32_t nt = (a.n + B - 1) / B, kt = (a.k + B - 1) / B;
+  // every group's tiles in 8 rectangles, one for each XCD, whose L2 then serves each of its rows and columns once; groups
+  // differ in their slots, so an XCD must not have a group to itself
+  const uint32_t gn = nt >= kt ? 4 : 2, gk = 8 / gn, hn = (nt + gn - 1) / gn, hk = (kt + gk - 1) / gk;
+  const uint32_t xcd = blockIdx.x % 8, at8 = blockIdx.x / 8, in = at8 % (hn * hk);
+  const uint32_t n0 = (xcd % gn * hn + in % hn) * B, c0 = (xcd / gn * hk + in / hn) * B;
+  if (in % hn + xcd % gn * hn >= nt || in / hn + xcd / gn * hk >= kt) return;
+  const uint32_t e = nth_longest(a.offsets, a.E, a.slots, at8 / (hn * hk), lane);
+  const int64_t begin = group_begin(a.offsets, e, a.E, a.slots), end = group_begin(a.offsets, e + 1, a.E, a.slots);
+  const char* zero = (const char*)&mix_zero16;
+  f32x4 acc[NI][MI];
+#pragma unroll
+  for (int i = 0; i < NI; ++i)
+#pragma unroll
+    for (int j = 0; j < MI; ++j) acc[i][j] = f32x4{0, 0, 0, 0};
+
+  const uint32_t tiles = begin < end ? (uint32_t)((end - begin + 63) / 64) : 0;
+  if (tiles) {
+    const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)) + wave * JOBS * 1024;
+    uint32_t slot[JOBS];  // of this lane's rows of the tile that is loaded next, ~0 past the group
+    const uint32_t row0 = wave * JOBS * PER + lane / CHUNKS;
+    auto look = [&](uint32_t i) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < JOBS; ++j) {
+        const int64_t at = begin + (int64_t)i * 64 + row0 + j * PER;
+        slot[j] = at < end ? (uint32_t)a.order[at] : ~0u;
+      }
+    };
+    // the numbers have arrived here, before any load that would be waited for with them
+    auto looked = [&]() __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < JOBS; ++j) asm volatile("" ::"v"(slot[j]));
+    };
+    auto load = [&](int j, uint32_t stage) __attribute__((always_inline)) {
+      const uint32_t s = slot[j % JOBS];
+      const uint32_t c = ((lane % CHUNKS) ^ tr_swizzle<B>(row0 + j % JOBS * PER)) * 8;
+      const void* p = zero;
+      if (j < JOBS) {
+        if (s < (uint64_t)a.slots && n0 + c < a.n) p = (const T*)a.dy + (int64_t)s * a.lddy + (n0 + c);
+      } else {
+        if (s < (uint64_t)a.slots && c0 + c < a.k) p = (const T*)a.x + (int64_t)(s / a.div) * a.ldx + (c0 + c);
+      }
+      load_lds16(p, lds0 + stage * STAGE + (j < JOBS ? 0 : TILE) + j % JOBS * 1024);
+    };
+    vec8<T> fa[2][MI], fb[2][NI];
+    auto half = [&](int set, bool reads, uint32_t stage, int kk, bool loads, uint32_t to)
+        __attribute__((always_inline)) {
+#pragma unroll
+      for (int p = 0; p < 8; ++p) {
+        if (reads)
+#pragma unroll
+          for (int f = p * (MI + NI) / 8; f < (p + 1) * (MI + NI) / 8; ++f) {
+            const char* at = lds + stage * STAGE;
+            if (f < NI) fb[set ^ 1][f] = tr_fragment<T, B>(at + TILE, wn * TN + f * 16, kk * 32, lane);
+            else fa[set ^ 1][f - NI] = tr_fragment<T, B>(at, wm * TM + (f - NI) * 16, kk * 32, lane);
+          }
+        if (loads)
+#pragma unroll
+          for (int j = p * JOBS / 4; j < (p + 1) * JOBS / 4; ++j) load(j, to);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int q = p * MI * NI / 8; q < (p + 1) * MI * NI / 8; ++q)
+          acc[q / MI][q % MI] = mfma(fb[set][q / MI], fa[set][q % MI], acc[q / MI][q % MI]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    look(0);
+    looked();
+#pragma unroll
+    for (int j = 0; j < 2 * JOBS; ++j) load(j, 0);
+    look(1);  // past the end: zeros
+    looked();
+#pragma unroll
+    for (int j = 0; j < 2 * JOBS; ++j) load(j, 1);
+    look(2);
+    arrived_barrier();
+#pragma unroll
+    for (int f = 0; f < NI; ++f) fb[0][f] = tr_fragment<T, B>(lds + TILE, wn * TN + f * 16, 0, lane);
+#pragma unroll
+    for (int f = 0; f < MI; ++f) fa[0][f] = tr_fragment<T, B>(lds, wm * TM + f * 16, 0, lane);
+    uint32_t stage = 0;
+    for (uint32_t i = 0; i + 2 < tiles; ++i, stage ^= 1) {
+      half(0, true, stage, 1, false, 0);
+      arrived_barrier();
+      looked();
+      half(1, true, stage ^ 1, 0, true, stage);
+      look(i + 3);
+    }
+    for (uint32_t i = tiles > 2 ? tiles - 2 : 0; i < tiles; ++i, stage ^= 1) {
+      half(0, true, stage, 1, false, 0);
+      arrived_barrier();
+      half(1, i + 1 < tiles, stage ^ 1, 0, false, 0);
+    }
+  }
+  __syncthreads();
+  // rows of the output are dy's columns
+  const Out out{(T*)a.out + ((int64_t)e * a.n + n0) * a.k, a.k, a.k, nullptr};
+  put<T, T, TM, TN>(out, acc, lds + wave * (TM * TN * 2), nullptr, wm * TM, a.n - n0, c0 + wn * TN, lane);
+}
+
+// The same for rows that do not start on 16 bytes or widths that are no
+// multiples of 8: 128 x 128 outputs, tiles through registers.
+template <class T>
+__global__ void __launch_bounds__(256) unaligned_outer_kernel(OuterArgs a) {
   constexpr int BN = 128, JOBS = 4;  // 1 KiB loads (4 slots) per wavefront and tile
   constexpr uint32_t TILE = 64 * BN * 2, STAGE = 2 * TILE;
   extern __shared__ __attribute__((aligned(1024))) char lds[];
@@ -30,7 +176,6 @@ __global__ void __launch_bounds__(256) outer_kernel(OuterArgs a) {
     cn[j] = n0 + c;
     ck[j] = c0 + c;
   }
-  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds));
   int64_t slot[JOBS];  // of the step that is fetched next; -1 past the group
   auto look = [&](int64_t s0) {
     for (int j = 0; j < JOBS; ++j) {
@@ -39,40 +184,34 @@ __global__ void __launch_bounds__(256) outer_kernel(OuterArgs a) {
     }
   };
   vec8<T> rn[JOBS], rk[JOBS];
-  auto fetch = [&](uint32_t stage) {
+  auto fetch = [&]() {
     for (int j = 0; j < JOBS; ++j) {
       const bool inn = slot[j] >= 0 && cn[j] < a.n, ink = slot[j] >= 0 && ck[j] < a.k;
       const T* pn = inn ? (const T*)a.dy + slot[j] * a.lddy + cn[j] : (const T*)zero;
       const T* pk = ink ? (const T*)a.x + slot[j] / a.div * a.ldx + ck[j] : (const T*)zero;
-      if constexpr (ALIGNED) {
-        load_lds16(pn, lds0 + stage * STAGE + (wave * JOBS + j) * 1024);
-        load_lds16(pk, lds0 + stage * STAGE + TILE + (wave * JOBS + j) * 1024);
-      } else {
-        rn[j] = load8<T>(pn, inn ? a.n - cn[j] : 0);
-        rk[j] = load8<T>(pk, ink ? a.k - ck[j] : 0);
-      }
+      rn[j] = load8<T>(pn, inn ? a.n - cn[j] : 0);
+      rk[j] = load8<T>(pk, ink ? a.k - ck[j] : 0);
     }
   };
   auto commit = [&](uint32_t stage) {
-    if constexpr (!ALIGNED)
-      for (int j = 0; j < JOBS; ++j) {
-        char* p = lds + stage * STAGE + (wave * JOBS + j) * 1024 + lane * 16;
-        *(vec8<T>*)p = rn[j];
-        *(vec8<T>*)(p + TILE) = rk[j];
-      }
+    for (int j = 0; j < JOBS; ++j) {
+      char* p = lds + stage * STAGE + (wave * JOBS + j) * 1024 + lane * 16;
+      *(vec8<T>*)p = rn[j];
+      *(vec8<T>*)(p + TILE) = rk[j];
+    }
   };
   if (begin < end) {
     look(begin);
-    fetch(0);
+    fetch();
     commit(0);
     look(begin + 64);
   }
   uint32_t stage = 0;
   for (int64_t s0 = begin; s0 < end; s0 += 64, stage ^= 1) {
-    arrived_barrier();
+    __syncthreads();
     const bool more = s0 + 64 < end;
     if (more) {
-      fetch(stage ^ 1);
+      fetch();
       look(s0 + 128);
     }
     const char* tn = lds + stage * STAGE;
@@ -244,14 +383,21 @@ __global__ void __launch_bounds__(256) gate_grad_kernel(const float* u, const fl
 
 }  // namespace
 
-hipError_t launch_outer(MixType type, const OuterArgs& a, hipStream_t s) {
-  const uint64_t blocks = th::ceil_div(a.n, 128) * th::ceil_div(a.k, 128) * a.E;
-  constexpr uint32_t bytes = 2 * 2 * 64 * 128 * 2;
-  if (type == MIX_BF16 && a.aligned) outer_kernel<bf16_t, true><<<(uint32_t)blocks, 256, bytes, s>>>(a);
-  else if (type == MIX_BF16) outer_kernel<bf16_t, false><<<(uint32_t)blocks, 256, bytes, s>>>(a);
-  else if (a.aligned) outer_kernel<f16_t, true><<<(uint32_t)blocks, 256, bytes, s>>>(a);
-  else outer_kernel<f16_t, false><<<(uint32_t)blocks, 256, bytes, s>>>(a);
+template <class T>
+static hipError_t outer_typed(const OuterArgs& a, hipStream_t s) {
+  if (!a.aligned) {
+    const uint64_t blocks = th::ceil_div(a.n, 128) * th::ceil_div(a.k, 128) * a.E;
+    unaligned_outer_kernel<T><<<(uint32_t)blocks, 256, 2 * 2 * 64 * 128 * 2, s>>>(a);
+    return hipGetLastError();
+  }
+  constexpr uint32_t B = 128;
+  const uint64_t nt = th::ceil_div(a.n, B), kt = th::ceil_div(a.k, B), gn = nt >= kt ? 4 : 2, gk = 8 / gn;
+  const uint64_t blocks = 8 * th::ceil_div(nt, gn) * th::ceil_div(kt, gk) * a.E;
+  outer_kernel<T, B, 2, 4><<<(uint32_t)blocks, 512, 2 * 2 * B * 128, s>>>(a);
   return hipGetLastError();
+}
+hipError_t launch_outer(MixType type, const OuterArgs& a, hipStream_t s) {
+  return type == MIX_BF16 ? outer_typed<bf16_t>(a, s) : outer_typed<f16_t>(a, s);
 }
 
 hipError_t launch_low_outer(MixType type, LowOuterArgs a, hipStream_t s) {

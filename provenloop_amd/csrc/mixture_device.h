@@ -90,6 +90,14 @@ __device__ inline void arrived_barrier() {
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
+// The same for this wavefront alone: at most N loads into LDS are under way;
+// its LDS reads have been answered.
+template <int N>
+__device__ inline void arrived(void) {
+  asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+__device__ inline void answered(void) { asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory"); }
+
 __device__ inline uint32_t lds_address(const void* p) {
   return (uint32_t)(uintptr_t)(__attribute__((address_space(3))) const void*)p;
 }

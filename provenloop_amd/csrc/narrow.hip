@@ -3,24 +3,26 @@
 //
 // What bounds them is the latency of reading w (a decode reads each weight for
 // a few rows) and how many CUs take part, not the matrix cores. So a workgroup
-// takes a small tile (16 to 64 rows by 16 or 32 columns), its 8 wavefronts split
-// the contraction among them, and operands go straight from memory into
-// registers in the matrix instructions' layout, several 128-byte lines of each
-// row in flight a wavefront; the wavefronts' sums meet in LDS, added in order.
+// takes a small tile (16 or 32 rows by 16 or 32 columns), and its wavefronts
+// split the contraction among them: a wavefront's step is one 128-byte line (64
+// values) of every row. Each has a ring of lines of its own in LDS, filled by
+// asynchronous loads of whole lines and waited for by that wavefront alone, so
+// nothing but the last sum, in LDS and in order, needs a barrier. Measured
+// against operands loaded into registers in the matrix instructions' layout
+// (16 rows by 64 bytes a load): 32 x 3584 x 3584 6.7 us against 13.2, 250 x 1536
+// x 1536 6.7 against 12.3, 8192 x 32 x 3584 10.8 against 16.8; one row of 1536 x
+// 1536 2.8 against 4.4.
 //
-// A wavefront's step is one 128-byte line (64 values) of every row: lane l reads
-// 32 bytes of row l % 16 from (l / 16) * 32 on, two matrix instructions' worth.
-// The contraction steps are thereby taken in another order than memory's, the
-// same for both operands.
+// Operands whose rows do not start on 16 bytes go through registers, 32 bytes a
+// lane from (l / 16) * 32 on in a line, two matrix instructions' worth; the
+// contraction is then taken in another order, the same for both operands.
 //
 // The low-rank part of the shared projection is a dot product of `rank` floats
 // per output and choice, in ordinary float arithmetic: rows of a small batch
-// seldom share an adapter, and the loads run under the weights'.
+// seldom share an adapter.
 #include "mixture_device.h"
 
 namespace {
-
-constexpr int WAVES = 8, THREADS = 64 * WAVES;
 
 template <class T>
 __device__ __forceinline__ float lowrank_at(const MatArgs& a, int64_t row, uint32_t n) {
@@ -47,13 +49,21 @@ __device__ __forceinline__ float lowrank_at(const MatArgs& a, int64_t row, uint3
   return sum;
 }
 
-template <class T, int MT, int NT, bool ALIGNED, bool LR>
-__global__ void __launch_bounds__(THREADS) narrow_kernel(MatArgs a, uint32_t shares) {
-  constexpr int BM = 16 * MT, BN = 16 * NT, LD = BN + 4;
-  constexpr int U = MT * NT == 1 ? 4 : MT * NT == 2 ? 3 : MT * NT == 4 ? 2 : 1;  // lines of a row, twice, in registers
+template <int MT, int NT, int WAVES, int S>
+constexpr uint32_t narrow_lds() {
+  const uint32_t rings = WAVES * S * 16 * (MT + NT) * 128, sums = WAVES * 16 * MT * (16 * NT + 4) * 4;
+  return rings > sums ? rings : sums;
+}
+
+// 16 MT rows by 16 NT columns, WAVES wavefronts, S lines of each row in a ring.
+template <class T, int MT, int NT, int WAVES, int S, bool ALIGNED, bool LR>
+__global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t shares) {
+  constexpr int BM = 16 * MT, BN = 16 * NT, LD = BN + 4, THREADS = 64 * WAVES;
   constexpr int OUTS = BM * BN / THREADS ? BM * BN / THREADS : 1;
-  extern __shared__ __attribute__((aligned(16))) char lds[];
-  float* red = (float*)lds;                       // WAVES x BM x LD
+  constexpr int LOADS = 2 * (MT + NT);             // of a line of every row, 8 rows each
+  constexpr uint32_t STAGE = (BM + BN) * 128;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  float* red = (float*)lds;                        // WAVES x BM x LD, after the rings
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const uint32_t ntiles = (a.n + BN - 1) / BN;
 
@@ -61,7 +71,7 @@ __global__ void __launch_bounds__(THREADS) narrow_kernel(MatArgs a, uint32_t sha
   const bool scan = a.scan, grouped = a.offsets != nullptr;
   GroupTile g{0, 0, 0};
   uint32_t n0, share = 0;
-  int32_t* list = (int32_t*)(red + WAVES * BM * LD);  // scan: this group's slots
+  int32_t* list = (int32_t*)(lds + narrow_lds<MT, NT, WAVES, S>());  // scan: this group's slots
   uint32_t listed = 0;
   if (scan) {
     // workgroup (column tile, group, share): the group's slots by looking at every slot's
@@ -106,80 +116,123 @@ __global__ void __launch_bounds__(THREADS) narrow_kernel(MatArgs a, uint32_t sha
   const bool has = !grouped || g.group < a.E;
   const T* w = (const T*)a.w + (grouped || scan ? (int64_t)g.group * a.ldwe : 0);
   const T* zero = (const T*)&mix_zero16;
-  const uint32_t kl = lane / 16 * 16;  // this lane's 16 values of a line
-  const uint32_t lines = (a.k + 63) / 64;
-  const T* wp[NT];
-  for (int ni = 0; ni < NT; ++ni) wp[ni] = w + (int64_t)min(n0 + ni * 16 + lane % 16, a.n - 1) * a.ldw + kl;
+  const uint32_t lines = has ? (a.k + 63) / 64 : 0;
+  const uint32_t mine = wave < lines ? (lines - wave + WAVES - 1) / WAVES : 0;  // this wavefront's: wave + i WAVES
 
   for (int64_t m0 = g.begin; m0 < g.end; m0 += (int64_t)shares * BM) {
-    const T* xp[MT];
-    for (int mi = 0; mi < MT; ++mi) xp[mi] = (const T*)a.x + slot_of(m0 + mi * 16 + lane % 16) / a.div * a.ldx + kl;
     f32x4 acc[NT][MT];
+#pragma unroll
     for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
       for (int mi = 0; mi < MT; ++mi) acc[ni][mi] = f32x4{0, 0, 0, 0};
-    struct Step {
-      vec8<T> x[U][MT][2], w[U][NT][2];
-    };
-    auto piece = [&](const T* p, int64_t left) __attribute__((always_inline)) -> vec8<T> {
-      if constexpr (ALIGNED) return *(const vec8<T>*)(left > 0 ? p : zero);
-      else return load8<T>(left > 0 ? p : zero, left);
-    };
-    // a line that ends within the contraction, or is past it, reads zeros there
-    auto fetch = [&](Step& s, uint32_t line) __attribute__((always_inline)) {
-      for (int q = 0; q < U; ++q) {
-        const uint32_t k0 = (line + q * WAVES) * 64;
-        if (ALIGNED && k0 + 64 <= a.k) {
-          for (int ni = 0; ni < NT; ++ni)
-            for (int h = 0; h < 2; ++h) s.w[q][ni][h] = *(const vec8<T>*)(wp[ni] + k0 + h * 8);
-          for (int mi = 0; mi < MT; ++mi)
-            for (int h = 0; h < 2; ++h) s.x[q][mi][h] = *(const vec8<T>*)(xp[mi] + k0 + h * 8);
-        } else {
-          for (int h = 0; h < 2; ++h) {
-            const int64_t left = (int64_t)a.k - (k0 + kl + h * 8);
-            for (int ni = 0; ni < NT; ++ni) s.w[q][ni][h] = piece(wp[ni] + k0 + h * 8, left);
-            for (int mi = 0; mi < MT; ++mi) s.x[q][mi][h] = piece(xp[mi] + k0 + h * 8, left);
+    if constexpr (ALIGNED) {
+      const uint32_t xk = ((lane % 8) ^ (lane / 8)) * 8;  // chunk c of row i lies at c ^ (i % 8)
+      const T* p[LOADS];
+#pragma unroll
+      for (int j = 0; j < LOADS; ++j)
+        p[j] = j < 2 * MT ? (const T*)a.x + slot_of(m0 + j * 8 + lane / 8) / a.div * a.ldx + xk
+                          : w + (int64_t)min(n0 + (j - 2 * MT) * 8 + lane / 8, a.n - 1) * a.ldw + xk;
+      const char* ring = lds + wave * (S * STAGE);
+      const uint32_t base = __builtin_amdgcn_readfirstlane(lds_address(ring));
+      auto load = [&](uint32_t i, uint32_t stage) __attribute__((always_inline)) {
+        const uint32_t k0 = (wave + i * WAVES) * 64;
+#pragma unroll
+        for (int j = 0; j < LOADS; ++j) load_lds16(k0 + xk < a.k ? p[j] + k0 : zero, base + stage * STAGE + j * 1024);
+      };
+#pragma unroll
+      for (int i = 0; i < S; ++i)
+        if (i < (int)mine) load(i, i);
+      uint32_t stage = 0;
+      for (uint32_t i = 0; i < mine; ++i) {
+        if (i + S <= mine) arrived<(S - 1) * LOADS>();
+        else arrived<0>();
+        const char *xt = ring + stage * STAGE, *wt = xt + BM * 128;
+        vec8<T> xf[2][MT], wf[2][NT];
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk) {
+          const uint32_t c = kk * 4 + lane / 16;
+#pragma unroll
+          for (int mi = 0; mi < MT; ++mi) {
+            const uint32_t r = mi * 16 + lane % 16;
+            xf[kk][mi] = *(const vec8<T>*)(xt + r * 128 + (c ^ (r & 7)) * 16);
+          }
+#pragma unroll
+          for (int ni = 0; ni < NT; ++ni) {
+            const uint32_t r = ni * 16 + lane % 16;
+            wf[kk][ni] = *(const vec8<T>*)(wt + r * 128 + (c ^ (r & 7)) * 16);
           }
         }
-      }
-    };
-    auto multiply = [&](const Step& s) __attribute__((always_inline)) {
-      for (int q = 0; q < U; ++q)
-        for (int h = 0; h < 2; ++h)
+        answered();  // the stage has been read before its place is loaded again
+        if (i + S < mine) load(i + S, stage);
+        stage = stage + 1 == S ? 0 : stage + 1;
+#pragma unroll
+        for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
           for (int ni = 0; ni < NT; ++ni)
-            for (int mi = 0; mi < MT; ++mi) acc[ni][mi] = mfma(s.w[q][ni][h], s.x[q][mi][h], acc[ni][mi]);
-    };
-    float low[OUTS];
-    if (has && wave < lines) {
-      Step s0, s1;
-      fetch(s0, wave);
-      uint32_t line = wave;
-      for (;;) {
-        line += U * WAVES;
-        const bool more = line < lines;
-        if (more) fetch(s1, line);
-        multiply(s0);
-        if (!more) break;
-        line += U * WAVES;
-        const bool again = line < lines;
-        if (again) fetch(s0, line);
-        multiply(s1);
-        if (!again) break;
+#pragma unroll
+            for (int mi = 0; mi < MT; ++mi) acc[ni][mi] = mfma(wf[kk][ni], xf[kk][mi], acc[ni][mi]);
+      }
+    } else {
+      const uint32_t kl = lane / 16 * 16;  // this lane's 16 values of a line
+      const T *xp[MT], *wp[NT];
+#pragma unroll
+      for (int mi = 0; mi < MT; ++mi) xp[mi] = (const T*)a.x + slot_of(m0 + mi * 16 + lane % 16) / a.div * a.ldx + kl;
+#pragma unroll
+      for (int ni = 0; ni < NT; ++ni) wp[ni] = w + (int64_t)min(n0 + ni * 16 + lane % 16, a.n - 1) * a.ldw + kl;
+      struct Line {
+        vec8<T> x[MT][2], w[NT][2];
+      };
+      auto piece = [&](const T* p, int64_t left) __attribute__((always_inline)) -> vec8<T> {
+        return load8<T>(left > 0 ? p : zero, left);
+      };
+      auto fetch = [&](Line& s, uint32_t i) __attribute__((always_inline)) {
+        const uint32_t k0 = (wave + i * WAVES) * 64;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const int64_t left = (int64_t)a.k - (k0 + kl + h * 8);
+#pragma unroll
+          for (int ni = 0; ni < NT; ++ni) s.w[ni][h] = piece(wp[ni] + k0 + h * 8, left);
+#pragma unroll
+          for (int mi = 0; mi < MT; ++mi) s.x[mi][h] = piece(xp[mi] + k0 + h * 8, left);
+        }
+      };
+      Line s[2];
+      if (mine) fetch(s[0], 0);
+      for (uint32_t i = 0; i < mine; i += 2) {
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+          if (i + q >= mine) break;
+          if (i + q + 1 < mine) fetch(s[q ^ 1], i + q + 1);
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
+              for (int mi = 0; mi < MT; ++mi) acc[ni][mi] = mfma(s[q].w[ni][h], s[q].x[mi][h], acc[ni][mi]);
+        }
       }
     }
+    float low[OUTS];
+#pragma unroll
     for (int o = 0; o < OUTS; ++o) {
       const uint32_t at = threadIdx.x + o * THREADS;
       const int64_t row = m0 + at / BN;
       low[o] = LR && at < BM * BN && row < g.end && n0 + at % BN < a.n ? lowrank_at<T>(a, row, n0 + at % BN) : 0;
     }
+    __syncthreads();  // every wavefront's ring has been read
+#pragma unroll
     for (int ni = 0; ni < NT; ++ni)
+#pragma unroll
       for (int mi = 0; mi < MT; ++mi)
         *(f32x4*)&red[(wave * BM + mi * 16 + lane % 16) * LD + ni * 16 + lane / 16 * 4] = acc[ni][mi];
     __syncthreads();
+#pragma unroll
     for (int o = 0; o < OUTS; ++o) {
       const uint32_t at = threadIdx.x + o * THREADS, m = at / BN, n = n0 + at % BN;
       const int64_t i = m0 + m;
       if (at >= BM * BN || i >= g.end || n >= a.n) continue;
       float v = 0;
+#pragma unroll
       for (int q = 0; q < WAVES; ++q) v += red[(q * BM + m) * LD + at % BN];
       v += low[o];
       if (a.bias) v += to_float(((const T*)a.bias)[n]);
@@ -192,36 +245,39 @@ __global__ void __launch_bounds__(THREADS) narrow_kernel(MatArgs a, uint32_t sha
   }
 }
 
-template <class T, int MT, int NT>
+template <class T, int MT, int NT, int WAVES, int S>
 hipError_t run(const MatArgs& a, hipStream_t s) {
-  constexpr uint32_t BM = 16 * MT, BN = 16 * NT;
+  constexpr uint32_t BM = 16 * MT, BN = 16 * NT, most = narrow_lds<MT, NT, WAVES, S>() + (th::NARROW_SCAN_SLOTS + 1) * 4;
   const uint64_t ntiles = th::ceil_div(a.n, BN);
   uint64_t mtiles = th::ceil_div(a.rows, BM), blocks;
-  uint32_t shares = 1, bytes = WAVES * BM * (BN + 4) * 4;
+  uint32_t shares = 1;
   if (a.scan) {
     // workgroups of one group: as many as its slots can need, no more than fill the GPU
     shares = (uint32_t)min(mtiles, th::ceil_div(256, ntiles * a.E));
     blocks = ntiles * a.E * shares;
-    bytes += (th::NARROW_SCAN_SLOTS + 1) * 4;
   } else {
     if (a.offsets) mtiles = a.rows / BM + (uint64_t)min((int64_t)a.E + 1, a.rows);
     blocks = mtiles * ntiles;
   }
   auto go = [&](auto kernel) {
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)blocks), dim3(THREADS), bytes, s, a, shares);
+    static const hipError_t ready =
+        hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, most);
+    if (ready != hipSuccess) return ready;
+    const uint32_t bytes = a.scan ? most : narrow_lds<MT, NT, WAVES, S>();
+    kernel<<<(uint32_t)blocks, 64 * WAVES, bytes, s>>>(a, shares);
     return hipGetLastError();
   };
-  if (a.u) return a.aligned ? go(narrow_kernel<T, MT, NT, true, true>) : go(narrow_kernel<T, MT, NT, false, true>);
-  return a.aligned ? go(narrow_kernel<T, MT, NT, true, false>) : go(narrow_kernel<T, MT, NT, false, false>);
+  if (a.u)
+    return a.aligned ? go(narrow_kernel<T, MT, NT, WAVES, S, true, true>) : go(narrow_kernel<T, MT, NT, WAVES, S, false, true>);
+  return a.aligned ? go(narrow_kernel<T, MT, NT, WAVES, S, true, false>) : go(narrow_kernel<T, MT, NT, WAVES, S, false, false>);
 }
 
 template <class T>
 hipError_t typed(const MatArgs& a, hipStream_t s) {
   switch (th::narrow_tile(a.rows, a.n, a.offsets || a.scan ? a.E : 1)) {
-    case th::NARROW_16x16: return run<T, 1, 1>(a, s);
-    case th::NARROW_32x16: return run<T, 2, 1>(a, s);
-    case th::NARROW_32x32: return run<T, 2, 2>(a, s);
-    default: return run<T, 4, 2>(a, s);
+    case th::NARROW_16x16: return run<T, 1, 1, 8, 2>(a, s);
+    case th::NARROW_32x16: return run<T, 2, 1, 8, 3>(a, s);
+    default: return run<T, 2, 2, 4, 2>(a, s);
   }
 }
 

@@ -124,8 +124,9 @@ __global__ void __launch_bounds__(64 * WM * WN) unaligned_kernel(MatArgs a) {
   __syncthreads();
   char* own = lds + wave * (TM * TN * 2);
   const uint32_t rows = (uint32_t)(g.end - g.begin);
-  if (a.y_float) put<float, T, TM, TN>(a, acc, own, slots, wm * TM, rows, n0 + wn * TN, lane);
-  else put<T, T, TM, TN>(a, acc, own, slots, wm * TM, rows, n0 + wn * TN, lane);
+  const Out out{a.y, a.ldy, a.n, a.bias};
+  if (a.y_float) put<float, T, TM, TN>(out, acc, own, slots, wm * TM, rows, n0 + wn * TN, lane);
+  else put<T, T, TM, TN>(out, acc, own, slots, wm * TM, rows, n0 + wn * TN, lane);
 }
 
 template <class T, int BM, int BN, int WM, int WN, int S, bool TR, bool LR>

@@ -147,22 +147,28 @@ constexpr uint32_t wide_lds() {
 // of what a store can carry, so they go through the wavefront's own TM TN 2
 // bytes of LDS and leave as 16 bytes a lane, whole lines of a row: a 16384 x
 // 3584 x 1536 product takes STORE_US.
+struct Out {
+  void* y;
+  int64_t ld;
+  uint32_t n;
+  const void* bias;  // null, or a value per column
+};
 template <class O, class T, int TM, int TN>
-__device__ inline void put(const MatArgs& a, f32x4 (&acc)[TN / 16][TM / 16], char* own, const uint32_t* slots,
+__device__ inline void put(const Out& out, f32x4 (&acc)[TN / 16][TM / 16], char* own, const uint32_t* slots,
                            uint32_t m0, uint32_t rows, uint32_t n0, uint32_t lane) {
   constexpr int PER = 16 / sizeof(O), CH = TN / PER;      // values of a 16-byte chunk, chunks of a row
   constexpr int SLAB = TM * 2 / (int)sizeof(O);           // rows that fit
   constexpr int MASK = CH < 16 ? CH - 1 : 15;
-  const bool wide = a.ldy % PER == 0 && ((uintptr_t)a.y & 15) == 0;
+  const bool wide = out.ld % PER == 0 && ((uintptr_t)out.y & 15) == 0;
 #pragma unroll
   for (int s0 = 0; s0 < TM; s0 += SLAB) {
 #pragma unroll
     for (int ni = 0; ni < TN / 16; ++ni) {
       float bias[4] = {0, 0, 0, 0};
       const uint32_t n = n0 + ni * 16 + lane / 16 * 4;
-      if (a.bias)
+      if (out.bias)
         for (int q = 0; q < 4; ++q)
-          if (n + q < a.n) bias[q] = to_float(((const T*)a.bias)[n + q]);
+          if (n + q < out.n) bias[q] = to_float(((const T*)out.bias)[n + q]);
 #pragma unroll
       for (int mi = s0 / 16; mi < (s0 + SLAB) / 16; ++mi) {
         const f32x4 v = acc[ni][mi];
@@ -175,18 +181,18 @@ __device__ inline void put(const MatArgs& a, f32x4 (&acc)[TN / 16][TM / 16], cha
     __builtin_amdgcn_wave_barrier();  // a wavefront's LDS accesses are answered in order
     for (uint32_t i = lane; i < SLAB * CH; i += 64) {
       const uint32_t row = i / CH, m = m0 + s0 + row, n = n0 + i % CH * PER;
-      if (m >= rows || n >= a.n) continue;
+      if (m >= rows || n >= out.n) continue;
       O o[PER];
       __builtin_memcpy(o, __builtin_assume_aligned(own + (row * CH + ((i % CH) ^ (row & MASK))) * 16, 16), 16);
-      O* y = (O*)a.y + (int64_t)slots[m] * a.ldy + n;
-      if (wide && n + PER <= a.n) {
+      O* y = (O*)out.y + (int64_t)(slots ? slots[m] : m) * out.ld + n;
+      if (wide && n + PER <= out.n) {
         u32x4 v;
         __builtin_memcpy(&v, o, 16);
         __builtin_nontemporal_store(v, (u32x4*)y);
       }
       else
         for (int q = 0; q < PER; ++q)
-          if (n + q < a.n) y[q] = o[q];
+          if (n + q < out.n) y[q] = o[q];
     }
     __builtin_amdgcn_wave_barrier();
   }
@@ -357,8 +363,9 @@ __global__ void __launch_bounds__(64 * WM * WN) wide_kernel(MatArgs a) {
   __syncthreads();
   char* own = lds + wave * (TM * TN * 2);
   const uint32_t rows = (uint32_t)(g.end - g.begin);
-  if (a.y_float) put<float, T, TM, TN>(a, acc, own, slots, wm * TM, rows, n0 + wn * TN, lane);
-  else put<T, T, TM, TN>(a, acc, own, slots, wm * TM, rows, n0 + wn * TN, lane);
+  const Out out{a.y, a.ldy, a.n, a.bias};
+  if (a.y_float) put<float, T, TM, TN>(out, acc, own, slots, wm * TM, rows, n0 + wn * TN, lane);
+  else put<T, T, TM, TN>(out, acc, own, slots, wm * TM, rows, n0 + wn * TN, lane);
 }
 
 }  // namespace mix
