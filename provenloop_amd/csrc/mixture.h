@@ -29,12 +29,12 @@ struct RouteArgs {
   const uint8_t* mask;  // null, or T x E, row stride mask_ld (0: one row for all)
   int64_t T, ld, mask_ld;
   uint32_t E, k, chunk;
-  int normalize;
+  int normalize, vector;  // vector: 8 logits, and their mask bytes, can be loaded at once
   float* weights;     // T x k
   int32_t* experts;   // T x k (input of launch_group)
   int32_t* order;     // T k
   int32_t* offsets;   // E + 1
-  uint32_t* hist;     // (E + 1) x chunks, with more than one chunk
+  uint32_t* hist;     // chunks x (E + 1), with more than one chunk
 };
 hipError_t launch_route(MixType type, RouteArgs a, hipStream_t s);
 hipError_t launch_group(RouteArgs a, hipStream_t s);

@@ -249,8 +249,20 @@ int th_route(int dtype, const void* logits, int64_t ld, int64_t tokens, uint32_t
     need(offsets && (tokens == 0 || (weights && experts && order)), "null output");
     need_work(work, work_bytes, hist_words(tokens, n_experts, choices) * 4);
     need_device();
-    RouteArgs a{logits, mask,    tokens,  ld,    mask_ld, n_experts, choices, 0,
-                normalize, weights, experts, order, offsets, (uint32_t*)work};
+    RouteArgs a{};
+    a.logits = logits;
+    a.mask = mask;
+    a.T = tokens;
+    a.ld = ld;
+    a.mask_ld = mask_ld;
+    a.E = n_experts;
+    a.k = choices;
+    a.normalize = normalize;
+    a.weights = weights;
+    a.experts = experts;
+    a.order = order;
+    a.offsets = offsets;
+    a.hist = (uint32_t*)work;
     HIPCHK(launch_route(type, a, (hipStream_t)stream));
   });
 }

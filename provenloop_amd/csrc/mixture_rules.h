@@ -12,13 +12,16 @@ constexpr uint32_t MIX_MAX_RANK = 128;      // eight 16-row tiles of an adapter 
 
 constexpr uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
-// Tokens whose (token, choice) slots one workgroup of 1024 threads groups: up
-// to 4096 slots, fewer (from 1024) while that gives more workgroups than 128.
-// One workgroup alone needs no second launch, so up to 2048 slots stay whole.
+// Tokens whose (token, choice) slots one workgroup of 1024 threads groups: 1024
+// to 4096 slots, as few as give a workgroup to each of the 256 CUs, and more
+// where there would be more than 1024 workgroups, each of which adds up the
+// others' counts. One workgroup alone needs no second launch, so up to 2048
+// slots stay whole.
 constexpr uint64_t group_chunk_tokens(uint64_t tokens, uint32_t k) {
   const uint64_t slots = tokens * k;
-  uint64_t chunk = slots <= 2048 ? 2048 : ceil_div(slots, 128);
+  uint64_t chunk = slots <= 2048 ? 2048 : ceil_div(slots, 256);
   chunk = chunk < 1024 ? 1024 : chunk > 4096 ? 4096 : chunk;
+  if (chunk < ceil_div(slots, 1024)) chunk = ceil_div(slots, 1024);
   const uint64_t t = chunk / k;
   return t ? t : 1;
 }

@@ -11,23 +11,76 @@
 //
 // Both read their input once and write 12 bytes a slot; what bounds them is
 // the latency of the chain of dependent steps, at small sizes the launch.
+// Candidates are single numbers in a lane's registers, sorted once, and lanes
+// compare by DPP: 65536 tokens over 64 experts, 8 chosen, take ROUTE_US.
 #include "mixture.h"
 
 namespace {
 
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
 
-__device__ inline uint64_t u64_shfl_xor(uint64_t v, int m) {
-  const uint32_t lo = __shfl_xor((uint32_t)v, m), hi = __shfl_xor((uint32_t)(v >> 32), m);
-  return (uint64_t)hi << 32 | lo;
-}
+// A logit as a whole number that orders candidates: its bits made to rise with
+// its value (NaN above +inf, as a comparison sort of the framework's users puts
+// it; -0 with +0), over the expert's number from the top, so that of equal
+// logits the lowest expert is the largest. 0 is kept for "not allowed".
+template <class T>
+struct Ranked {  // bf16 and f16: 16 bits and 16 bits
+  using type = uint32_t;
+  static __device__ inline uint32_t of(T v, uint32_t e) {
+    uint16_t b = __builtin_bit_cast(uint16_t, v);
+    b = b == 0x8000 ? 0 : b;
+    const uint32_t key = v != v ? 0xffffu : b & 0x8000 ? 0xffffu & ~b : b | 0x8000u;
+    return key << 16 | (0xffffu - e);
+  }
+  static __device__ inline uint32_t expert(uint32_t c) { return 0xffffu - (c & 0xffffu); }
+  static __device__ inline float value(uint32_t c) {
+    const uint32_t key = c >> 16;
+    const uint16_t b = (uint16_t)(key & 0x8000 ? key ^ 0x8000 : ~key);
+    return key == 0xffffu ? NAN : (float)__builtin_bit_cast(T, b);
+  }
+};
+template <>
+struct Ranked<float> {
+  using type = uint64_t;
+  static __device__ inline uint64_t of(float v, uint32_t e) {
+    const uint32_t b = __float_as_uint(v + 0.0f);
+    const uint32_t key = v != v ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
+    return (uint64_t)key << 32 | (0xffffffffu - e);
+  }
+  static __device__ inline uint32_t expert(uint64_t c) { return 0xffffffffu - (uint32_t)c; }
+  static __device__ inline float value(uint64_t c) {
+    const uint32_t key = (uint32_t)(c >> 32);
+    return key == 0xffffffffu ? NAN : __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
+  }
+};
 
-// Orders logits as whole numbers above 0: NaN above +inf (as a comparison sort
-// of the framework's users puts it), -0 with +0. 0 is kept for "not allowed".
-__device__ inline uint32_t order_key(float v) {
-  if (v != v) return 0xffffffffu;
-  const uint32_t b = __float_as_uint(v + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+// The same value from a lane on the other side, of pairs, quads, 8, 16, 32 or
+// 64 lanes whose halves each agree on theirs.
+template <int D>
+__device__ inline uint32_t across(uint32_t v) {
+  if constexpr (D == 1) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
+  else if constexpr (D == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);   // quad_perm 2 3 0 1
+  else if constexpr (D == 4) return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);  // row_half_mirror
+  else if constexpr (D == 8) return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);  // row_mirror
+  else return __shfl_xor(v, D);
+}
+template <int D>
+__device__ inline uint64_t across(uint64_t v) {
+  return (uint64_t)across<D>((uint32_t)(v >> 32)) << 32 | across<D>((uint32_t)v);
+}
+template <int G, class C, int D = 1>
+__device__ inline C group_max(C v) {
+  if constexpr (D < G) {
+    const C o = across<D>(v);
+    return group_max<G, C, 2 * D>(o > v ? o : v);
+  } else {
+    return v;
+  }
+}
+template <int G, int D = 1>
+__device__ inline float group_sum(float v) {
+  if constexpr (D < G) return group_sum<G, 2 * D>(v + __uint_as_float(across<D>(__float_as_uint(v))));
+  else return v;
 }
 
 template <class T>
@@ -97,96 +150,125 @@ __device__ void place_slots(const int32_t* experts, int64_t s0, int64_t s1, uint
 }
 
 // base = where this chunk's slots start, per expert, from every chunk's counts
-// hist[key][chunk]; offsets written by chunk 0.
-__device__ void chunk_bases(const uint32_t* hist, uint32_t E, uint32_t chunks, uint32_t* base, uint32_t* total,
+// hist[chunk][key]; offsets written by chunk 0. A wavefront adds up every 16th
+// chunk, 64 keys at a time; sums: LDS, 2 WAVES (E + 1) words.
+__device__ void chunk_bases(const uint32_t* hist, uint32_t E, uint32_t chunks, uint32_t* base, uint32_t* sums,
                             int32_t* offsets) {
-  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  for (uint32_t key = wave; key <= E; key += WAVES) {
+  const uint32_t wave = threadIdx.x >> 6, lane = threadIdx.x & 63, keys = E + 1;
+  for (uint32_t key = lane; key < keys; key += 64) {
     uint32_t before = 0, all = 0;
-    for (uint32_t c = lane; c < chunks; c += 64) {
-      const uint32_t n = hist[(size_t)key * chunks + c];
+#pragma unroll 8
+    for (uint32_t c = wave; c < chunks; c += WAVES) {
+      const uint32_t n = hist[(size_t)c * keys + key];
       all += n;
-      if (c < blockIdx.x) before += n;
+      before += c < blockIdx.x ? n : 0;
     }
-    for (int d = 32; d; d >>= 1) {
-      before += __shfl_xor(before, d);
-      all += __shfl_xor(all, d);
-    }
-    if (lane == 0) {
-      base[key] = before;
-      total[key] = all;
-    }
+    sums[wave * keys + key] = before;
+    sums[(WAVES + wave) * keys + key] = all;
   }
   __syncthreads();
-  prefix_words(total, E + 1);
+  for (uint32_t key = threadIdx.x; key < keys; key += THREADS) {
+    uint32_t before = 0, all = 0;
+    for (int w = 0; w < WAVES; ++w) {
+      before += sums[w * keys + key];
+      all += sums[(WAVES + w) * keys + key];
+    }
+    base[key] = before;
+    sums[key] = all;
+  }
   __syncthreads();
-  for (uint32_t key = threadIdx.x; key <= E; key += THREADS) {
-    base[key] += total[key];
-    if (blockIdx.x == 0) offsets[key] = (int32_t)total[key];
+  prefix_words(sums, keys);
+  __syncthreads();
+  for (uint32_t key = threadIdx.x; key < keys; key += THREADS) {
+    base[key] += sums[key];
+    if (blockIdx.x == 0 && key < keys) offsets[key] = (int32_t)sums[key];
   }
   __syncthreads();
 }
 
 // One workgroup's tokens [t0, t1): a group of G lanes per token, 8 experts a
-// lane, k rounds of a maximum over (logit, lowest index). Counts the chosen
-// experts in `base`.
+// lane in falling order in its registers, and k rounds: the largest of the
+// lanes' first candidates is chosen and its lane moves on. Lane j of the group
+// keeps choice j. Counts the chosen experts in `base`.
 template <class T, int G>
 __device__ void choose(const RouteArgs& a, int64_t t0, int64_t t1, uint32_t* base) {
+  using R = Ranked<T>;
+  using C = typename R::type;
   const uint32_t g = threadIdx.x % G;
+  const bool whole = g * 8 + 8 <= a.E && a.vector;
   for (int64_t at = t0; at < t1; at += THREADS / G) {
     const int64_t t = at + threadIdx.x / G;
     if (t >= t1) continue;  // whole groups of G lanes leave together
-    uint32_t key[8];
-    float l[8], big = -INFINITY;
-    for (int i = 0; i < 8; ++i) {
-      const uint32_t e = g * 8 + i;
-      key[i] = 0;
-      l[i] = -INFINITY;
-      if (e < a.E && allowed_at<T>(a, t, e, l[i])) key[i] = order_key(l[i]);
+    const T* row = (const T*)a.logits + t * a.ld + g * 8;
+    const uint8_t* mask = a.mask ? a.mask + t * a.mask_ld + g * 8 : nullptr;
+    T l[8];
+    uint64_t allowed = ~0ull;  // a byte per expert
+    if (whole) {
+      __builtin_memcpy(l, __builtin_assume_aligned(row, 16), sizeof(l));
+      if (mask) __builtin_memcpy(&allowed, __builtin_assume_aligned(mask, 8), 8);
+    } else {
+      for (uint32_t i = 0; i < 8; ++i) {
+        const bool in = g * 8 + i < a.E;
+        l[i] = in ? row[i] : (T)0.0f;
+        if (!in || (mask && !mask[i])) allowed &= ~(0xffull << (8 * i));
+      }
     }
+    C c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      c[i] = (allowed >> (8 * i) & 0xff) && !((float)l[i] == -INFINITY) ? R::of(l[i], g * 8 + i) : 0;
+    // Batcher's odd-even merge of 8: 19 exchanges
+    auto order = [&](int i, int j) __attribute__((always_inline)) {
+      const C hi = c[i] > c[j] ? c[i] : c[j], lo = c[i] > c[j] ? c[j] : c[i];
+      c[i] = hi;
+      c[j] = lo;
+    };
+    order(0, 1), order(2, 3), order(4, 5), order(6, 7), order(0, 2), order(1, 3), order(4, 6), order(5, 7);
+    order(1, 2), order(5, 6), order(0, 4), order(1, 5), order(2, 6), order(3, 7), order(2, 4), order(3, 5);
+    order(1, 2), order(3, 4), order(5, 6);
+    const C first = group_max<G>(c[0]);
+    const float big = first ? R::value(first) : -INFINITY;
     float z = 0;
-    for (uint32_t j = 0; j < a.k; ++j) {
-      uint64_t best = 0;
-      for (int i = 0; i < 8; ++i) {
-        const uint64_t c = (uint64_t)key[i] << 32 | (0xffffffffu - (g * 8 + i));
-        if (key[i] && c > best) best = c;
-      }
-      for (int d = 1; d < G; d <<= 1) {
-        const uint64_t o = u64_shfl_xor(best, d);
-        best = o > best ? o : best;
-      }
-      const int32_t e = best ? (int32_t)(0xffffffffu - (uint32_t)best) : -1;
-      float v = -INFINITY;
+    if (!a.normalize) {
+#pragma unroll
       for (int i = 0; i < 8; ++i)
-        if (e == (int32_t)(g * 8 + i)) {
-          v = l[i];
-          key[i] = 0;
+        if (c[i]) z += expf(R::value(c[i]) - big);
+      z = group_sum<G>(z);
+    }
+    constexpr int KEEP = G >= 32 ? 1 : G >= 4 ? 32 / G : 8;  // choices that one lane can have to keep
+    float p[KEEP];
+    int32_t e[KEEP];
+#pragma unroll
+    for (int r = 0; r < KEEP; ++r) {
+      p[r] = 0;
+      e[r] = -1;
+      if (r * G < (int)a.k) {
+        for (uint32_t j = 0; j < G && r * G + j < a.k; ++j) {
+          const C best = group_max<G>(c[0]);
+          if (c[0] == best) {
+#pragma unroll
+            for (int i = 0; i < 7; ++i) c[i] = c[i + 1];
+            c[7] = 0;
+          }
+          if (g == j && best) {
+            e[r] = (int32_t)R::expert(best);
+            p[r] = expf(R::value(best) - big);
+          }
         }
-      // the chosen logit is in one lane of the group; the others hold -inf, and
-      // a NaN has to survive the exchange, so it goes by the owner's lane
-      if (G > 1) v = __shfl(v, e < 0 ? 0 : (int)((threadIdx.x & 63) / G * G + e / 8));
-      if (e < 0) v = -INFINITY;
-      if (j == 0) {
-        big = v;
-        if (!a.normalize) {
-          for (int i = 0; i < 8; ++i)  // the keys but the first chosen one's are still whole
-            if (key[i]) z += expf(l[i] - big);
-          for (int d = 1; d < G; d <<= 1) z += __shfl_xor(z, d);
-          if (e >= 0) z += expf(v - big);
-        }
-      }
-      const float p = e < 0 ? 0.0f : expf(v - big);
-      if (a.normalize) z += p;
-      if (g == 0) {
-        a.experts[t * a.k + j] = e;
-        a.weights[t * a.k + j] = p;
-        atomicAdd(&base[e < 0 ? a.E : e], 1u);
       }
     }
-    if (g == 0) {
-      for (uint32_t j = 0; j < a.k; ++j) {
-        const float p = a.weights[t * a.k + j];
-        a.weights[t * a.k + j] = a.experts[t * a.k + j] < 0 ? 0.0f : p / z;
+    if (a.normalize) {
+#pragma unroll
+      for (int r = 0; r < KEEP; ++r) z += p[r];
+      z = group_sum<G>(z);
+    }
+#pragma unroll
+    for (int r = 0; r < KEEP; ++r) {
+      const uint32_t j = r * G + g;
+      if (j < a.k) {
+        a.experts[t * a.k + j] = e[r];
+        a.weights[t * a.k + j] = e[r] < 0 ? 0.0f : p[r] / z;
+        atomicAdd(&base[e[r] < 0 ? a.E : e[r]], 1u);
       }
     }
   }
@@ -204,7 +286,7 @@ __global__ void __launch_bounds__(THREADS) route_kernel(RouteArgs a) {
   __threadfence_block();
   __syncthreads();
   if (gridDim.x > 1) {
-    for (uint32_t i = threadIdx.x; i <= a.E; i += THREADS) a.hist[(size_t)i * gridDim.x + blockIdx.x] = base[i];
+    for (uint32_t i = threadIdx.x; i <= a.E; i += THREADS) a.hist[(size_t)blockIdx.x * (a.E + 1) + i] = base[i];
     return;
   }
   prefix_words(base, a.E + 1);
@@ -227,7 +309,7 @@ __global__ void __launch_bounds__(THREADS) count_kernel(RouteArgs a) {
   }
   __syncthreads();
   if (gridDim.x > 1) {
-    for (uint32_t i = threadIdx.x; i <= a.E; i += THREADS) a.hist[(size_t)i * gridDim.x + blockIdx.x] = base[i];
+    for (uint32_t i = threadIdx.x; i <= a.E; i += THREADS) a.hist[(size_t)blockIdx.x * (a.E + 1) + i] = base[i];
     return;
   }
   prefix_words(base, a.E + 1);
@@ -297,10 +379,14 @@ hipError_t route_typed(const RouteArgs& a, uint32_t chunks, size_t lds, hipStrea
   return hipGetLastError();
 }
 
-size_t group_lds(uint32_t E) { return (size_t)(WAVES + 1) * (E + 1) * 4; }
+size_t group_lds(uint32_t E, bool chunks = false) { return (size_t)((chunks ? 2 : 1) * WAVES + 1) * (E + 1) * 4; }
 
 hipError_t place(const RouteArgs& a, uint32_t chunks, hipStream_t s) {
-  if (chunks > 1) place_kernel<<<chunks, THREADS, group_lds(a.E), s>>>(a);
+  if (chunks == 1) return hipSuccess;
+  static const hipError_t ready = hipFuncSetAttribute((const void*)place_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                      (int)group_lds(th::MIX_MAX_EXPERTS, true));
+  if (ready != hipSuccess) return ready;
+  place_kernel<<<chunks, THREADS, group_lds(a.E, true), s>>>(a);
   return hipGetLastError();
 }
 
@@ -309,6 +395,9 @@ hipError_t place(const RouteArgs& a, uint32_t chunks, hipStream_t s) {
 hipError_t launch_route(MixType type, RouteArgs a, hipStream_t s) {
   const uint32_t chunks = (uint32_t)th::group_chunks(a.T, a.k);
   a.chunk = (uint32_t)th::group_chunk_tokens(a.T, a.k);
+  const uint32_t size = type == MIX_F32 ? 4 : 2;
+  a.vector = (uintptr_t)a.logits % 16 == 0 && (a.T == 1 || a.ld * size % 16 == 0) &&
+             (!a.mask || ((uintptr_t)a.mask % 8 == 0 && a.mask_ld % 8 == 0));
   hipError_t e = type == MIX_BF16  ? route_typed<bf16_t>(a, chunks, group_lds(a.E), s)
                  : type == MIX_F16 ? route_typed<f16_t>(a, chunks, group_lds(a.E), s)
                                    : route_typed<float>(a, chunks, group_lds(a.E), s);
