@@ -42,13 +42,14 @@ constexpr uint64_t lowrank_spans(uint64_t slots, uint32_t E, uint32_t span) {
 }
 
 // Products of few output tiles (narrow.hip). The tile: 16 rows where groups
-// have no more, else 32; 32 columns once there are enough workgroups (32 x 3584
+// have no more, or the output no more columns (8192 x 16 x 1536: 5.9 us, 6.1
+// with 32 rows), else 32; 32 columns once there are enough workgroups (32 x 3584
 // x 3584: 6.7 us with 16 columns, 7.7 with 32; 250 x 1536 x 1536: 9.0 and 6.7).
 enum NarrowTile { NARROW_16x16, NARROW_32x16, NARROW_32x32 };
 constexpr NarrowTile narrow_tile(uint64_t rows, uint32_t n, uint32_t groups) {
   const uint64_t each = ceil_div(rows, groups);
-  if (each <= 16) return NARROW_16x16;
-  return n <= 16 || groups * ceil_div(each, 32) * ceil_div(n, 32) < 192 ? NARROW_32x16 : NARROW_32x32;
+  if (each <= 16 || n <= 16) return NARROW_16x16;
+  return groups * ceil_div(each, 32) * ceil_div(n, 32) < 192 ? NARROW_32x16 : NARROW_32x32;
 }
 // Whether a product is one of those: fewer than 128 tiles of 128 x 128.
 constexpr bool narrow_product(uint64_t rows, uint32_t n, uint32_t groups) {

@@ -91,6 +91,8 @@ __global__ void __launch_bounds__(64 * WM * WN) unaligned_kernel(MatArgs a) {
     };
     fetch(0);
     commit(0);
+    LowLists<BM>& lists = *(LowLists<BM>*)(slots + BM);
+    if (LR) list_adapters<BM, 64 * WAVES>(a, g.begin, g.end, lists);
     uint32_t stage = 0;
     for (uint32_t k0 = 0; k0 < a.k; k0 += BK, stage ^= 1) {
       __syncthreads();
@@ -118,7 +120,7 @@ __global__ void __launch_bounds__(64 * WM * WN) unaligned_kernel(MatArgs a) {
       }
       if (more) commit(stage ^ 1);
     }
-    if (LR) add_lowrank<T, BM, BN, WM, WN>(a, g.begin, g.end, n0, lds, acc);
+    if (LR) add_lowrank<T, BM, BN, WM, WN>(a, g.begin, g.end, n0, lds, lists, acc);
   }
 
   __syncthreads();

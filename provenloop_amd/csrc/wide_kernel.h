@@ -25,100 +25,148 @@ __device__ inline void arrived_but(void) {
 // bf16 pairs, high and low, so that u keeps its float's 16 leading bits: one
 // more product with the low halves costs little next to the main one, and
 // rounding u once to bf16 would be as large an error as rounding y.
-template <class T, int BM, int BN, int WM, int WN>
-__device__ void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, uint32_t n0, char* lds,
-                            f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
-  constexpr int THREADS = 64 * WM * WN, TM = BM / WM, TN = BN / WN;
-  constexpr bool PAIR = !std::is_same<T, bf16_t>::value;  // f16 operands are pairs too
-  char *xhi = lds, *xlo = xhi + BM * 128, *whi = xlo + BM * 128, *wlo = whi + (PAIR ? BN * 128 : 0);
-  uint32_t* words = (uint32_t*)lds;  // which adapters, a bit each, before the tiles come there
-  uint16_t* list = (uint16_t*)(wlo + BN * 128);
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
-  const uint32_t used = (uint32_t)(mend - m0) * a.kc;
-  const int32_t* ids = a.ids + m0 * a.kc;
-  __syncthreads();
-  if (threadIdx.x < 32) words[threadIdx.x] = 0;
+//
+// list_adapters runs under the main product's first loads and leaves in LDS the
+// adapters and, for up to KEPT choices, each row's and its coefficients; the
+// loads of one set of 64 ranks then go out together.
+constexpr uint32_t KEPT = 4;
+template <int BM>
+struct LowLists {
+  uint32_t words[32];  // a bit per adapter
+  uint32_t count;
+  uint16_t list[th::MIX_MAX_EXPERTS];  // those used, rising
+  uint32_t id[BM * KEPT];              // rows x choices; ~0: none
+  float c[BM * KEPT];
+};
+
+template <int BM, int THREADS>
+__device__ inline void list_adapters(const MatArgs& a, int64_t m0, int64_t mend, LowLists<BM>& l) {
+  const uint32_t lane = threadIdx.x & 63, used = (uint32_t)(mend - m0) * a.kc;
+  if (threadIdx.x < 32) l.words[threadIdx.x] = 0;
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < used; i += THREADS) {
-    const uint32_t e = (uint32_t)ids[i];
-    if (e < a.E) atomicOr(&words[e / 32], 1u << (e % 32));
+    const int64_t s = m0 * a.kc + i;
+    const uint32_t e = (uint32_t)a.ids[s];
+    float c = a.gate ? a.gate[s] : 1.0f;
+    if (e < a.E) {
+      atomicOr(&l.words[e / 32], 1u << (e % 32));
+      if (a.scale) c *= a.scale[e];
+    }
+    if (a.kc <= KEPT) {
+      l.id[i] = e < a.E ? e : ~0u;
+      l.c[i] = c;
+    }
   }
   __syncthreads();
-  uint32_t count;
-  {
-    const uint32_t word = lane < 32 ? words[lane] : 0, own = __popc(word);
+  if (threadIdx.x < 64) {
+    const uint32_t word = lane < 32 ? l.words[lane] : 0, own = __popc(word);
     uint32_t sum = own;
     for (int d = 1; d < 64; d <<= 1) {
       const uint32_t up = __shfl_up(sum, d);
       if ((int)lane >= d) sum += up;
     }
-    count = __shfl(sum, 63);
-    if (wave == 0) {
-      uint32_t at = sum - own;
-      for (uint32_t w = word; w; w &= w - 1) list[at++] = (uint16_t)(lane * 32 + __ffs(w) - 1);
-    }
+    uint32_t at = sum - own;
+    for (uint32_t w = word; w; w &= w - 1) l.list[at++] = (uint16_t)(lane * 32 + __ffs(w) - 1);
+    if (lane == 63) l.count = sum;
   }
   __syncthreads();
-  const uint32_t each = (a.r + 7) / 8, chunks = count * each;  // chunks of 8 ranks
+}
+
+template <class T, int BM, int BN, int WM, int WN>
+__device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, uint32_t n0, char* lds,
+                                   const LowLists<BM>& l, f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
+  constexpr int THREADS = 64 * WM * WN, TM = BM / WM, TN = BN / WN;
+  constexpr int XI = BM * 8 / THREADS, WI = BN * 8 / THREADS;   // 16-byte pieces of a thread
+  constexpr bool PAIR = !std::is_same<T, bf16_t>::value;  // f16 operands are pairs too
+  char *xhi = lds, *xlo = xhi + BM * 128, *whi = xlo + BM * 128, *wlo = whi + (PAIR ? BN * 128 : 0);
+  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wm = wave / WN, wn = wave % WN;
+  const uint32_t rows = (uint32_t)(mend - m0);
+  const uint32_t each = (a.r + 7) / 8, chunks = l.count * each;  // chunks of 8 ranks
+  const uint32_t piece = threadIdx.x % 8;                        // this thread's chunk of a set, in all its rows
   for (uint32_t c0 = 0; c0 < chunks; c0 += 8) {
-    if (c0) __syncthreads();
-    for (uint32_t i = threadIdx.x; i < BM * 8; i += THREADS) {
-      const uint32_t row = i / 8, c = c0 + i % 8;
-      f32x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
-      if (c < chunks && m0 + row < mend) {
-        const uint32_t e = list[c / each], r0 = c % each * 8;
-        for (uint32_t j = 0; j < a.kc; ++j)
-          if ((uint32_t)ids[row * a.kc + j] == e) {
-            const int64_t s = (m0 + row) * a.kc + j;
-            const float* u = a.u + s * a.ru + r0;
-            float f = a.gate ? a.gate[s] : 1.0f;
-            if (a.scale) f *= a.scale[e];
-            for (uint32_t q = 0; q < 8; ++q)
-              if (r0 + q < a.r) v[q] += f * u[q];
-          }
+    const uint32_t c = c0 + piece, e = c < chunks ? l.list[c / each] : ~1u, r0 = c % each * 8;
+    const bool whole = r0 + 8 <= a.r;
+    f32x4 u0[XI], u1[XI];
+    float f[XI];
+    vec8<T> v[WI];
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+      const uint32_t row = i * (THREADS / 8) + threadIdx.x / 8;
+      u0[i] = u1[i] = f32x4{0, 0, 0, 0};
+      f[i] = 0;
+      uint32_t at = ~0u;
+      if (row < rows && c < chunks) {
+        for (uint32_t j = 0; j < a.kc; ++j) {  // an adapter chosen twice counts with both coefficients
+          const uint32_t s = row * a.kc + j;
+          uint32_t id;
+          if (a.kc <= KEPT) id = l.id[s];
+          else id = (uint32_t)a.ids[m0 * a.kc + s];
+          if (id != e) continue;
+          at = s;
+          if (a.kc <= KEPT) f[i] += l.c[s];
+          else f[i] += (a.gate ? a.gate[m0 * a.kc + s] : 1.0f) * (a.scale ? a.scale[e] : 1.0f);
+        }
       }
+      if (at != ~0u) {
+        const float* u = a.u + (m0 * a.kc + at) * a.ru + r0;
+        if (whole) {
+          u0[i] = *(const f32x4*)u;
+          u1[i] = *(const f32x4*)(u + 4);
+        } else {
+          for (uint32_t q = 0; q < 8; ++q)
+            if (r0 + q < a.r) (q < 4 ? u0[i] : u1[i])[q % 4] = u[q];
+        }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < WI; ++i) {
+      const uint32_t n = n0 + i * (THREADS / 8) + threadIdx.x / 8;
+      const bool in = c < chunks && n < a.n;
+      v[i] = load8<T>(in ? (const T*)a.p + e * a.ldpe + (int64_t)n * a.ldp + r0 : (const T*)&mix_zero16,
+                      in ? (int64_t)a.r - r0 : 0);
+    }
+    __syncthreads();  // the LDS below has been read
+#pragma unroll
+    for (int i = 0; i < XI; ++i) {
+      const uint32_t row = i * (THREADS / 8) + threadIdx.x / 8, at = row * 128 + (piece ^ (row & 7)) * 16;
+      f32x8 x;
+#pragma unroll
+      for (int q = 0; q < 8; ++q) x[q] = f[i] * (q < 4 ? u0[i] : u1[i])[q % 4];
       bf16x8 hi, lo;
-      split8(v, hi, lo);
-      const uint32_t at = row * 128 + ((i % 8) ^ (row & 7)) * 16;
+      split8(x, hi, lo);
       *(bf16x8*)(xhi + at) = hi;
       *(bf16x8*)(xlo + at) = lo;
     }
-    for (uint32_t i = threadIdx.x; i < BN * 8; i += THREADS) {
-      const uint32_t row = i / 8, c = c0 + i % 8, n = n0 + row;
-      vec8<T> v;
-      for (int q = 0; q < 8; ++q) v[q] = (T)0.0f;
-      if (c < chunks && n < a.n) {
-        const uint32_t r0 = c % each * 8;
-        v = load8<T>((const T*)a.p + list[c / each] * a.ldpe + (int64_t)n * a.ldp + r0, (int64_t)a.r - r0);
-      }
-      const uint32_t at = row * 128 + ((i % 8) ^ (row & 7)) * 16;
+#pragma unroll
+    for (int i = 0; i < WI; ++i) {
+      const uint32_t row = i * (THREADS / 8) + threadIdx.x / 8, at = row * 128 + (piece ^ (row & 7)) * 16;
       if constexpr (PAIR) {
-        const SplitF16 s = widen(v);
+        const SplitF16 s = widen(v[i]);
         *(bf16x8*)(whi + at) = s.hi;
         *(bf16x8*)(wlo + at) = s.lo;
       } else {
-        *(bf16x8*)(whi + at) = v;
+        *(bf16x8*)(whi + at) = v[i];
       }
     }
     __syncthreads();
     for (uint32_t kk = 0; kk < 2; ++kk) {
       if (c0 + kk * 4 >= chunks) break;
       bf16x8 hi[TM / 16], lo[TM / 16];
-      #pragma unroll
+#pragma unroll
       for (int mi = 0; mi < TM / 16; ++mi) {
         const uint32_t row = wm * TM + mi * 16 + lane % 16, at = row * 128 + ((kk * 4 + lane / 16) ^ (row & 7)) * 16;
         hi[mi] = *(const bf16x8*)(xhi + at);
         lo[mi] = *(const bf16x8*)(xlo + at);
       }
-      #pragma unroll
+#pragma unroll
       for (int ni = 0; ni < TN / 16; ++ni) {
         const uint32_t row = wn * TN + ni * 16 + lane % 16, at = row * 128 + ((kk * 4 + lane / 16) ^ (row & 7)) * 16;
         const bf16x8 wf = *(const bf16x8*)(whi + at);
-        #pragma unroll
+#pragma unroll
         for (int mi = 0; mi < TM / 16; ++mi) acc[ni][mi] = mfma(wf, hi[mi], mfma(wf, lo[mi], acc[ni][mi]));
         if constexpr (PAIR) {
           const bf16x8 wl = *(const bf16x8*)(wlo + at);
-          #pragma unroll
+#pragma unroll
           for (int mi = 0; mi < TM / 16; ++mi) acc[ni][mi] = mfma(wl, hi[mi], acc[ni][mi]);
         }
       }
@@ -127,11 +175,11 @@ __device__ void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, uint32_t
 }
 template <class T, int BM, int BN>
 constexpr uint32_t lowrank_lds() {
-  return 2 * BM * 128 + (std::is_same<T, bf16_t>::value ? 1 : 2) * BN * 128 + 2048;
+  return 2 * BM * 128 + (std::is_same<T, bf16_t>::value ? 1 : 2) * BN * 128;
 }
 
 // LDS: the stages, the low-rank tiles and each wavefront's outputs in turn in
-// the same place, then the tile's rows.
+// the same place, then the tile's rows and low-rank lists.
 template <class T, int BM, int BN, int S, bool LR>
 constexpr uint32_t wide_slots() {
   const uint32_t main = S * (BM + BN) * BK * 2, low = LR ? lowrank_lds<T, BM, BN>() : 0, out = BM * BN * 2;
@@ -139,7 +187,7 @@ constexpr uint32_t wide_slots() {
 }
 template <class T, int BM, int BN, int S, bool LR>
 constexpr uint32_t wide_lds() {
-  return wide_slots<T, BM, BN, S, LR>() + BM * 4;
+  return wide_slots<T, BM, BN, S, LR>() + BM * 4 + (LR ? (uint32_t)sizeof(LowLists<BM>) : 0);
 }
 
 // A wavefront's TM x TN outputs to memory. A lane holds 4 neighbouring columns
@@ -336,6 +384,8 @@ __global__ void __launch_bounds__(64 * WM * WN) wide_kernel(MatArgs a) {
       if (s < tiles)
 #pragma unroll
         for (int j = 0; j < LOADS; ++j) load(j, s * BK, s);
+    LowLists<BM>& lists = *(LowLists<BM>*)(slots + BM);
+    if (LR) list_adapters<BM, 64 * WAVES>(a, g.begin, g.end, lists);
     if (tiles >= S) arrived_but<(S - 1) * LOADS>();
     else arrived_but<0>();
 #pragma unroll
@@ -357,7 +407,7 @@ __global__ void __launch_bounds__(64 * WM * WN) wide_kernel(MatArgs a) {
       half(1, i + 1 < tiles, next, 0, false, 0, 0);
       stage = next;
     }
-    if (LR) add_lowrank<T, BM, BN, WM, WN>(a, g.begin, g.end, n0, lds, acc);
+    if (LR) add_lowrank<T, BM, BN, WM, WN>(a, g.begin, g.end, n0, lds, lists, acc);
   }
 
   __syncthreads();
