@@ -6,6 +6,10 @@ using namespace mix;
 
 namespace {
 
+// Slots whose rows a workgroup of low_outer_kernel holds in LDS: 64 KiB of the
+// wide operand and up to 64 KiB of ranks.
+constexpr int low_batch(int mr) { return mr <= 4 ? 256 : 128; }
+
 // ---------------------------------------------------------------- weight gradients
 // The group that comes n-th by its number of slots, most first (of up to 256;
 // further ones in their own order): the long contractions then start first and
@@ -244,115 +248,209 @@ __global__ void __launch_bounds__(256) unaligned_outer_kernel(OuterArgs a) {
 
 // ---------------------------------------------------------------- low-rank gradients
 // Partial sums over a span of one adapter's slots: 16 MR rows of the low-rank
-// factor (float, scaled, as a bf16 pair) by 128 columns of the wide operand.
-template <class T, int MR>
-__global__ void __launch_bounds__(256) low_outer_kernel(LowOuterArgs a, uint32_t ctiles) {
-  constexpr int BN = 128, LD = 72;  // LDS row of 64 slots, padded
-  __shared__ __attribute__((aligned(16))) char wide[64 * BN * 2];
-  __shared__ __attribute__((aligned(16))) bf16_t low[2][MR * 16 * LD];
-  const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const uint32_t c0 = blockIdx.x % ctiles * BN, span = blockIdx.x / ctiles;
+// factor (float, scaled, as a bf16 pair) by 128 columns of the wide operand,
+// BATCH slots at a time. Few flops and short contractions: what bounds it is
+// the chain slot -> row -> product, so a batch's loads all go out together, and
+// the CU's other workgroups run meanwhile. Both gradients share a launch.
+template <class T, int MR, bool ALIGNED>
+__global__ void __launch_bounds__(256) low_outer_kernel(LowOuterPair pair) {
+  constexpr int BATCH = low_batch(MR), BN = 128, R = 16 * MR;
+  constexpr int JOBS = BATCH / 16;  // 1 KiB loads (4 slots) per wavefront and batch
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  char *wide = lds, *low[2] = {wide + BATCH * BN * 2, wide + BATCH * BN * 2 + BATCH * R * 2};
+  uint32_t* slot = (uint32_t*)(low[1] + BATCH * R * 2);
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const bool second = blockIdx.x >= pair.blocks;
+  const LowOuterArgs& a = pair.p[second];
+  const uint32_t block = blockIdx.x - (second ? pair.blocks : 0), ctiles = (a.cols + BN - 1) / BN;
+  const uint32_t c0 = block % ctiles * BN, span = block / ctiles;
   const GroupTile g = find_group_tile(a.offsets, a.E, a.E, a.slots, a.span, span, lane);
   if (g.begin >= g.end) return;
+  const char* zero = (const char*)&mix_zero16;
   f32x4 acc[MR][2];
+#pragma unroll
   for (int i = 0; i < MR; ++i) acc[i][0] = acc[i][1] = f32x4{0, 0, 0, 0};
   const float se = a.scale ? a.scale[g.group] : 1.0f;
-  for (int64_t s0 = g.begin; s0 < g.end; s0 += 64) {
-    __syncthreads();
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t piece = j * 256 + threadIdx.x, row = piece / 16;
-      const uint32_t c = c0 + ((piece % 16) ^ tr_swizzle<BN>(row)) * 8;
-      const int64_t i = s0 + row;
-      vec8<T> v;
-      if (i < g.end && c < a.cols) {
-        const int64_t s = min((int64_t)(uint32_t)a.order[i], a.slots - 1);
-        const T* p = (const T*)a.wide + s / a.div * a.ldwide + c;
-        v = load8<T>(p, a.cols - c);
-      } else {
-        v = load8<T>((const T*)&mix_zero16, 0);
-      }
-      *(vec8<T>*)(wide + piece * 16) = v;
-    }
-    for (uint32_t i = threadIdx.x; i < MR * 16 * 64; i += 256) {
-      const uint32_t q = i % (MR * 16), row = i / (MR * 16);
-      const int64_t at = s0 + row;
-      float v = 0;
-      if (at < g.end && q < a.r) {
-        const int64_t s = min((int64_t)(uint32_t)a.order[at], a.slots - 1);
-        v = a.low[s * a.ru + q] * ((a.gate ? a.gate[s] : 1.0f) * se);
-      }
-      const bf16_t hi = (bf16_t)v;
-      low[0][q * LD + row] = hi;
-      low[1][q * LD + row] = (bf16_t)(v - (float)hi);
+  const uint32_t lds0 = __builtin_amdgcn_readfirstlane(lds_address(lds)) + wave * JOBS * 1024;
+  for (int64_t s0 = g.begin; s0 < g.end; s0 += BATCH) {
+    // thread i < BATCH: slot i of the batch, its coefficient and its row of the low-rank factor
+    uint32_t s = ~0u;
+    float c = 0;
+    if (threadIdx.x < BATCH && s0 + threadIdx.x < g.end) {
+      s = (uint32_t)a.order[s0 + threadIdx.x];
+      if (s >= (uint64_t)a.slots) s = ~0u;
+      else c = (a.gate ? a.gate[s] : 1.0f) * se;
     }
     __syncthreads();
-    for (int kk = 0; kk < 2; ++kk) {
+    if (threadIdx.x < BATCH) slot[threadIdx.x] = s;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < JOBS; ++j) {
+      const uint32_t row = (wave * JOBS + j) * 4 + lane / 16, sr = slot[row];
+      const uint32_t col = c0 + ((lane % 16) ^ tr_swizzle<BN>(row)) * 8;
+      const bool in = sr != ~0u && col < a.cols;
+      const T* p = in ? (const T*)a.wide + (int64_t)(sr / a.div) * a.ldwide + col : (const T*)zero;
+      if constexpr (ALIGNED) load_lds16(p, lds0 + j * 1024);
+      else *(vec8<T>*)(wide + (wave * JOBS + j) * 1024 + lane * 16) = load8<T>(p, in ? (int64_t)a.cols - col : 0);
+    }
+    if (threadIdx.x < BATCH) {
+      const float* u = a.low + (int64_t)(s == ~0u ? 0 : s) * a.ru;
+      const uint32_t limit = s == ~0u ? 0 : a.r;
+#pragma unroll
+      for (int q = 0; q < R; q += 8) {
+        f32x8 v = {0, 0, 0, 0, 0, 0, 0, 0};
+        if (q + 8 <= (int)limit) {
+          const f32x4 u0 = *(const f32x4*)(u + q), u1 = *(const f32x4*)(u + q + 4);
+          for (int x = 0; x < 8; ++x) v[x] = c * (x < 4 ? u0 : u1)[x % 4];
+        } else {
+          for (int x = 0; x < 8; ++x)
+            if (q + x < (int)limit) v[x] = c * u[q + x];
+        }
+        bf16x8 hi, lo;
+        split8(v, hi, lo);
+        const uint32_t at = threadIdx.x * (R * 2) + ((q / 8) ^ tr_swizzle<R>(threadIdx.x)) * 16;
+        *(bf16x8*)(low[0] + at) = hi;
+        *(bf16x8*)(low[1] + at) = lo;
+      }
+    }
+    arrived_barrier();
+    const uint32_t steps = min((uint32_t)BATCH, (uint32_t)(g.end - s0));
+    for (uint32_t k = 0; k < steps; k += 32) {
       decltype(widen(vec8<T>())) wf[2];
-      for (int i = 0; i < 2; ++i) wf[i] = widen(tr_fragment<T, BN>(wide, wave * 32 + i * 16, kk * 32, lane));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) wf[i] = widen(tr_fragment<T, BN>(wide, wave * 32 + i * 16, k, lane));
+#pragma unroll
       for (int m = 0; m < MR; ++m) {
-        const uint32_t at = (m * 16 + lane % 16) * LD + kk * 32 + lane / 16 * 8;
-        const bf16x8 hi = *(const bf16x8*)&low[0][at], lo = *(const bf16x8*)&low[1][at];
+        const bf16x8 hi = tr_fragment<bf16_t, R>(low[0], m * 16, k, lane);
+        const bf16x8 lo = tr_fragment<bf16_t, R>(low[1], m * 16, k, lane);
+#pragma unroll
         for (int i = 0; i < 2; ++i) acc[m][i] = mfma_split(wf[i], hi, lo, acc[m][i]);
       }
     }
   }
   // a lane: row lane % 16 of the low-rank factor, 4 neighbouring columns
+#pragma unroll
   for (int m = 0; m < MR; ++m)
+#pragma unroll
     for (int i = 0; i < 2; ++i) {
       const uint32_t q = m * 16 + lane % 16, c = c0 + wave * 32 + i * 16 + lane / 16 * 4;
       if (q >= a.r) continue;
       float* o = a.partial + ((int64_t)span * a.r + q) * a.cols + c;
-      for (int x = 0; x < 4; ++x)
-        if (c + x < a.cols) o[x] = acc[m][i][x];
+      if (c + 4 <= a.cols && a.cols % 4 == 0) {
+        *(f32x4*)o = acc[m][i];
+      } else {
+        for (int x = 0; x < 4; ++x)
+          if (c + x < a.cols) o[x] = acc[m][i][x];
+      }
     }
 }
 
-// Adds an adapter's partial sums, in slot order.
+// Adds an adapter's partial sums, in slot order. A thread: 4 columns of a rank,
+// or, where the output is transposed, a column of 8 ranks, so that it writes
+// 8 or 16 bytes; loads of several partial sums are under way at once.
 template <class T>
-__global__ void __launch_bounds__(256) low_sum_kernel(LowOuterArgs a) {
+__global__ void __launch_bounds__(256) low_sum_kernel(LowOuterPair pair) {
+  const LowOuterArgs& a = pair.p[blockIdx.z];
   const uint32_t e = blockIdx.y, lane = threadIdx.x & 63;
-  uint32_t first = count_group_tiles(a.offsets, a.E, e, a.slots, a.span, lane);
+  if (!a.out) return;
+  const uint32_t first = count_group_tiles(a.offsets, a.E, e, a.slots, a.span, lane);
   const int64_t c = group_begin(a.offsets, e + 1, a.E, a.slots) - group_begin(a.offsets, e, a.E, a.slots);
   const uint32_t n = c > 0 ? (uint32_t)((c + a.span - 1) / a.span) : 0;
   const uint64_t size = (uint64_t)a.r * a.cols;
-  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (uint64_t)gridDim.x * 256) {
-    const uint64_t at = a.transposed ? i % a.r * a.cols + i / a.r : i;
-    float v = 0;
-    for (uint32_t p = 0; p < n; ++p) v += a.partial[(uint64_t)(first + p) * size + at];
-    ((T*)a.out)[e * size + i] = (T)v;
+  const float* partial = a.partial + first * size;
+  T* out = (T*)a.out + e * size;
+  const uint32_t across = a.transposed ? a.cols : (a.cols + 3) / 4, down = a.transposed ? (a.r + 7) / 8 : a.r;
+  for (uint64_t i = (uint64_t)blockIdx.x * 256 + threadIdx.x; i < (uint64_t)across * down;
+       i += (uint64_t)gridDim.x * 256) {
+    const uint32_t x = (uint32_t)(i % across), y = (uint32_t)(i / across);
+    if (a.transposed) {
+      const uint32_t q0 = y * 8, many = min(8u, a.r - q0);
+      float v[8] = {0, 0, 0, 0, 0, 0, 0, 0};
+      const float* from = partial + (uint64_t)q0 * a.cols + x;
+      if (many == 8) {
+#pragma unroll 4
+        for (uint32_t p = 0; p < n; ++p)
+#pragma unroll
+          for (uint32_t q = 0; q < 8; ++q) v[q] += from[p * size + (uint64_t)q * a.cols];
+      } else {
+        for (uint32_t p = 0; p < n; ++p)
+          for (uint32_t q = 0; q < many; ++q) v[q] += from[p * size + (uint64_t)q * a.cols];
+      }
+      T* o = out + (uint64_t)x * a.r + q0;
+      if (many == 8 && a.r % 8 == 0) {
+        vec8<T> w;
+        for (int q = 0; q < 8; ++q) w[q] = (T)v[q];
+        *(vec8<T>*)o = w;
+      } else {
+        for (uint32_t q = 0; q < many; ++q) o[q] = (T)v[q];
+      }
+    } else if (a.cols % 4 == 0) {
+      f32x4 v = {0, 0, 0, 0};
+#pragma unroll 4
+      for (uint32_t p = 0; p < n; ++p) v += *(const f32x4*)(partial + p * size + (uint64_t)y * a.cols + x * 4);
+      const T w[4] = {(T)v[0], (T)v[1], (T)v[2], (T)v[3]};
+      *(uint64_t*)(out + (uint64_t)y * a.cols + x * 4) = __builtin_bit_cast(uint64_t, w);
+    } else {
+      for (uint32_t q = x * 4; q < min(x * 4 + 4, a.cols); ++q) {
+        float v = 0;
+        for (uint32_t p = 0; p < n; ++p) v += partial[p * size + (uint64_t)y * a.cols + q];
+        out[(uint64_t)y * a.cols + q] = (T)v;
+      }
+    }
   }
+}
+
+template <class T, int MR>
+hipError_t run_low(const LowOuterPair& pair, uint32_t blocks, hipStream_t s) {
+  constexpr uint32_t bytes = low_batch(MR) * (128 * 2 + 2 * 16 * MR * 2 + 4);
+  auto go = [&](auto kernel) {
+    static const hipError_t ready =
+        hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (ready != hipSuccess) return ready;
+    kernel<<<blocks, 256, bytes, s>>>(pair);
+    return hipGetLastError();
+  };
+  const bool aligned = pair.p[0].aligned && pair.p[1].aligned;
+  return aligned ? go(low_outer_kernel<T, MR, true>) : go(low_outer_kernel<T, MR, false>);
 }
 
 template <class T>
-hipError_t low_outer_typed(const LowOuterArgs& a, hipStream_t s) {
-  const uint32_t ctiles = (uint32_t)th::ceil_div(a.cols, 128);
-  const uint32_t blocks = ctiles * (uint32_t)th::lowrank_spans(a.slots, a.E, a.span);
-  if (blocks) {
-    if (a.r <= 16) low_outer_kernel<T, 1><<<blocks, 256, 0, s>>>(a, ctiles);
-    else if (a.r <= 32) low_outer_kernel<T, 2><<<blocks, 256, 0, s>>>(a, ctiles);
-    else if (a.r <= 64) low_outer_kernel<T, 4><<<blocks, 256, 0, s>>>(a, ctiles);
-    else low_outer_kernel<T, 8><<<blocks, 256, 0, s>>>(a, ctiles);
+hipError_t low_outer_typed(LowOuterPair pair, hipStream_t s) {
+  uint32_t blocks = 0, rows = 0;
+  for (int i = 0; i < 2; ++i) {
+    const LowOuterArgs& a = pair.p[i];
+    if (i == 1) pair.blocks = blocks;
+    if (!a.out) continue;
+    blocks += (uint32_t)(th::ceil_div(a.cols, 128) * th::lowrank_spans(a.slots, a.E, a.span));
+    const uint64_t threads = a.transposed ? a.cols * th::ceil_div(a.r, 8) : a.r * th::ceil_div(a.cols, 4);
+    rows = max(rows, (uint32_t)min(th::ceil_div(threads, 256), (uint64_t)1024));
   }
-  hipError_t e = hipGetLastError();
-  if (e != hipSuccess) return e;
-  const uint64_t size = (uint64_t)a.r * a.cols;
-  low_sum_kernel<T><<<dim3((uint32_t)min(th::ceil_div(size, 256), (uint64_t)1024), a.E), 256, 0, s>>>(a);
+  const LowOuterArgs& a = pair.p[pair.p[0].out ? 0 : 1];
+  if (blocks) {
+    const hipError_t e = a.r <= 16   ? run_low<T, 1>(pair, blocks, s)
+                         : a.r <= 32 ? run_low<T, 2>(pair, blocks, s)
+                         : a.r <= 64 ? run_low<T, 4>(pair, blocks, s)
+                                     : run_low<T, 8>(pair, blocks, s);
+    if (e != hipSuccess) return e;
+  }
+  low_sum_kernel<T><<<dim3(rows, a.E, 2), 256, 0, s>>>(pair);
   return hipGetLastError();
 }
 
-__global__ void __launch_bounds__(256) transpose_kernel(const uint16_t* in, int64_t ld, int64_t lde, uint16_t* out,
-                                                        uint32_t rows, uint32_t cols) {
+// 64 x 64 pieces of the matrices of up to two stacks.
+__global__ void __launch_bounds__(256) transpose_kernel(TransposePair pair) {
   __shared__ uint16_t tile[64][66];
-  const uint32_t r0 = blockIdx.x * 64, c0 = blockIdx.y * 64, e = blockIdx.z;
-  for (uint32_t i = threadIdx.x; i < 64 * 64; i += 256) {
-    const uint32_t r = r0 + i / 64, c = c0 + i % 64;
-    if (r < rows && c < cols) tile[i / 64][i % 64] = in[e * lde + r * ld + c];
-  }
+  const bool second = blockIdx.x >= pair.blocks;
+  const TransposeArgs& a = pair.p[second];
+  const uint32_t block = blockIdx.x - (second ? pair.blocks : 0);
+  const uint32_t rt = (a.rows + 63) / 64, ct = (a.cols + 63) / 64;
+  const uint32_t r0 = block % rt * 64, c0 = block / rt % ct * 64, e = block / rt / ct;
+  const uint32_t h = min(64u, a.rows - r0), w = min(64u, a.cols - c0);
+  for (uint32_t i = threadIdx.x; i < h * w; i += 256)
+    tile[i / w][i % w] = ((const uint16_t*)a.in)[e * a.lde + (int64_t)(r0 + i / w) * a.ld + c0 + i % w];
   __syncthreads();
-  for (uint32_t i = threadIdx.x; i < 64 * 64; i += 256) {
-    const uint32_t c = c0 + i / 64, r = r0 + i % 64;
-    if (r < rows && c < cols) out[((int64_t)e * cols + c) * rows + r] = tile[i % 64][i / 64];
-  }
+  for (uint32_t i = threadIdx.x; i < h * w; i += 256)
+    ((uint16_t*)a.out)[((int64_t)e * a.cols + c0 + i / h) * a.rows + r0 + i % h] = tile[i % h][i / h];
 }
 
 template <class T>
@@ -400,14 +498,18 @@ hipError_t launch_outer(MixType type, const OuterArgs& a, hipStream_t s) {
   return type == MIX_BF16 ? outer_typed<bf16_t>(a, s) : outer_typed<f16_t>(a, s);
 }
 
-hipError_t launch_low_outer(MixType type, LowOuterArgs a, hipStream_t s) {
-  return type == MIX_BF16 ? low_outer_typed<bf16_t>(a, s) : low_outer_typed<f16_t>(a, s);
+hipError_t launch_low_outer(MixType type, const LowOuterPair& pair, hipStream_t s) {
+  return type == MIX_BF16 ? low_outer_typed<bf16_t>(pair, s) : low_outer_typed<f16_t>(pair, s);
 }
 
-hipError_t launch_transpose(const void* in, int64_t ld, int64_t lde, void* out, uint32_t E, uint32_t rows,
-                            uint32_t cols, hipStream_t s) {
-  const dim3 grid((uint32_t)th::ceil_div(rows, 64), (uint32_t)th::ceil_div(cols, 64), E);
-  transpose_kernel<<<grid, 256, 0, s>>>((const uint16_t*)in, ld, lde, (uint16_t*)out, rows, cols);
+hipError_t launch_transpose(TransposePair pair, hipStream_t s) {
+  uint32_t blocks = 0;
+  for (int i = 0; i < 2; ++i) {
+    const TransposeArgs& a = pair.p[i];
+    if (i == 1) pair.blocks = blocks;
+    if (a.out) blocks += (uint32_t)(th::ceil_div(a.rows, 64) * th::ceil_div(a.cols, 64) * a.E);
+  }
+  if (blocks) transpose_kernel<<<blocks, 256, 0, s>>>(pair);
   return hipGetLastError();
 }
 

@@ -103,11 +103,26 @@ struct LowOuterArgs {
   uint32_t r, ru, cols, E, div, span;  // span: slots of one partial sum
   int aligned, transposed;
 };
-hipError_t launch_low_outer(MixType type, LowOuterArgs a, hipStream_t s);
+// Two such sums with the same slots and ranks in one launch; one without `out` is left out.
+struct LowOuterPair {
+  LowOuterArgs p[2];
+  uint32_t blocks;  // of the first
+};
+hipError_t launch_low_outer(MixType type, const LowOuterPair& pair, hipStream_t s);
 
-// out (E x cols x rows) = transposes of E matrices of rows x cols
-hipError_t launch_transpose(const void* in, int64_t ld, int64_t lde, void* out, uint32_t E, uint32_t rows,
-                            uint32_t cols, hipStream_t s);
+// out (E x cols x rows) = transposes of E matrices of rows x cols; two stacks in
+// one launch, one without `out` is left out.
+struct TransposeArgs {
+  const void* in;
+  void* out;
+  int64_t ld, lde;
+  uint32_t E, rows, cols;
+};
+struct TransposePair {
+  TransposeArgs p[2];
+  uint32_t blocks;  // of the first
+};
+hipError_t launch_transpose(TransposePair pair, hipStream_t s);
 // out[t] = sum_j in[t k + j], rows of n floats
 hipError_t launch_sum_choices(MixType type, const float* in, void* out, int64_t tokens, uint32_t k, uint32_t n,
                               hipStream_t s);

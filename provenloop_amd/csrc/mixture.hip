@@ -112,7 +112,7 @@ void check_lora(const th_lora_linear_args* d) {
 struct LoraWork {
   int32_t *order = nullptr, *offsets = nullptr;
   uint32_t* hist = nullptr;
-  float *u = nullptr, *v = nullptr, *partial = nullptr;
+  float *u = nullptr, *v = nullptr, *partial[2] = {};
   uint16_t *at = nullptr, *bt = nullptr;
 };
 // Few slots that nothing else needs grouped: the low-rank product finds each
@@ -140,10 +140,11 @@ LoraWork lay_backward(Pieces& p, const th_lora_linear_args* d) {
   w.v = p.take<float>(slots * padded_rank(d->rank));
   w.at = p.take<uint16_t>((uint64_t)d->adapters * d->d_in * d->rank);
   w.bt = p.take<uint16_t>((uint64_t)d->adapters * d->d_out * d->rank);
-  uint64_t most = 0;
-  for (uint32_t cols : {d->d_in, d->d_out})
-    most = std::max(most, th::lowrank_spans(slots, d->adapters, th::lowrank_span(slots, cols)) * d->rank * cols);
-  w.partial = p.take<float>(most);
+  for (int i = 0; i < 2; ++i) {
+    const uint32_t cols = i ? d->d_out : d->d_in;
+    w.partial[i] =
+        p.take<float>(th::lowrank_spans(slots, d->adapters, th::lowrank_span(slots, cols)) * d->rank * cols);
+  }
   return w;
 }
 
@@ -454,11 +455,13 @@ int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const 
     const int64_t slots = d->tokens * d->choices;
     make_groups(d, w, s);
     if (slots && (dx || da || dgate)) {
-      HIPCHK(launch_transpose(d->b, d->ldb, d->ldb_adapter, w.bt, d->adapters, d->d_out, d->rank, s));
+      TransposePair t{};
+      t.p[0] = TransposeArgs{d->b, w.bt, d->ldb, d->ldb_adapter, d->adapters, d->d_out, d->rank};
+      if (dx) t.p[1] = TransposeArgs{d->a, w.at, d->lda, d->lda_adapter, d->adapters, d->rank, d->d_in};
+      HIPCHK(launch_transpose(t, s));
       shrink(d, w, dy, lddy, d->d_out, w.bt, d->d_out, (int64_t)d->d_out * d->rank, w.v, s);
     }
     if (slots && dx) {
-      HIPCHK(launch_transpose(d->a, d->lda, d->lda_adapter, w.at, d->adapters, d->rank, d->d_in, s));
       MatArgs m{};
       m.x = dy;
       m.ldx = lddy;
@@ -474,28 +477,30 @@ int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const 
       set_lowrank(m, d, w.v, w.at, d->rank, (int64_t)d->d_in * d->rank);
       HIPCHK(launch_mat(type, m, 1, s));
     }
-    for (int which = 0; which < 2; ++which) {
-      void* out = which ? db : da;
-      if (!out) continue;
-      LowOuterArgs o{};
-      o.low = which ? u : w.v;
-      o.wide = which ? dy : d->x;
-      o.ldwide = which ? lddy : d->ldx;
-      o.cols = which ? d->d_out : d->d_in;
-      o.out = out;
-      o.partial = w.partial;
-      o.order = w.order;
-      o.offsets = w.offsets;
-      o.gate = d->gate;
-      o.scale = d->scale;
-      o.slots = slots;
-      o.r = d->rank;
-      o.ru = ru;
-      o.E = d->adapters;
-      o.div = d->choices;
-      o.span = th::lowrank_span(slots, o.cols);
-      o.transposed = which;
-      HIPCHK(launch_low_outer(type, o, s));
+    if (da || db) {
+      LowOuterPair pair{};
+      for (int which = 0; which < 2; ++which) {
+        LowOuterArgs& o = pair.p[which];
+        o.low = which ? u : w.v;
+        o.wide = which ? dy : d->x;
+        o.ldwide = which ? lddy : d->ldx;
+        o.cols = which ? d->d_out : d->d_in;
+        o.out = which ? db : da;
+        o.partial = w.partial[which];
+        o.order = w.order;
+        o.offsets = w.offsets;
+        o.gate = d->gate;
+        o.scale = d->scale;
+        o.slots = slots;
+        o.r = d->rank;
+        o.ru = ru;
+        o.E = d->adapters;
+        o.div = d->choices;
+        o.span = th::lowrank_span(slots, o.cols);
+        o.aligned = !o.out || (on16(o.wide, o.ldwide, d->tokens) && o.cols % 8 == 0);
+        o.transposed = which;
+      }
+      HIPCHK(launch_low_outer(type, pair, s));
     }
     if (dgate) HIPCHK(launch_gate_grad(u, w.v, d->experts, d->scale, dgate, slots, d->rank, ru, d->adapters, s));
   });
