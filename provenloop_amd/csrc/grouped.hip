@@ -453,15 +453,24 @@ __global__ void __launch_bounds__(256) transpose_kernel(TransposePair pair) {
     ((uint16_t*)a.out)[((int64_t)e * a.cols + c0 + i / h) * a.rows + r0 + i % h] = tile[i % h][i / h];
 }
 
-template <class T>
+// A thread: 8 columns of a token, or 1 where rows are no multiple of 8.
+template <class T, int W>
 __global__ void __launch_bounds__(256) sum_choices_kernel(const float* in, T* out, int64_t tokens, uint32_t k,
                                                           uint32_t n) {
-  const int64_t size = tokens * n;
-  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < size; i += (int64_t)gridDim.x * 256) {
-    const int64_t t = i / n;
-    float v = 0;
-    for (uint32_t j = 0; j < k; ++j) v += in[(t * k + j) * n + i % n];
-    out[i] = (T)v;
+  const uint32_t c = (blockIdx.x * 256 + threadIdx.x) * W;
+  if (c >= n) return;
+  for (int64_t t = blockIdx.y; t < tokens; t += gridDim.y) {
+    const float* p = in + t * k * n + c;
+    float v[W] = {};
+#pragma unroll 2
+    for (uint32_t j = 0; j < k; ++j) {
+      float x[W];
+      __builtin_memcpy(x, __builtin_assume_aligned(p + (int64_t)j * n, W == 8 ? 16 : 4), sizeof(x));
+      for (int q = 0; q < W; ++q) v[q] += x[q];
+    }
+    T o[W];
+    for (int q = 0; q < W; ++q) o[q] = (T)v[q];
+    __builtin_memcpy(__builtin_assume_aligned(out + t * n + c, W == 8 ? 16 : 2), o, sizeof(o));
   }
 }
 
@@ -515,11 +524,13 @@ hipError_t launch_transpose(TransposePair pair, hipStream_t s) {
 
 hipError_t launch_sum_choices(MixType type, const float* in, void* out, int64_t tokens, uint32_t k, uint32_t n,
                               hipStream_t s) {
-  const uint64_t size = (uint64_t)tokens * n;
-  if (!size) return hipSuccess;
-  const uint32_t blocks = (uint32_t)min(th::ceil_div(size, 256), (uint64_t)8192);
-  if (type == MIX_BF16) sum_choices_kernel<<<blocks, 256, 0, s>>>(in, (bf16_t*)out, tokens, k, n);
-  else sum_choices_kernel<<<blocks, 256, 0, s>>>(in, (f16_t*)out, tokens, k, n);
+  if (!tokens) return hipSuccess;
+  const bool by8 = n % 8 == 0 && ((uintptr_t)out & 15) == 0;
+  const dim3 grid((uint32_t)th::ceil_div(n, by8 ? 2048 : 256), (uint32_t)min(tokens, (int64_t)16384));
+  if (type == MIX_BF16 && by8) sum_choices_kernel<bf16_t, 8><<<grid, 256, 0, s>>>(in, (bf16_t*)out, tokens, k, n);
+  else if (type == MIX_BF16) sum_choices_kernel<bf16_t, 1><<<grid, 256, 0, s>>>(in, (bf16_t*)out, tokens, k, n);
+  else if (by8) sum_choices_kernel<f16_t, 8><<<grid, 256, 0, s>>>(in, (f16_t*)out, tokens, k, n);
+  else sum_choices_kernel<f16_t, 1><<<grid, 256, 0, s>>>(in, (f16_t*)out, tokens, k, n);
   return hipGetLastError();
 }
 

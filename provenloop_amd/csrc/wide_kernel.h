@@ -236,7 +236,8 @@ __device__ inline void put(const Out& out, f32x4 (&acc)[TN / 16][TM / 16], char*
       if (wide && n + PER <= out.n) {
         u32x4 v;
         __builtin_memcpy(&v, o, 16);
-        __builtin_nontemporal_store(v, (u32x4*)y);
+        if constexpr (std::is_same<O, float>::value) *(u32x4*)y = v;  // a workspace: read again at once
+        else __builtin_nontemporal_store(v, (u32x4*)y);
       }
       else
         for (int q = 0; q < PER; ++q)
