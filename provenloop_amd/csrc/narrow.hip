@@ -24,29 +24,55 @@
 
 namespace {
 
-template <class T>
-__device__ __forceinline__ float lowrank_at(const MatArgs& a, int64_t row, uint32_t n) {
-  float sum = 0;
+// low[o] = the low-rank part of output (m0 + (tid + o THREADS) / BN, n0 + (tid +
+// o THREADS) % BN), clamped to the tile's rows and the product's columns; the
+// outputs' loads go out together.
+template <class T, int OUTS, int THREADS, int BN>
+__device__ __forceinline__ void lowrank_at(const MatArgs& a, int64_t m0, int64_t mend, uint32_t n0, float (&low)[OUTS]) {
+  const T* p[OUTS];
+  const float* u[OUTS];
+  int64_t row[OUTS];
+#pragma unroll
+  for (int o = 0; o < OUTS; ++o) {
+    const uint32_t at = threadIdx.x + o * THREADS;
+    row[o] = min(m0 + at / BN, mend - 1) * a.kc;
+    p[o] = (const T*)a.p + (int64_t)min(n0 + at % BN, a.n - 1) * a.ldp;
+    low[o] = 0;
+  }
   for (uint32_t j = 0; j < a.kc; ++j) {
-    const int64_t s = row * a.kc + j;
-    const uint32_t e = (uint32_t)a.ids[s];
-    if (e >= a.E) continue;
-    const T* p = (const T*)a.p + (int64_t)e * a.ldpe + (int64_t)n * a.ldp;
-    const float* u = a.u + s * a.ru;
-    float d = 0;
+    uint32_t e[OUTS];
+    float c[OUTS], d[OUTS];
+#pragma unroll
+    for (int o = 0; o < OUTS; ++o) {
+      e[o] = (uint32_t)a.ids[row[o] + j];
+      c[o] = a.gate ? a.gate[row[o] + j] : 1.0f;
+      u[o] = a.u + (row[o] + j) * a.ru;
+      d[o] = 0;
+    }
+    // a slot without an adapter takes part with the first one's values, and its product is dropped
     uint32_t i = 0;
     for (; i + 8 <= a.r; i += 8) {
-      const vec8<T> v = load8<T>(p + i, 8);
-      const f32x4 u0 = *(const f32x4*)(u + i), u1 = *(const f32x4*)(u + i + 4);
-      for (int q = 0; q < 4; ++q) d = fmaf(u0[q], (float)v[q], d);
-      for (int q = 0; q < 4; ++q) d = fmaf(u1[q], (float)v[q + 4], d);
+      vec8<T> v[OUTS];
+      f32x4 u0[OUTS], u1[OUTS];
+#pragma unroll
+      for (int o = 0; o < OUTS; ++o) {
+        v[o] = load8<T>(p[o] + (e[o] < a.E ? e[o] : 0) * a.ldpe + i, 8);
+        u0[o] = *(const f32x4*)(u[o] + i);
+        u1[o] = *(const f32x4*)(u[o] + i + 4);
+      }
+#pragma unroll
+      for (int o = 0; o < OUTS; ++o)
+#pragma unroll
+        for (int q = 0; q < 8; ++q) d[o] = fmaf((q < 4 ? u0[o] : u1[o])[q % 4], (float)v[o][q], d[o]);
     }
-    for (; i < a.r; ++i) d = fmaf(u[i], (float)p[i], d);
-    float c = a.gate ? a.gate[s] : 1.0f;
-    if (a.scale) c *= a.scale[e];
-    sum = fmaf(c, d, sum);
+    for (; i < a.r; ++i)
+#pragma unroll
+      for (int o = 0; o < OUTS; ++o)
+        d[o] = fmaf(u[o][i], (float)p[o][(e[o] < a.E ? e[o] : 0) * a.ldpe + i], d[o]);
+#pragma unroll
+    for (int o = 0; o < OUTS; ++o)
+      if (e[o] < a.E) low[o] = fmaf(a.scale ? c[o] * a.scale[e[o]] : c[o], d[o], low[o]);
   }
-  return sum;
 }
 
 template <int MT, int NT, int WAVES, int S>
@@ -125,6 +151,7 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
     for (int ni = 0; ni < NT; ++ni)
 #pragma unroll
       for (int mi = 0; mi < MT; ++mi) acc[ni][mi] = f32x4{0, 0, 0, 0};
+    float low[OUTS] = {};
     if constexpr (ALIGNED) {
       const uint32_t xk = ((lane % 8) ^ (lane / 8)) * 8;  // chunk c of row i lies at c ^ (i % 8)
       const T* p[LOADS];
@@ -142,6 +169,7 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
 #pragma unroll
       for (int i = 0; i < S; ++i)
         if (i < (int)mine) load(i, i);
+      if (LR) lowrank_at<T, OUTS, THREADS, BN>(a, m0, g.end, n0, low);  // while the first lines are on their way
       uint32_t stage = 0;
       for (uint32_t i = 0; i < mine; ++i) {
         if (i + S <= mine) arrived<(S - 1) * LOADS>();
@@ -198,6 +226,7 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
       };
       Line s[2];
       if (mine) fetch(s[0], 0);
+      if (LR) lowrank_at<T, OUTS, THREADS, BN>(a, m0, g.end, n0, low);
       for (uint32_t i = 0; i < mine; i += 2) {
 #pragma unroll
         for (int q = 0; q < 2; ++q) {
@@ -211,13 +240,6 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
               for (int mi = 0; mi < MT; ++mi) acc[ni][mi] = mfma(s[q].w[ni][h], s[q].x[mi][h], acc[ni][mi]);
         }
       }
-    }
-    float low[OUTS];
-#pragma unroll
-    for (int o = 0; o < OUTS; ++o) {
-      const uint32_t at = threadIdx.x + o * THREADS;
-      const int64_t row = m0 + at / BN;
-      low[o] = LR && at < BM * BN && row < g.end && n0 + at % BN < a.n ? lowrank_at<T>(a, row, n0 + at % BN) : 0;
     }
     __syncthreads();  // every wavefront's ring has been read
 #pragma unroll
