@@ -51,15 +51,25 @@ constexpr NarrowTile narrow_tile(uint64_t rows, uint32_t n, uint32_t groups) {
   if (each <= 16 || n <= 16) return NARROW_16x16;
   return groups * ceil_div(each, 32) * ceil_div(n, 32) < 192 ? NARROW_32x16 : NARROW_32x32;
 }
-// Whether a product is one of those: fewer than 128 tiles of 128 x 128.
-constexpr bool narrow_product(uint64_t rows, uint32_t n, uint32_t groups) {
+// Whether a product is one of those: up to 1024 tiles of 32 x 32, about what the
+// time of one round of large tiles pays for (narrow / wide in us: 256 columns of
+// 1536 steps, 2048 rows 12.6 / 21.1, 4096 rows 22.9 / 21.4; 1536 of 1536, 512
+// rows 15.7 / 21.5, 1024 rows 25.9 / 22.4; 3584 of 3584, 256 rows 26 / 42, 512
+// rows 45 / 43; 4096 of 512, 128 rows 7.3 / 11.4, 256 rows 12.3 / 11.7). Groups of
+// up to 16 rows are weights to be read, which small tiles do faster if the
+// contraction is long (8 groups of 8 rows: 3584 of 3584 38 / 54, 4096 of 512
+// 20 / 13).
+constexpr bool narrow_product(uint64_t rows, uint32_t n, uint32_t k, uint32_t groups) {
   const uint64_t each = ceil_div(rows, groups);
-  return groups * ceil_div(each, 128) * ceil_div(n, 128) < 128 || each <= 32;
+  if (each <= 16) return k >= 1024 || groups * ceil_div(n, 16) <= 1024;
+  return groups * ceil_div(each, 32) * ceil_div(n, 32) <= 1024;
 }
 // The wide products' tile: 256 x 256 or 256 x 128. A CU holds one workgroup of
-// either; a square tile takes 1.75 times as long as the other (8192^3: 3.4 us
-// a 1000 steps of 2 tiles against ...), so it is better where the number of
-// rounds over the 256 CUs allows it.
+// either, and a square tile takes 1.75 times as long as the other (1.72 and
+// 0.97 us per 64 steps at 8192 x 8192 x 8192, 1288 and 1113 TFLOP/s), so it is
+// better where the number of rounds over the 256 CUs allows it: 8192 x 3584 x
+// 3584 takes 204 us with squares and 249 with halves, 4096 x 1536 x 1536 36 and
+// 24.5.
 constexpr bool wide_square(uint64_t rows, uint32_t n, uint32_t groups) {
   const uint64_t m = groups * ceil_div(ceil_div(rows, groups), 256);
   return ceil_div(m * ceil_div(n, 256), 256) * 7 <= ceil_div(m * ceil_div(n, 128), 256) * 4;
