@@ -70,7 +70,7 @@ struct MatArgs {
 };
 // w is n x k (transposed = 0: y = x w^T) or k x n (1: y = x w).
 hipError_t launch_mat(MixType type, const MatArgs& a, int transposed, hipStream_t s);
-hipError_t launch_narrow(MixType type, const MatArgs& a, hipStream_t s);  // w as n x k; launch_mat's choice
+hipError_t launch_narrow(MixType type, const MatArgs& a, int transposed, hipStream_t s);  // launch_mat's choice
 
 // out[g] = sum over the slots s of group g of left[s] (outer) right[s / div]:
 // n x k per group, with left row s of dy (n values), right row s / div of x (k).

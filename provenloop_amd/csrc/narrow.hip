@@ -1,5 +1,5 @@
-// Matrix products with few rows of output tiles: y = x w^T for decodes, small
-// batches and the low-rank factors A x.
+// Matrix products with few output tiles: y = x w^T for decodes, small batches and
+// the low-rank factors A x, and y = x w for the gradients of small batches.
 //
 // What bounds them is the latency of reading w (a decode reads each weight for
 // a few rows) and how many CUs take part, not the matrix cores. So a workgroup
@@ -82,7 +82,9 @@ constexpr uint32_t narrow_lds() {
 }
 
 // 16 MT rows by 16 NT columns, WAVES wavefronts, S lines of each row in a ring.
-template <class T, int MT, int NT, int WAVES, int S, bool ALIGNED, bool LR>
+// TR: w is k x n, and a line of it 64 rows of 16 NT values, read through the
+// transposing LDS read.
+template <class T, int MT, int NT, int WAVES, int S, bool TR, bool ALIGNED, bool LR>
 __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t shares) {
   constexpr int BM = 16 * MT, BN = 16 * NT, LD = BN + 4, THREADS = 64 * WAVES;
   constexpr int OUTS = BM * BN / THREADS ? BM * BN / THREADS : 1;
@@ -154,17 +156,33 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
     float low[OUTS] = {};
     if constexpr (ALIGNED) {
       const uint32_t xk = ((lane % 8) ^ (lane / 8)) * 8;  // chunk c of row i lies at c ^ (i % 8)
+      constexpr int CH = 2 * NT;                          // chunks of a row of a transposed line
       const T* p[LOADS];
 #pragma unroll
-      for (int j = 0; j < LOADS; ++j)
-        p[j] = j < 2 * MT ? (const T*)a.x + slot_of(m0 + j * 8 + lane / 8) / a.div * a.ldx + xk
-                          : w + (int64_t)min(n0 + (j - 2 * MT) * 8 + lane / 8, a.n - 1) * a.ldw + xk;
+      for (int j = 0; j < LOADS; ++j) {
+        const int jw = j - 2 * MT;
+        if (j < 2 * MT) {
+          p[j] = (const T*)a.x + slot_of(m0 + j * 8 + lane / 8) / a.div * a.ldx + xk;
+        } else if constexpr (TR) {
+          const uint32_t row = jw * (64 / CH) + lane / CH, col = n0 + ((lane % CH) ^ tr_swizzle<BN>(row)) * 8;
+          p[j] = col < a.n ? w + (int64_t)row * a.ldw + col : nullptr;
+        } else {
+          p[j] = w + (int64_t)min(n0 + jw * 8 + lane / 8, a.n - 1) * a.ldw + xk;
+        }
+      }
       const char* ring = lds + wave * (S * STAGE);
       const uint32_t base = __builtin_amdgcn_readfirstlane(lds_address(ring));
       auto load = [&](uint32_t i, uint32_t stage) __attribute__((always_inline)) {
         const uint32_t k0 = (wave + i * WAVES) * 64;
 #pragma unroll
-        for (int j = 0; j < LOADS; ++j) load_lds16(k0 + xk < a.k ? p[j] + k0 : zero, base + stage * STAGE + j * 1024);
+        for (int j = 0; j < LOADS; ++j) {
+          const T* q;
+          if (TR && j >= 2 * MT)
+            q = k0 + (j - 2 * MT) * (64 / CH) + lane / CH < a.k && p[j] ? p[j] + (int64_t)k0 * a.ldw : zero;
+          else
+            q = k0 + xk < a.k ? p[j] + k0 : zero;
+          load_lds16(q, base + stage * STAGE + j * 1024);
+        }
       };
 #pragma unroll
       for (int i = 0; i < S; ++i)
@@ -187,7 +205,8 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
 #pragma unroll
           for (int ni = 0; ni < NT; ++ni) {
             const uint32_t r = ni * 16 + lane % 16;
-            wf[kk][ni] = *(const vec8<T>*)(wt + r * 128 + (c ^ (r & 7)) * 16);
+            if constexpr (TR) wf[kk][ni] = tr_fragment<T, BN>(wt, ni * 16, kk * 32, lane);
+            else wf[kk][ni] = *(const vec8<T>*)(wt + r * 128 + (c ^ (r & 7)) * 16);
           }
         }
         answered();  // the stage has been read before its place is loaded again
@@ -268,7 +287,7 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
 }
 
 template <class T, int MT, int NT, int WAVES, int S>
-hipError_t run(const MatArgs& a, hipStream_t s) {
+hipError_t run(const MatArgs& a, int transposed, hipStream_t s) {
   constexpr uint32_t BM = 16 * MT, BN = 16 * NT, most = narrow_lds<MT, NT, WAVES, S>() + (th::NARROW_SCAN_SLOTS + 1) * 4;
   const uint64_t ntiles = th::ceil_div(a.n, BN);
   uint64_t mtiles = th::ceil_div(a.rows, BM), blocks;
@@ -289,22 +308,27 @@ hipError_t run(const MatArgs& a, hipStream_t s) {
     kernel<<<(uint32_t)blocks, 64 * WAVES, bytes, s>>>(a, shares);
     return hipGetLastError();
   };
-  if (a.u)
-    return a.aligned ? go(narrow_kernel<T, MT, NT, WAVES, S, true, true>) : go(narrow_kernel<T, MT, NT, WAVES, S, false, true>);
-  return a.aligned ? go(narrow_kernel<T, MT, NT, WAVES, S, true, false>) : go(narrow_kernel<T, MT, NT, WAVES, S, false, false>);
+  if (transposed)
+    return a.u ? go(narrow_kernel<T, MT, NT, WAVES, S, true, true, true>)
+               : go(narrow_kernel<T, MT, NT, WAVES, S, true, true, false>);
+  if (a.aligned)
+    return a.u ? go(narrow_kernel<T, MT, NT, WAVES, S, false, true, true>)
+               : go(narrow_kernel<T, MT, NT, WAVES, S, false, true, false>);
+  return a.u ? go(narrow_kernel<T, MT, NT, WAVES, S, false, false, true>)
+             : go(narrow_kernel<T, MT, NT, WAVES, S, false, false, false>);
 }
 
 template <class T>
-hipError_t typed(const MatArgs& a, hipStream_t s) {
+hipError_t typed(const MatArgs& a, int transposed, hipStream_t s) {
   switch (th::narrow_tile(a.rows, a.n, a.offsets || a.scan ? a.E : 1)) {
-    case th::NARROW_16x16: return run<T, 1, 1, 8, 2>(a, s);
-    case th::NARROW_32x16: return run<T, 2, 1, 8, 3>(a, s);
-    default: return run<T, 2, 2, 4, 2>(a, s);
+    case th::NARROW_16x16: return run<T, 1, 1, 8, 2>(a, transposed, s);
+    case th::NARROW_32x16: return run<T, 2, 1, 8, 3>(a, transposed, s);
+    default: return run<T, 2, 2, 4, 2>(a, transposed, s);
   }
 }
 
 }  // namespace
 
-hipError_t launch_narrow(MixType type, const MatArgs& a, hipStream_t s) {
-  return type == MIX_BF16 ? typed<bf16_t>(a, s) : typed<f16_t>(a, s);
+hipError_t launch_narrow(MixType type, const MatArgs& a, int transposed, hipStream_t s) {
+  return type == MIX_BF16 ? typed<bf16_t>(a, transposed, s) : typed<f16_t>(a, transposed, s);
 }

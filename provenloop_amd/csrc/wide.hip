@@ -164,6 +164,7 @@ hipError_t typed(const MatArgs& a, int transposed, hipStream_t s) {
 
 hipError_t launch_mat(MixType type, const MatArgs& a, int transposed, hipStream_t s) {
   if (a.rows == 0 || a.n == 0) return hipSuccess;
-  if (a.scan || (!transposed && th::narrow_product(a.rows, a.n, a.k, a.offsets ? a.E : 1))) return launch_narrow(type, a, s);
+  if (a.scan || ((!transposed || a.aligned) && th::narrow_product(a.rows, a.n, a.k, a.offsets ? a.E : 1)))
+    return launch_narrow(type, a, transposed, s);
   return type == MIX_BF16 ? typed<bf16_t>(a, transposed, s) : typed<f16_t>(a, transposed, s);
 }
