@@ -450,7 +450,23 @@ __global__ void __launch_bounds__(256) transpose_kernel(TransposePair pair) {
     tile[i / w][i % w] = ((const uint16_t*)a.in)[e * a.lde + (int64_t)(r0 + i / w) * a.ld + c0 + i % w];
   __syncthreads();
   for (uint32_t i = threadIdx.x; i < h * w; i += 256)
-    ((uint16_t*)a.out)[((int64_t)e * a.cols + c0 + i / h) * a.rows + r0 + i % h] = tile[i % h][i / h];
+    ((uint16_t*)a.out)[((int64_t)e * a.cols + c0 + i / h) * a.out_ld + r0 + i % h] = tile[i % h][i / h];
+  const uint32_t tail = r0 + 64 >= a.rows ? a.out_ld - a.rows : 0;
+  for (uint32_t i = threadIdx.x; i < tail * w; i += 256)
+    ((uint16_t*)a.out)[((int64_t)e * a.cols + c0 + i / tail) * a.out_ld + a.rows + i % tail] = 0;
+}
+
+// 8 values a thread.
+__global__ void __launch_bounds__(256) pad_kernel(PadSet set) {
+  const uint32_t which = (blockIdx.x >= set.blocks[0]) + (blockIdx.x >= set.blocks[1]);
+  const PadArgs& a = set.p[which];
+  const uint64_t i = (uint64_t)(blockIdx.x - (which ? set.blocks[which - 1] : 0)) * 256 + threadIdx.x;
+  const uint32_t chunks = (a.cols + 7) / 8;
+  const uint64_t row = i / chunks;
+  if (row >= (uint64_t)a.rows * a.E) return;
+  const uint32_t c = (uint32_t)(i % chunks) * 8;
+  const bf16_t* p = (const bf16_t*)a.in + (int64_t)(row / a.rows) * a.lde + (int64_t)(row % a.rows) * a.ld + c;
+  ((bf16x8*)a.out)[i] = load8<bf16_t>(p, (int64_t)a.cols - c);
 }
 
 // A thread: 8 columns of a token, or 1 where rows are no multiple of 8.
@@ -519,6 +535,16 @@ hipError_t launch_transpose(TransposePair pair, hipStream_t s) {
     if (a.out) blocks += (uint32_t)(th::ceil_div(a.rows, 64) * th::ceil_div(a.cols, 64) * a.E);
   }
   if (blocks) transpose_kernel<<<blocks, 256, 0, s>>>(pair);
+  return hipGetLastError();
+}
+
+hipError_t launch_pad(PadSet set, hipStream_t s) {
+  uint64_t blocks = 0;
+  for (int i = 0; i < 3; ++i) {
+    if (i) set.blocks[i - 1] = (uint32_t)blocks;
+    if (set.p[i].out) blocks += th::ceil_div((uint64_t)set.p[i].rows * set.p[i].E * th::ceil_div(set.p[i].cols, 8), 256);
+  }
+  if (blocks) pad_kernel<<<(uint32_t)blocks, 256, 0, s>>>(set);
   return hipGetLastError();
 }
 

@@ -56,7 +56,7 @@ struct MatArgs {
   int64_t rows;                 // rows of y
   uint32_t n, k, E, div;        // outputs, contraction length
   int y_float;                  // y holds floats (a workspace)
-  int aligned;                  // every row of x and w starts on 16 bytes and k (n, if transposed) is a multiple of 8
+  int aligned;                  // every row of x and w starts on 16 bytes and has a multiple of 8 values, or zeros up to one
   int scan;                     // no order or offsets: a slot's matrix is ids[slot], rows without one are not written
   // low-rank part: y_t += sum_j c_tj P[id_tj] u_tj over the token's choices
   // with P[e] = `p` + e * ldpe, n x r with row stride ldp
@@ -112,17 +112,32 @@ hipError_t launch_low_outer(MixType type, const LowOuterPair& pair, hipStream_t 
 
 // out (E x cols x rows) = transposes of E matrices of rows x cols; two stacks in
 // one launch, one without `out` is left out.
+// out_ld: the row stride of `out`, zeros from `rows` on.
 struct TransposeArgs {
   const void* in;
   void* out;
   int64_t ld, lde;
-  uint32_t E, rows, cols;
+  uint32_t E, rows, cols, out_ld;
 };
 struct TransposePair {
   TransposeArgs p[2];
   uint32_t blocks;  // of the first
 };
 hipError_t launch_transpose(TransposePair pair, hipStream_t s);
+// out = E matrices of rows x cols with rows of a multiple of 8 values, zeros
+// beyond cols; up to three stacks in one launch, one without `out` is left out.
+struct PadArgs {
+  const void* in;
+  void* out;
+  int64_t ld, lde;
+  uint32_t E, cols;
+  int64_t rows;
+};
+struct PadSet {
+  PadArgs p[3];
+  uint32_t blocks[2];  // up to the second, up to the third
+};
+hipError_t launch_pad(PadSet set, hipStream_t s);
 // out[t] = sum_j in[t k + j], rows of n floats
 hipError_t launch_sum_choices(MixType type, const float* in, void* out, int64_t tokens, uint32_t k, uint32_t n,
                               hipStream_t s);

@@ -109,7 +109,40 @@ void check_lora(const th_lora_linear_args* d) {
   need(d->tokens == 0 || (d->order == nullptr) == (d->offsets == nullptr), "order and offsets go together");
 }
 
+// A stack of matrices as the products read it: the caller's, or a copy with
+// rows of a multiple of 8 values, zeros beyond the caller's.
+struct Stack {
+  const void* p;
+  int64_t ld, lde;
+  uint32_t E, cols;
+  int64_t rows;
+  void* copy;
+  bool ready() const { return on16(p, ld, rows) && (E < 2 || lde % 8 == 0) && cols % 8 == 0; }
+  uint32_t padded() const { return (cols + 7) & ~7u; }
+  // A place for a copy, if rows of the product pay for it and the stack needs it.
+  void lay(Pieces& work, int64_t tokens, bool needed) {
+    if (needed && tokens > th::MIX_PAD_ROWS) copy = work.take<uint16_t>((uint64_t)E * rows * padded());
+  }
+  void use_copy() {
+    if (!copy) return;
+    cols = padded();
+    p = copy;
+    ld = cols;
+    lde = ld * rows;
+  }
+};
+void make_copies(Stack& a, Stack& b, Stack& c, hipStream_t s) {
+  PadSet set{};
+  Stack* all[3] = {&a, &b, &c};
+  for (int i = 0; i < 3; ++i) {
+    set.p[i] = PadArgs{all[i]->p, all[i]->copy, all[i]->ld, all[i]->lde, all[i]->E, all[i]->cols, all[i]->rows};
+    all[i]->use_copy();
+  }
+  HIPCHK(launch_pad(set, s));
+}
+
 struct LoraWork {
+  Stack x{}, weight{}, a{}, dy{};
   int32_t *order = nullptr, *offsets = nullptr;
   uint32_t* hist = nullptr;
   float *u = nullptr, *v = nullptr, *partial[2] = {};
@@ -122,6 +155,9 @@ bool scans(const th_lora_linear_args* d, bool keep_u) {
 }
 LoraWork lay_groups(Pieces& p, const th_lora_linear_args* d, bool own_lists = false) {
   LoraWork w;
+  w.x = Stack{d->x, d->ldx, 0, 1, d->d_in, d->tokens, nullptr};
+  w.weight = Stack{d->weight, d->ldw, 0, 1, d->d_in, d->d_out, nullptr};
+  w.a = Stack{d->a, d->lda, d->lda_adapter, d->adapters, d->d_in, d->rank, nullptr};
   if (!d->order && !own_lists) {
     w.order = p.take<int32_t>((uint64_t)d->tokens * d->choices);
     w.offsets = p.take<int32_t>(d->adapters + 1);
@@ -131,15 +167,19 @@ LoraWork lay_groups(Pieces& p, const th_lora_linear_args* d, bool own_lists = fa
 }
 LoraWork lay_forward(Pieces& p, const th_lora_linear_args* d, bool keep_u) {
   LoraWork w = lay_groups(p, d, scans(d, keep_u));
+  for (Stack* t : {&w.x, &w.weight, &w.a}) t->lay(p, d->tokens, !t->ready());
   if (!keep_u) w.u = p.take<float>((uint64_t)d->tokens * d->choices * padded_rank(d->rank));
   return w;
 }
-LoraWork lay_backward(Pieces& p, const th_lora_linear_args* d) {
+LoraWork lay_backward(Pieces& p, const th_lora_linear_args* d, const void* dy, int64_t lddy) {
   LoraWork w = lay_groups(p, d);
+  w.dy = Stack{dy, lddy, 0, 1, d->d_out, d->tokens, nullptr};
+  for (Stack* t : {&w.x, &w.weight}) t->lay(p, d->tokens, !t->ready());
+  w.dy.lay(p, d->tokens, d->d_out % 8 != 0);  // the workspace's size does not depend on where dy lies
   const uint64_t slots = (uint64_t)d->tokens * d->choices;
   w.v = p.take<float>(slots * padded_rank(d->rank));
   w.at = p.take<uint16_t>((uint64_t)d->adapters * d->d_in * d->rank);
-  w.bt = p.take<uint16_t>((uint64_t)d->adapters * d->d_out * d->rank);
+  w.bt = p.take<uint16_t>((uint64_t)d->adapters * w.dy.padded() * d->rank);
   for (int i = 0; i < 2; ++i) {
     const uint32_t cols = i ? d->d_out : d->d_in;
     w.partial[i] =
@@ -168,16 +208,16 @@ void make_groups(const th_lora_linear_args* d, LoraWork& w, hipStream_t s) {
 
 // low (slots x rank floats) = one low-rank factor of every slot's adapter times
 // its token's row of `wide`.
-void shrink(const th_lora_linear_args* d, const LoraWork& w, const void* wide, int64_t ldwide, uint32_t width,
-            const void* factor, int64_t ldf, int64_t ldfe, float* low, hipStream_t s) {
+void shrink(const th_lora_linear_args* d, const LoraWork& w, const Stack& wide, const Stack& factor, float* low,
+            hipStream_t s) {
   MatArgs m{};
   m.scan = w.offsets == nullptr;
   m.ids = d->experts;
-  m.x = wide;
-  m.ldx = ldwide;
-  m.w = factor;
-  m.ldw = ldf;
-  m.ldwe = ldfe;
+  m.x = wide.p;
+  m.ldx = wide.ld;
+  m.w = factor.p;
+  m.ldw = factor.ld;
+  m.ldwe = factor.lde;
   m.y = low;
   m.ldy = padded_rank(d->rank);
   m.y_float = 1;
@@ -185,10 +225,10 @@ void shrink(const th_lora_linear_args* d, const LoraWork& w, const void* wide, i
   m.offsets = w.offsets;
   m.rows = d->tokens * d->choices;
   m.n = d->rank;
-  m.k = width;
+  m.k = wide.cols;
   m.E = d->adapters;
   m.div = d->choices;
-  m.aligned = on16(wide, ldwide, d->tokens) && on16(factor, ldf) && ldfe % 8 == 0 && width % 8 == 0;
+  m.aligned = wide.ready() && factor.ready();
   HIPCHK(launch_mat((MixType)d->dtype, m, 0, s));
 }
 
@@ -410,20 +450,21 @@ int th_lora_linear(const th_lora_linear_args* d, void* y, int64_t ldy, float* u,
     const hipStream_t s = (hipStream_t)stream;
     float* low = u ? u : w.u;
     if (!scans(d, u != nullptr)) make_groups(d, w, s);
-    shrink(d, w, d->x, d->ldx, d->d_in, d->a, d->lda, d->lda_adapter, low, s);
+    make_copies(w.x, w.weight, w.a, s);
+    shrink(d, w, w.x, w.a, low, s);
     MatArgs m{};
-    m.x = d->x;
-    m.ldx = d->ldx;
-    m.w = d->weight;
-    m.ldw = d->ldw;
+    m.x = w.x.p;
+    m.ldx = w.x.ld;
+    m.w = w.weight.p;
+    m.ldw = w.weight.ld;
     m.y = y;
     m.ldy = ldy;
     m.bias = d->bias;
     m.rows = d->tokens;
     m.n = d->d_out;
-    m.k = d->d_in;
+    m.k = w.x.cols;
     m.div = 1;
-    m.aligned = on16(d->x, d->ldx, d->tokens) && on16(d->weight, d->ldw) && d->d_in % 8 == 0;
+    m.aligned = w.x.ready() && w.weight.ready();
     set_lowrank(m, d, low, d->b, d->ldb, d->ldb_adapter);
     HIPCHK(launch_mat((MixType)d->dtype, m, 0, s));
   });
@@ -434,7 +475,7 @@ int th_lora_linear_backward_workspace(const th_lora_linear_args* d, size_t* byte
     need(bytes != nullptr, "null output");
     check_lora(d);
     Pieces p(nullptr);
-    lay_backward(p, d);
+    lay_backward(p, d, nullptr, d->d_out);
     *bytes = p.used();
   });
 }
@@ -446,7 +487,7 @@ int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const 
     need_rows(dy, d->tokens, lddy, d->d_out, "dy");
     need(d->tokens == 0 || u != nullptr || !(db || dgate), "null u");
     Pieces p(work);
-    LoraWork w = lay_backward(p, d);
+    LoraWork w = lay_backward(p, d, dy, lddy);
     need_work(work, work_bytes, p.used());
     need_device();
     const hipStream_t s = (hipStream_t)stream;
@@ -454,26 +495,28 @@ int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const 
     const uint32_t ru = padded_rank(d->rank);
     const int64_t slots = d->tokens * d->choices;
     make_groups(d, w, s);
+    if (slots) make_copies(w.x, w.weight, w.dy, s);
     if (slots && (dx || da || dgate)) {
       TransposePair t{};
-      t.p[0] = TransposeArgs{d->b, w.bt, d->ldb, d->ldb_adapter, d->adapters, d->d_out, d->rank};
-      if (dx) t.p[1] = TransposeArgs{d->a, w.at, d->lda, d->lda_adapter, d->adapters, d->rank, d->d_in};
+      t.p[0] = TransposeArgs{d->b, w.bt, d->ldb, d->ldb_adapter, d->adapters, d->d_out, d->rank, w.dy.padded()};
+      if (dx) t.p[1] = TransposeArgs{d->a, w.at, d->lda, d->lda_adapter, d->adapters, d->rank, d->d_in, d->rank};
       HIPCHK(launch_transpose(t, s));
-      shrink(d, w, dy, lddy, d->d_out, w.bt, d->d_out, (int64_t)d->d_out * d->rank, w.v, s);
+      const uint32_t n = w.dy.padded();
+      shrink(d, w, w.dy, Stack{w.bt, n, (int64_t)n * d->rank, d->adapters, n, d->rank, nullptr}, w.v, s);
     }
     if (slots && dx) {
       MatArgs m{};
-      m.x = dy;
-      m.ldx = lddy;
-      m.w = d->weight;
-      m.ldw = d->ldw;
+      m.x = w.dy.p;
+      m.ldx = w.dy.ld;
+      m.w = w.weight.p;
+      m.ldw = w.weight.ld;
       m.y = dx;
       m.ldy = d->d_in;
       m.rows = d->tokens;
       m.n = d->d_in;
       m.k = d->d_out;
       m.div = 1;
-      m.aligned = on16(dy, lddy, d->tokens) && on16(d->weight, d->ldw) && d->d_in % 8 == 0 && d->d_out % 8 == 0;
+      m.aligned = w.dy.ready() && w.weight.ready();
       set_lowrank(m, d, w.v, w.at, d->rank, (int64_t)d->d_in * d->rank);
       HIPCHK(launch_mat(type, m, 1, s));
     }
@@ -482,8 +525,9 @@ int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const 
       for (int which = 0; which < 2; ++which) {
         LowOuterArgs& o = pair.p[which];
         o.low = which ? u : w.v;
-        o.wide = which ? dy : d->x;
-        o.ldwide = which ? lddy : d->ldx;
+        const Stack& wide = which ? w.dy : w.x;
+        o.wide = wide.p;
+        o.ldwide = wide.ld;
         o.cols = which ? d->d_out : d->d_in;
         o.out = which ? db : da;
         o.partial = w.partial[which];
@@ -497,7 +541,7 @@ int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const 
         o.E = d->adapters;
         o.div = d->choices;
         o.span = th::lowrank_span(slots, o.cols);
-        o.aligned = !o.out || (on16(o.wide, o.ldwide, d->tokens) && o.cols % 8 == 0);
+        o.aligned = !o.out || wide.ready();
         o.transposed = which;
       }
       HIPCHK(launch_low_outer(type, pair, s));

@@ -74,6 +74,10 @@ constexpr bool wide_square(uint64_t rows, uint32_t n, uint32_t groups) {
   const uint64_t m = groups * ceil_div(ceil_div(rows, groups), 256);
   return ceil_div(m * ceil_div(n, 256), 256) * 7 <= ceil_div(m * ceil_div(n, 128), 256) * 4;
 }
+// Rows from which operands that do not start on 16 bytes, or are no multiple of
+// 8 wide, are copied to ones that are: fewer rows read a weight but once, which
+// costs less than copying it (PAD_US).
+constexpr uint32_t MIX_PAD_ROWS = 32;
 // Slots whose adapters a workgroup of the low-rank product looks through by
 // itself, which saves the launch that would group them.
 constexpr uint32_t NARROW_SCAN_SLOTS = 2048;
