@@ -81,34 +81,6 @@ uint32_t padded_rank(uint32_t r) { return (r + 3) & ~3u; }
 // Rows of 2-byte elements that all start on 16 bytes.
 bool on16(const void* p, int64_t ld, int64_t rows = 2) { return ((uintptr_t)p & 15) == 0 && (rows < 2 || ld % 8 == 0); }
 
-// ---------------------------------------------------------------- grouped products
-void check_grouped(const th_grouped* d) {
-  need(d != nullptr, "null descriptor");
-  mix_type(d->dtype, false);
-  need_slots(d->tokens, d->experts, d->choices);
-  need(d->d_in >= 1 && d->d_out >= 1, "d_in and d_out must be positive");
-  need_rows(d->x, d->tokens, d->ldx, d->d_in, "x");
-  need(d->w != nullptr, "null w");
-  need(d->ldw >= d->d_in, "w: the row stride is shorter than a row");
-  need(d->tokens == 0 || (d->order && d->offsets), "null groups");
-}
-
-// ---------------------------------------------------------------- shared projection with adapters
-void check_lora(const th_lora_linear_args* d) {
-  need(d != nullptr, "null descriptor");
-  mix_type(d->dtype, false);
-  need_slots(d->tokens, d->adapters, d->choices);
-  need(d->d_in >= 1 && d->d_out >= 1, "d_in and d_out must be positive");
-  need(d->rank >= 1 && d->rank <= th::MIX_MAX_RANK, "rank must be in [1, " + std::to_string(th::MIX_MAX_RANK) + "]");
-  need_rows(d->x, d->tokens, d->ldx, d->d_in, "x");
-  need(d->weight && d->a && d->b, "null weight or adapter");
-  need(d->ldw >= d->d_in, "weight: the row stride is shorter than a row");
-  need(d->lda >= d->d_in, "a: the row stride is shorter than a row");
-  need(d->ldb >= d->rank, "b: the row stride is shorter than a row");
-  need(d->tokens == 0 || d->experts, "null experts");
-  need(d->tokens == 0 || (d->order == nullptr) == (d->offsets == nullptr), "order and offsets go together");
-}
-
 // A stack of matrices as the products read it: the caller's, or a copy with
 // rows of a multiple of 8 values, zeros beyond the caller's.
 struct Stack {
@@ -119,9 +91,8 @@ struct Stack {
   void* copy;
   bool ready() const { return on16(p, ld, rows) && (E < 2 || lde % 8 == 0) && cols % 8 == 0; }
   uint32_t padded() const { return (cols + 7) & ~7u; }
-  // A place for a copy, if rows of the product pay for it and the stack needs it.
-  void lay(Pieces& work, int64_t tokens, bool needed) {
-    if (needed && tokens > th::MIX_PAD_ROWS) copy = work.take<uint16_t>((uint64_t)E * rows * padded());
+  void lay(Pieces& work, bool needed) {
+    if (needed) copy = work.take<uint16_t>((uint64_t)E * rows * padded());
   }
   void use_copy() {
     if (!copy) return;
@@ -139,6 +110,50 @@ void make_copies(Stack& a, Stack& b, Stack& c, hipStream_t s) {
     all[i]->use_copy();
   }
   HIPCHK(launch_pad(set, s));
+}
+
+// ---------------------------------------------------------------- grouped products
+void check_grouped(const th_grouped* d) {
+  need(d != nullptr, "null descriptor");
+  mix_type(d->dtype, false);
+  need_slots(d->tokens, d->experts, d->choices);
+  need(d->d_in >= 1 && d->d_out >= 1, "d_in and d_out must be positive");
+  need_rows(d->x, d->tokens, d->ldx, d->d_in, "x");
+  need(d->w != nullptr, "null w");
+  need(d->ldw >= d->d_in, "w: the row stride is shorter than a row");
+  need(d->tokens == 0 || (d->order && d->offsets), "null groups");
+}
+
+struct GroupedWork {
+  Stack x{}, w{}, dy{};
+  float* part = nullptr;  // a token's choices, to be summed
+};
+GroupedWork lay_grouped_backward(Pieces& p, const th_grouped* d, const void* dy, int64_t lddy) {
+  GroupedWork g;
+  const int64_t slots = d->tokens * d->choices;
+  g.x = Stack{d->x, d->ldx, 0, 1, d->d_in, d->x_per_slot ? slots : d->tokens, nullptr};
+  g.w = Stack{d->w, d->ldw, d->ldwe, d->experts, d->d_in, d->d_out, nullptr};
+  g.dy = Stack{dy, lddy, 0, 1, d->d_out, slots, nullptr};
+  for (Stack* t : {&g.x, &g.w}) t->lay(p, !t->ready());
+  g.dy.lay(p, d->d_out % 8 != 0);  // the workspace's size does not depend on where dy lies
+  if (!d->x_per_slot && d->choices > 1) g.part = p.take<float>((uint64_t)slots * d->d_in);
+  return g;
+}
+
+// ---------------------------------------------------------------- shared projection with adapters
+void check_lora(const th_lora_linear_args* d) {
+  need(d != nullptr, "null descriptor");
+  mix_type(d->dtype, false);
+  need_slots(d->tokens, d->adapters, d->choices);
+  need(d->d_in >= 1 && d->d_out >= 1, "d_in and d_out must be positive");
+  need(d->rank >= 1 && d->rank <= th::MIX_MAX_RANK, "rank must be in [1, " + std::to_string(th::MIX_MAX_RANK) + "]");
+  need_rows(d->x, d->tokens, d->ldx, d->d_in, "x");
+  need(d->weight && d->a && d->b, "null weight or adapter");
+  need(d->ldw >= d->d_in, "weight: the row stride is shorter than a row");
+  need(d->lda >= d->d_in, "a: the row stride is shorter than a row");
+  need(d->ldb >= d->rank, "b: the row stride is shorter than a row");
+  need(d->tokens == 0 || d->experts, "null experts");
+  need(d->tokens == 0 || (d->order == nullptr) == (d->offsets == nullptr), "order and offsets go together");
 }
 
 struct LoraWork {
@@ -167,15 +182,15 @@ LoraWork lay_groups(Pieces& p, const th_lora_linear_args* d, bool own_lists = fa
 }
 LoraWork lay_forward(Pieces& p, const th_lora_linear_args* d, bool keep_u) {
   LoraWork w = lay_groups(p, d, scans(d, keep_u));
-  for (Stack* t : {&w.x, &w.weight, &w.a}) t->lay(p, d->tokens, !t->ready());
+  for (Stack* t : {&w.x, &w.weight, &w.a}) t->lay(p, d->tokens > th::MIX_PAD_ROWS && !t->ready());
   if (!keep_u) w.u = p.take<float>((uint64_t)d->tokens * d->choices * padded_rank(d->rank));
   return w;
 }
 LoraWork lay_backward(Pieces& p, const th_lora_linear_args* d, const void* dy, int64_t lddy) {
   LoraWork w = lay_groups(p, d);
   w.dy = Stack{dy, lddy, 0, 1, d->d_out, d->tokens, nullptr};
-  for (Stack* t : {&w.x, &w.weight}) t->lay(p, d->tokens, !t->ready());
-  w.dy.lay(p, d->tokens, d->d_out % 8 != 0);  // the workspace's size does not depend on where dy lies
+  for (Stack* t : {&w.x, &w.weight}) t->lay(p, !t->ready());
+  w.dy.lay(p, d->d_out % 8 != 0);  // the workspace's size does not depend on where dy lies
   const uint64_t slots = (uint64_t)d->tokens * d->choices;
   w.v = p.take<float>(slots * padded_rank(d->rank));
   w.at = p.take<uint16_t>((uint64_t)d->adapters * d->d_in * d->rank);
@@ -366,7 +381,7 @@ int th_grouped_matmul_backward_workspace(const th_grouped* d, size_t* bytes) {
     need(bytes != nullptr, "null output");
     check_grouped(d);
     Pieces p(nullptr);
-    if (!d->x_per_slot && d->choices > 1) p.take<float>((uint64_t)d->tokens * d->choices * d->d_in);
+    lay_grouped_backward(p, d, nullptr, d->d_out);
     *bytes = p.used();
   });
 }
@@ -379,20 +394,20 @@ int th_grouped_matmul_backward(const th_grouped* d, const void* dy, int64_t lddy
     const MixType type = (MixType)d->dtype;
     const bool summed = !d->x_per_slot && d->choices > 1;
     Pieces p(work);
-    float* part = nullptr;
-    if (dx && summed) part = p.take<float>((uint64_t)d->tokens * d->choices * d->d_in);
+    GroupedWork g = lay_grouped_backward(p, d, dy, lddy);
     need_work(work, work_bytes, p.used());
     need_device();
     const hipStream_t s = (hipStream_t)stream;
     const int64_t slots = d->tokens * d->choices;
+    if (slots) make_copies(g.x, g.w, g.dy, s);
     if (dx) {
       MatArgs m{};
-      m.x = dy;
-      m.ldx = lddy;
-      m.w = d->w;
-      m.ldw = d->ldw;
-      m.ldwe = d->ldwe;
-      m.y = summed ? (void*)part : dx;
+      m.x = g.dy.p;
+      m.ldx = g.dy.ld;
+      m.w = g.w.p;
+      m.ldw = g.w.ld;
+      m.ldwe = g.w.lde;
+      m.y = summed ? (void*)g.part : dx;
       m.y_float = summed;
       m.ldy = d->d_in;
       m.order = d->order;
@@ -402,16 +417,16 @@ int th_grouped_matmul_backward(const th_grouped* d, const void* dy, int64_t lddy
       m.k = d->d_out;
       m.E = d->experts;
       m.div = 1;
-      m.aligned = on16(dy, lddy) && on16(d->w, d->ldw) && d->ldwe % 8 == 0 && d->d_in % 8 == 0 && d->d_out % 8 == 0;
+      m.aligned = g.dy.ready() && g.w.ready();
       HIPCHK(launch_mat(type, m, 1, s));
-      if (summed) HIPCHK(launch_sum_choices(type, part, dx, d->tokens, d->choices, d->d_in, s));
+      if (summed) HIPCHK(launch_sum_choices(type, g.part, dx, d->tokens, d->choices, d->d_in, s));
     }
     if (dw) {
       OuterArgs o{};
-      o.dy = dy;
-      o.lddy = lddy;
-      o.x = d->x;
-      o.ldx = d->ldx;
+      o.dy = g.dy.p;
+      o.lddy = g.dy.ld;
+      o.x = g.x.p;
+      o.ldx = g.x.ld;
       o.out = dw;
       o.order = d->order;
       o.offsets = d->offsets;
@@ -420,7 +435,7 @@ int th_grouped_matmul_backward(const th_grouped* d, const void* dy, int64_t lddy
       o.k = d->d_in;
       o.E = d->experts;
       o.div = d->x_per_slot ? 1 : d->choices;
-      o.aligned = on16(dy, lddy) && on16(d->x, d->ldx) && d->d_in % 8 == 0 && d->d_out % 8 == 0;
+      o.aligned = g.dy.ready() && g.x.ready();
       need(d->offsets != nullptr, "null groups");
       HIPCHK(launch_outer(type, o, s));
     }
