@@ -102,6 +102,8 @@ Tensor experts_of(const char* name, const Tensor& experts) {
 // The gradients of a node are not differentiable themselves.
 variable_list once(variable_list grads) {
   if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& t : grads)
+    if (t.defined()) t.set_requires_grad(true);  // so that the error's node joins the graph
   auto error = std::make_shared<torch::autograd::DelayedError>(
       "the mixture operators' gradients are not differentiable a second time", (int64_t)grads.size());
   return (*error)(std::move(grads));
