@@ -462,7 +462,10 @@ typedef struct th_lora_linear_args {
   const int32_t* offsets;
 } th_lora_linear_args;
 /* u, if not NULL, receives A_e x_t of every slot in float (row stride: the rank
- * rounded up to 4), which the backward pass reads. */
+ * rounded up to 4; zeros for slots without an adapter), which the backward pass
+ * reads. The workspace's size depends on the descriptor's pointers and strides
+ * too: operands that do not start on 16 bytes, or are no multiple of 8 wide, are
+ * copied there, in the forward pass where that is faster. */
 int th_lora_linear_workspace(const th_lora_linear_args* d, int keep_u, size_t* bytes);
 int th_lora_linear(const th_lora_linear_args* d, void* y, int64_t ldy, float* u, void* work, size_t work_bytes,
                    void* stream);

@@ -88,8 +88,8 @@ hipError_t launch_outer(MixType type, const OuterArgs& a, hipStream_t s);
 
 // The low-rank gradients: out[e] = sum over the slots s of adapter e of
 // c_s low[s] (outer) wide[s / div], low: slots x r floats (row stride ru).
-// Partial sums of a few hundred slots each in `partial` (lowrank_partials
-// floats), added in slot order. transposed: out is E x cols x r.
+// Partial sums of a few hundred slots each in `partial` (lowrank_spans x r x
+// cols floats), added in slot order. transposed: out is E x cols x r.
 struct LowOuterArgs {
   const float* low;
   const void* wide;

@@ -182,7 +182,7 @@ LoraWork lay_groups(Pieces& p, const th_lora_linear_args* d, bool own_lists = fa
 }
 LoraWork lay_forward(Pieces& p, const th_lora_linear_args* d, bool keep_u) {
   LoraWork w = lay_groups(p, d, scans(d, keep_u));
-  for (Stack* t : {&w.x, &w.weight, &w.a}) t->lay(p, d->tokens > th::MIX_PAD_ROWS && !t->ready());
+  for (Stack* t : {&w.x, &w.weight, &w.a}) t->lay(p, th::pad_operands(d->tokens, d->d_in) && !t->ready());
   if (!keep_u) w.u = p.take<float>((uint64_t)d->tokens * d->choices * padded_rank(d->rank));
   return w;
 }

@@ -79,8 +79,10 @@ __device__ inline vec8<T> load8(const T* p, int64_t valid) {
 }
 
 // 16 bytes per lane from global memory to lds + 16 * lane, without a register.
-// The compiler does not know of it: arrived_barrier() waits for it. (It keeps
-// nothing of its own in m0 here, which it does not let an asm name as written.)
+// The compiler does not know of it: the arrived... functions wait for it, and
+// the compiler's own waits, which count fewer loads than there are, only wait
+// longer. (It keeps nothing of its own in m0 here, which it does not let an asm
+// name as written.)
 __device__ inline void load_lds16(const void* src, uint32_t lds) {
   asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory");
 }

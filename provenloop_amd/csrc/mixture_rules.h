@@ -74,10 +74,12 @@ constexpr bool wide_square(uint64_t rows, uint32_t n, uint32_t groups) {
   const uint64_t m = groups * ceil_div(ceil_div(rows, groups), 256);
   return ceil_div(m * ceil_div(n, 256), 256) * 7 <= ceil_div(m * ceil_div(n, 128), 256) * 4;
 }
-// Rows from which operands that do not start on 16 bytes, or are no multiple of
-// 8 wide, are copied to ones that are: fewer rows read a weight but once, which
-// costs less than copying it (PAD_US).
-constexpr uint32_t MIX_PAD_ROWS = 32;
+// Whether operands that do not start on 16 bytes, or are no multiple of 8 wide,
+// are copied to ones that are (as they are / copied, in us a call: 1 row of 3585
+// -> 3584 30 / 27, 16 rows 42 / 27; 1537 -> 1536, 1 row 17 / 14, 32 rows 27 / 17;
+// 203 -> 515, 1 row 8.6 / 12.1, 32 rows 10.3 / 12.4; 1427 rows of 1389 -> 544
+// 82 / 41): a short contraction of few rows does not pay for the launch.
+constexpr bool pad_operands(uint64_t rows, uint32_t k) { return rows > 32 || k >= 1024; }
 // Slots whose adapters a workgroup of the low-rank product looks through by
 // itself, which saves the launch that would group them.
 constexpr uint32_t NARROW_SCAN_SLOTS = 2048;

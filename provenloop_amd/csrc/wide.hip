@@ -6,9 +6,10 @@ using namespace mix;
 
 namespace {
 
-// The same for operands whose rows do not start on 16 bytes or whose widths
-// are not multiples of 8: tiles pass through registers, with loads that end at
-// a row's end.
+// wide_kernel's product for operands whose rows do not start on 16 bytes or
+// whose widths are not multiples of 8 (grouped products, which have no workspace
+// for copies, and small gradients): tiles pass through registers, with loads
+// that end at a row's end.
 template <class T, int BM, int BN, int WM, int WN, bool TR, bool LR>
 __global__ void __launch_bounds__(64 * WM * WN) unaligned_kernel(MatArgs a) {
   constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN;

@@ -55,3 +55,7 @@ def test_which_tiles(evaluate):
     assert evaluate([f"narrow_tile({r}, {n}, {g})" for r, n, g in tile]) == list(tile.values())
     square = {(8192, 3584, 1): 1, (4096, 1536, 1): 0, (16384, 3584, 8): 1, (8186, 1536, 16): 1, (8192, 8192, 1): 1}
     assert evaluate([f"wide_square({r}, {n}, {g})" for r, n, g in square]) == list(square.values())
+
+
+def test_which_operands_are_copied(evaluate):
+    assert evaluate([f"pad_operands({r}, {k})" for r, k in ((1, 203), (32, 1016), (33, 8), (1, 1024))]) == [0, 0, 1, 1]
