@@ -7,7 +7,8 @@ using namespace mix;
 namespace {
 
 // Slots whose rows a workgroup of low_outer_kernel holds in LDS: 64 KiB of the
-// wide operand and up to 64 KiB of ranks.
+// wide operand and up to 64 KiB of ranks, 80 KiB in all up to rank 16, so that a
+// CU holds two.
 constexpr int low_batch(int mr) { return mr <= 4 ? 256 : 128; }
 
 // ---------------------------------------------------------------- weight gradients
@@ -247,21 +248,35 @@ __global__ void __launch_bounds__(256) unaligned_outer_kernel(OuterArgs a) {
 }
 
 // ---------------------------------------------------------------- low-rank gradients
+__device__ inline void gate_grad(const GateGradArgs& a, uint32_t block) {
+  const int64_t s = (int64_t)block * 256 + threadIdx.x;
+  if (s >= a.slots) return;
+  const uint32_t e = (uint32_t)a.ids[s];
+  float d = 0;
+  if (e < a.E) {
+    for (uint32_t i = 0; i < a.r; ++i) d += a.u[s * a.ru + i] * a.v[s * a.ru + i];
+    if (a.scale) d *= a.scale[e];
+  }
+  a.out[s] = d;
+}
+
 // Partial sums over a span of one adapter's slots: 16 MR rows of the low-rank
 // factor (float, scaled, as a bf16 pair) by 128 columns of the wide operand,
 // BATCH slots at a time. Few flops and short contractions: what bounds it is the
 // chain slot -> row -> product, so a batch's loads all go out together, and the
-// CU's other workgroups run meanwhile. Both gradients share a launch: 8192 slots
-// of 8 rank-16 adapters by 1536 columns each way take 26 us (50 MB of gathered
-// rows, 10 us at a copy's rate) and 6 for adding the partial sums.
+// CU's other workgroups run meanwhile. Both gradients, and the gate's, share a launch: 8192 slots
+// of 8 rank-16 adapters by 1536 columns each way take 17.6 us (50 MB of gathered
+// rows, 10 us at a copy's rate; 26 with one workgroup a CU) and 6 for adding the
+// partial sums.
 template <class T, int MR, bool ALIGNED>
 __global__ void __launch_bounds__(256) low_outer_kernel(LowOuterPair pair) {
   constexpr int BATCH = low_batch(MR), BN = 128, R = 16 * MR;
   constexpr int JOBS = BATCH / 16;  // 1 KiB loads (4 slots) per wavefront and batch
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   char *wide = lds, *low[2] = {wide + BATCH * BN * 2, wide + BATCH * BN * 2 + BATCH * R * 2};
-  uint32_t* slot = (uint32_t*)(low[1] + BATCH * R * 2);
+  uint32_t* slot = (uint32_t*)low[1];  // until the low-rank rows come there
   const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (blockIdx.x >= pair.gate_from) return gate_grad(pair.gate, blockIdx.x - pair.gate_from);
   const bool second = blockIdx.x >= pair.blocks;
   const LowOuterArgs& a = pair.p[second];
   const uint32_t block = blockIdx.x - (second ? pair.blocks : 0), ctiles = (a.cols + BN - 1) / BN;
@@ -295,6 +310,7 @@ __global__ void __launch_bounds__(256) low_outer_kernel(LowOuterPair pair) {
       if constexpr (ALIGNED) load_lds16(p, lds0 + j * 1024);
       else *(vec8<T>*)(wide + (wave * JOBS + j) * 1024 + lane * 16) = load8<T>(p, in ? (int64_t)a.cols - col : 0);
     }
+    __syncthreads();
     if (threadIdx.x < BATCH) {
       const float* u = a.low + (int64_t)(s == ~0u ? 0 : s) * a.ru;
       const uint32_t limit = s == ~0u ? 0 : a.r;
@@ -404,7 +420,7 @@ __global__ void __launch_bounds__(256) low_sum_kernel(LowOuterPair pair) {
 
 template <class T, int MR>
 hipError_t run_low(const LowOuterPair& pair, uint32_t blocks, hipStream_t s) {
-  constexpr uint32_t bytes = low_batch(MR) * (128 * 2 + 2 * 16 * MR * 2 + 4);
+  constexpr uint32_t bytes = low_batch(MR) * (128 * 2 + 2 * 16 * MR * 2);
   auto go = [&](auto kernel) {
     static const hipError_t ready =
         hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
@@ -428,6 +444,8 @@ hipError_t low_outer_typed(LowOuterPair pair, hipStream_t s) {
     rows = max(rows, (uint32_t)min(th::ceil_div(threads, 256), (uint64_t)1024));
   }
   const LowOuterArgs& a = pair.p[pair.p[0].out ? 0 : 1];
+  pair.gate_from = blocks;
+  if (pair.gate.out) blocks += (uint32_t)th::ceil_div(pair.gate.slots, 256);
   if (blocks) {
     const hipError_t e = a.r <= 16   ? run_low<T, 1>(pair, blocks, s)
                          : a.r <= 32 ? run_low<T, 2>(pair, blocks, s)
@@ -492,19 +510,7 @@ __global__ void __launch_bounds__(256) sum_choices_kernel(const float* in, T* ou
   }
 }
 
-__global__ void __launch_bounds__(256) gate_grad_kernel(const float* u, const float* v, const int32_t* ids,
-                                                        const float* scale, float* out, int64_t slots, uint32_t r,
-                                                        uint32_t ru, uint32_t E) {
-  const int64_t s = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (s >= slots) return;
-  const uint32_t e = (uint32_t)ids[s];
-  float d = 0;
-  if (e < E) {
-    for (uint32_t i = 0; i < r; ++i) d += u[s * ru + i] * v[s * ru + i];
-    if (scale) d *= scale[e];
-  }
-  out[s] = d;
-}
+__global__ void __launch_bounds__(256) gate_grad_kernel(GateGradArgs a) { gate_grad(a, blockIdx.x); }
 
 }  // namespace
 
@@ -562,9 +568,8 @@ hipError_t launch_sum_choices(MixType type, const float* in, void* out, int64_t 
   return hipGetLastError();
 }
 
-hipError_t launch_gate_grad(const float* u, const float* v, const int32_t* ids, const float* scale, float* out,
-                            int64_t slots, uint32_t r, uint32_t ru, uint32_t E, hipStream_t s) {
-  if (!slots) return hipSuccess;
-  gate_grad_kernel<<<(uint32_t)th::ceil_div(slots, 256), 256, 0, s>>>(u, v, ids, scale, out, slots, r, ru, E);
+hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t s) {
+  if (!a.slots) return hipSuccess;
+  gate_grad_kernel<<<(uint32_t)th::ceil_div(a.slots, 256), 256, 0, s>>>(a);
   return hipGetLastError();
 }

@@ -103,10 +103,22 @@ struct LowOuterArgs {
   uint32_t r, ru, cols, E, div, span;  // span: slots of one partial sum
   int aligned, transposed;
 };
-// Two such sums with the same slots and ranks in one launch; one without `out` is left out.
+// out[s] = scale_e (u_s . v_s)
+struct GateGradArgs {
+  const float *u, *v;  // slots x ru
+  const int32_t* ids;
+  const float* scale;  // null, or per adapter
+  float* out;
+  int64_t slots;
+  uint32_t r, ru, E;
+};
+
+// Two such sums with the same slots and ranks, and the gate's gradient, in one
+// launch; what has no `out` is left out.
 struct LowOuterPair {
   LowOuterArgs p[2];
-  uint32_t blocks;  // of the first
+  GateGradArgs gate;
+  uint32_t blocks, gate_from;  // workgroups of the first, of both
 };
 hipError_t launch_low_outer(MixType type, const LowOuterPair& pair, hipStream_t s);
 
@@ -141,6 +153,4 @@ hipError_t launch_pad(PadSet set, hipStream_t s);
 // out[t] = sum_j in[t k + j], rows of n floats
 hipError_t launch_sum_choices(MixType type, const float* in, void* out, int64_t tokens, uint32_t k, uint32_t n,
                               hipStream_t s);
-// out[s] = scale_e (u_s . v_s)
-hipError_t launch_gate_grad(const float* u, const float* v, const int32_t* ids, const float* scale, float* out,
-                            int64_t slots, uint32_t r, uint32_t ru, uint32_t E, hipStream_t s);
+hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t s);

@@ -535,8 +535,10 @@ int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const 
       set_lowrank(m, d, w.v, w.at, d->rank, (int64_t)d->d_in * d->rank);
       HIPCHK(launch_mat(type, m, 1, s));
     }
+    GateGradArgs gate{u, w.v, d->experts, d->scale, dgate, slots, d->rank, ru, d->adapters};
     if (da || db) {
       LowOuterPair pair{};
+      pair.gate = gate;
       for (int which = 0; which < 2; ++which) {
         LowOuterArgs& o = pair.p[which];
         o.low = which ? u : w.v;
@@ -561,7 +563,7 @@ int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const 
       }
       HIPCHK(launch_low_outer(type, pair, s));
     }
-    if (dgate) HIPCHK(launch_gate_grad(u, w.v, d->experts, d->scale, dgate, slots, d->rank, ru, d->adapters, s));
+    if (dgate && !(da || db)) HIPCHK(launch_gate_grad(gate, s));
   });
 }
 

@@ -41,14 +41,17 @@ constexpr uint64_t lowrank_spans(uint64_t slots, uint32_t E, uint32_t span) {
   return slots / span + (E < slots ? E : slots);
 }
 
-// Products of few output tiles (narrow.hip). The tile: 16 rows where groups
+// Products of few output tiles (narrow.hip). 16 x 16 tiles take 8 wavefronts,
+// two workgroups a CU, while those are all there at once, and 4, five a CU, from
+// 512 on (8192 slots of 8 groups by 16 columns of 1536 steps: 521 tiles, 9.1 us
+// and 11.9 with 8). The tile: 16 rows where groups
 // have no more, or the output no more columns (8192 x 16 x 1536: 5.9 us, 6.1
 // with 32 rows), else 32; 32 columns once there are enough workgroups (32 x 3584
 // x 3584: 6.7 us with 16 columns, 7.7 with 32; 250 x 1536 x 1536: 9.0 and 6.7).
-enum NarrowTile { NARROW_16x16, NARROW_32x16, NARROW_32x32 };
+enum NarrowTile { NARROW_16x16, NARROW_32x16, NARROW_32x32, NARROW_16x16_MANY };
 constexpr NarrowTile narrow_tile(uint64_t rows, uint32_t n, uint32_t groups) {
   const uint64_t each = ceil_div(rows, groups);
-  if (each <= 16 || n <= 16) return NARROW_16x16;
+  if (each <= 16 || n <= 16) return groups * ceil_div(each, 16) * ceil_div(n, 16) < 512 ? NARROW_16x16 : NARROW_16x16_MANY;
   return groups * ceil_div(each, 32) * ceil_div(n, 32) < 192 ? NARROW_32x16 : NARROW_32x32;
 }
 // Whether a product is one of those: up to 1024 tiles of 32 x 32, about what the

@@ -322,6 +322,7 @@ template <class T>
 hipError_t typed(const MatArgs& a, int transposed, hipStream_t s) {
   switch (th::narrow_tile(a.rows, a.n, a.offsets || a.scan ? a.E : 1)) {
     case th::NARROW_16x16: return run<T, 1, 1, 8, 2>(a, transposed, s);
+    case th::NARROW_16x16_MANY: return run<T, 1, 1, 4, 2>(a, transposed, s);
     case th::NARROW_32x16: return run<T, 2, 1, 8, 3>(a, transposed, s);
     default: return run<T, 2, 2, 4, 2>(a, transposed, s);
   }

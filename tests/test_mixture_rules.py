@@ -51,7 +51,7 @@ def test_which_tiles(evaluate):
               (512, 3584, 3584, 1): 0, (1024, 1536, 1536, 1): 0, (8192, 3584, 3584, 1): 0, (8192, 32, 3584, 8): 1, (32, 512, 3584, 8): 1,
               (64, 4096, 512, 8): 0, (64, 3584, 3584, 8): 1}
     assert evaluate([f"narrow_product({r}, {n}, {k}, {g})" for r, n, k, g in narrow]) == list(narrow.values())
-    tile = {(1, 1536, 1): 0, (32, 512, 8): 0, (8192, 16, 8): 0, (32, 3584, 1): 1, (250, 1536, 1): 2, (1021, 256, 1): 2}
+    tile = {(1, 1536, 1): 0, (32, 512, 8): 0, (8192, 16, 8): 3, (4096, 16, 8): 0, (32, 3584, 1): 1, (250, 1536, 1): 2, (1021, 256, 1): 2}
     assert evaluate([f"narrow_tile({r}, {n}, {g})" for r, n, g in tile]) == list(tile.values())
     square = {(8192, 3584, 1): 1, (4096, 1536, 1): 0, (16384, 3584, 8): 1, (8186, 1536, 16): 1, (8192, 8192, 1): 1}
     assert evaluate([f"wide_square({r}, {n}, {g})" for r, n, g in square]) == list(square.values())
