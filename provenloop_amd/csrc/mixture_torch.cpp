@@ -116,9 +116,9 @@ std::tuple<Tensor, Tensor, Tensor> group(const Tensor& given, int64_t n) {
   NEED(n >= 1 && n <= 1 << 30, "group: the number of groups must be positive");
   Guard guard(experts.device());
   const int64_t t = experts.size(0), k = experts.size(1);
-  Tensor order = make({t * k}, at::kInt, experts), offsets = make({n + 1}, at::kInt, experts);
   size_t bytes;
-  check(th_group_workspace(t, (uint32_t)n, (uint32_t)k, &bytes));
+  check(th_group_workspace(t, (uint32_t)n, (uint32_t)k, &bytes));  // refuses what is out of range
+  Tensor order = make({t * k}, at::kInt, experts), offsets = make({n + 1}, at::kInt, experts);
   const Work w = work(bytes, experts);
   check(th_group(ptr<int32_t>(experts), t, (uint32_t)n, (uint32_t)k, ptr<int32_t>(order), ptr<int32_t>(offsets), w.p,
                  w.bytes, stream(experts)));
