@@ -5,6 +5,8 @@
 // holds row (column) l % 16 of each operand, contraction steps
 // (l / 16) * 8 .. + 8, and of the result column l % 16, rows (l / 16) * 4 .. + 4.
 #pragma once
+#include <type_traits>
+
 #include "mixture.h"
 
 typedef __attribute__((ext_vector_type(4))) float f32x4;
@@ -45,6 +47,24 @@ __device__ inline void split8(const f32x8& v, bf16x8& hi, bf16x8& lo) {
     hi[i] = (bf16_t)v[i];
     lo[i] = (bf16_t)(v[i] - (float)hi[i]);
   }
+}
+
+// Infinities and NaN among 16-bit values: all exponent bits set.
+template <class T>
+constexpr uint32_t exponent_bits() {
+  return std::is_same<T, bf16_t>::value ? 0x7f80 : 0x7c00;
+}
+template <class T>
+__device__ inline bool is_finite(T v) {
+  return (__builtin_bit_cast(uint16_t, v) & exponent_bits<T>()) != exponent_bits<T>();
+}
+// Adding the exponent's lowest bit to a full exponent carries into the sign's place.
+template <class T>
+__device__ inline bool all_finite(const vec8<T>& v) {
+  constexpr uint32_t full = exponent_bits<T>(), one = full & -full;
+  const uint4 d = __builtin_bit_cast(uint4, v);
+  auto carry = [](uint32_t w) { return (w & (full << 16 | full)) + (one << 16 | one); };
+  return ((carry(d.x) | carry(d.y) | carry(d.z) | carry(d.w)) & 0x80008000u) == 0;
 }
 
 // acc += a * b with b given as floats split in two; an f16 operand is split

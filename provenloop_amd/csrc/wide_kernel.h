@@ -74,6 +74,58 @@ __device__ inline void list_adapters(const MatArgs& a, int64_t m0, int64_t mend,
   __syncthreads();
 }
 
+// Coefficient of choice `s` of the tile (row x choices + j), which uses adapter e.
+template <int BM>
+__device__ inline float coefficient(const MatArgs& a, int64_t m0, const LowLists<BM>& l, uint32_t s, uint32_t e) {
+  if (a.kc <= KEPT) return l.c[s];
+  return (a.gate ? a.gate[m0 * a.kc + s] : 1.0f) * (a.scale ? a.scale[e] : 1.0f);
+}
+template <int BM>
+__device__ inline uint32_t adapter_of(const MatArgs& a, int64_t m0, const LowLists<BM>& l, uint32_t s) {
+  return a.kc <= KEPT ? l.id[s] : (uint32_t)a.ids[m0 * a.kc + s];
+}
+
+// The products that add_lowrank leaves out, those of infinities and NaN, for a
+// wavefront's TM x TN outputs: each row's own adapters alone, one output at a
+// time in float, through the wavefront's own LDS in two halves. -0 where there
+// is none, which changes no sum.
+template <class T, int BM, int TM, int TN>
+__device__ inline void add_nonfinite(const MatArgs& a, int64_t m0, uint32_t rows, uint32_t row0, uint32_t n0, float* own,
+                                     const LowLists<BM>& l, uint32_t lane, f32x4 (&acc)[TN / 16][TM / 16]) {
+  constexpr int SLAB = TM / 2;
+#pragma unroll
+  for (int s0 = 0; s0 < TM; s0 += SLAB) {
+#pragma unroll 1
+    for (uint32_t i = lane; i < SLAB * TN; i += 64) {
+      const uint32_t row = row0 + s0 + i / TN, n = n0 + i % TN;
+      float sum = -0.0f;
+      for (uint32_t j = 0; row < rows && n < a.n && j < a.kc; ++j) {
+        const uint32_t s = row * a.kc + j, e = adapter_of(a, m0, l, s);
+        if (e >= a.E) continue;
+        const T* p = (const T*)a.p + e * a.ldpe + (int64_t)n * a.ldp;
+        const float* u = a.u + (m0 * a.kc + s) * a.ru;
+        float d = 0;
+        bool any = false;
+#pragma unroll 1
+        for (uint32_t q = 0; q < a.r; ++q)
+          if (!is_finite(p[q])) {
+            d = fmaf(u[q], (float)p[q], d);
+            any = true;
+          }
+        if (any) sum += coefficient(a, m0, l, s, e) * d;
+      }
+      own[i] = sum;
+    }
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll
+    for (int mi = s0 / 16; mi < (s0 + SLAB) / 16; ++mi)
+#pragma unroll
+      for (int ni = 0; ni < TN / 16; ++ni)
+        acc[ni][mi] += *(const f32x4*)&own[(mi * 16 - s0 + lane % 16) * TN + ni * 16 + lane / 16 * 4];
+    __builtin_amdgcn_wave_barrier();
+  }
+}
+
 template <class T, int BM, int BN, int WM, int WN>
 __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, uint32_t n0, char* lds,
                                    const LowLists<BM>& l, f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
@@ -85,6 +137,7 @@ __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, u
   const uint32_t rows = (uint32_t)(mend - m0);
   const uint32_t each = (a.r + 7) / 8, chunks = l.count * each;  // chunks of 8 ranks
   const uint32_t piece = threadIdx.x % 8;                        // this thread's chunk of a set, in all its rows
+  bool odd = false;                                              // it has left out an infinity or NaN
   for (uint32_t c0 = 0; c0 < chunks; c0 += 8) {
     const uint32_t c = c0 + piece, e = c < chunks ? l.list[c / each] : ~1u, r0 = c % each * 8;
     const bool whole = r0 + 8 <= a.r;
@@ -100,13 +153,9 @@ __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, u
       if (row < rows && c < chunks) {
         for (uint32_t j = 0; j < a.kc; ++j) {  // an adapter chosen twice counts with both coefficients
           const uint32_t s = row * a.kc + j;
-          uint32_t id;
-          if (a.kc <= KEPT) id = l.id[s];
-          else id = (uint32_t)a.ids[m0 * a.kc + s];
-          if (id != e) continue;
+          if (adapter_of(a, m0, l, s) != e) continue;
           at = s;
-          if (a.kc <= KEPT) f[i] += l.c[s];
-          else f[i] += (a.gate ? a.gate[m0 * a.kc + s] : 1.0f) * (a.scale ? a.scale[e] : 1.0f);
+          f[i] += coefficient(a, m0, l, s, e);
         }
       }
       if (at != ~0u) {
@@ -142,6 +191,10 @@ __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, u
 #pragma unroll
     for (int i = 0; i < WI; ++i) {
       const uint32_t row = i * (THREADS / 8) + threadIdx.x / 8, at = row * 128 + (piece ^ (row & 7)) * 16;
+      if (!all_finite<T>(v[i])) {
+        odd = true;
+        for (int q = 0; q < 8; ++q) v[i][q] = is_finite(v[i][q]) ? v[i][q] : (T)0.0f;
+      }
       if constexpr (PAIR) {
         const SplitF16 s = widen(v[i]);
         *(bf16x8*)(whi + at) = s.hi;
@@ -174,6 +227,8 @@ __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, u
       }
     }
   }
+  if (__syncthreads_or(odd))
+    add_nonfinite<T, BM, TM, TN>(a, m0, rows, wm * TM, n0 + wn * TN, (float*)(lds + wave * (TM * TN * 2)), l, lane, acc);
 }
 template <class T, int BM, int BN>
 constexpr uint32_t lowrank_lds() {

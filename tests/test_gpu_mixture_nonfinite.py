@@ -1,0 +1,97 @@
+"""Infinities and NaN in one adapter, token or coefficient: where the definition has them, and nowhere else.
+
+The oracle takes every adapter's own rows alone, in 64 bits on the CPU, so that
+nothing is multiplied that the definition does not multiply. Tolerances of the
+finite outputs as in test_gpu_mixture.py.
+"""
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from provenloop_amd import mixture  # noqa: E402
+from test_gpu_mixture import TYPES, choices, gen, near, normal  # noqa: E402
+
+INF, NAN = float("inf"), float("nan")
+
+# t, adapters, choices, d_in, d_out, rank: large tiles of both shapes each way, more choices than a tile lists, small tiles
+SIZES = [(2100, 5, 1, 72, 560, 16), (2100, 5, 2, 560, 72, 33), (2200, 9, 6, 136, 1040, 9), (8000, 6, 2, 72, 1100, 20),
+         (8000, 3, 1, 1100, 88, 8), (300, 4, 2, 72, 88, 12), (40, 4, 2, 264, 136, 16)]
+
+
+def low_rank(x, a, b, ids, gate, scale):
+    """sum_j gate_tj scale_e b_e (a_e x_t) over each token's own adapters, and its magnitude."""
+    x, a, b, ids = x.detach().cpu().double(), a.detach().cpu().double(), b.detach().cpu().double(), ids.cpu()
+    y, size = torch.zeros(len(x), b.shape[1], dtype=torch.float64), torch.zeros(len(x), b.shape[1], dtype=torch.float64)
+    for e in range(a.shape[0]):
+        for j in range(ids.shape[1]):
+            rows = torch.nonzero(ids[:, j] == e)[:, 0]
+            if len(rows):
+                c = (gate[rows, j].detach().cpu().double() if gate is not None else torch.ones(len(rows), dtype=torch.float64))[:, None]
+                c = c * float(scale[e]) if scale is not None else c
+                y[rows] += c * ((x[rows] @ a[e].t()) @ b[e].t())
+                size[rows] += c.abs() * ((x[rows].abs() @ a[e].abs().t()) @ b[e].abs().t())
+    return y.cuda(), size.cuda()
+
+
+def agrees(got, want, magnitude, n, low):
+    """The same infinities and NaN, and the finite values within their tolerance."""
+    fine = torch.isfinite(want)
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(got[torch.isinf(want)].double(), want[torch.isinf(want)])
+    near(got[fine], want[fine], magnitude[fine], n, low[fine])
+
+
+def case(t, e, k, din, dout, rank, dtype):
+    g, dt = gen(t + dout), TYPES[dtype]
+    c = dict(x=normal(g, t, din, dtype=dt), w=normal(g, dout, din, dtype=dt, std=din ** -0.5),
+             a=normal(g, e, rank, din, dtype=dt, std=din ** -0.5), b=normal(g, e, dout, rank, dtype=dt, std=0.3),
+             ids=choices(g, t, e, k), gate=torch.rand(t, k, generator=g, device="cuda"),
+             scale=torch.rand(e, generator=g, device="cuda") + 0.5, dy=normal(g, t, dout, dtype=dt))
+    return c
+
+
+def passes(c):
+    """(y, y without a graph, dx)"""
+    x = c["x"].clone().requires_grad_()
+    y = mixture.lora_linear(x, c["w"], c["a"], c["b"], c["ids"], weights=c["gate"], scale=c["scale"])
+    dx, = torch.autograd.grad(y, x, c["dy"])
+    with torch.no_grad():
+        return y.detach(), mixture.lora_linear(c["x"], c["w"], c["a"], c["b"], c["ids"], weights=c["gate"], scale=c["scale"]), dx
+
+
+def check_forward(c, got):
+    x, w = c["x"].double().cpu(), c["w"].double().cpu()
+    low, size = low_rank(c["x"], c["a"], c["b"], c["ids"], c["gate"], c["scale"])
+    main, whole = (x @ w.t()).cuda(), (x.abs() @ w.abs().t()).cuda()
+    agrees(got, main + low, whole + size, c["x"].shape[1] + c["a"].shape[1] * c["ids"].shape[1], size)
+
+
+def check_dx(c, got):
+    dy, w = c["dy"].double().cpu(), c["w"].double().cpu()
+    low, size = low_rank(c["dy"], c["b"].transpose(1, 2), c["a"].transpose(1, 2), c["ids"], c["gate"], c["scale"])
+    main, whole = (dy @ w).cuda(), (dy.abs() @ w.abs()).cuda()
+    agrees(got, main + low, whole + size, c["dy"].shape[1] + c["a"].shape[1] * c["ids"].shape[1], size)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_a_bad_adapter_stays_with_its_tokens(sizes, dtype):
+    """Infinities and NaN in the B (and, for dx, the A) of an adapter in use: other tokens' rows are bit for bit what
+    they are without them."""
+    c = case(*sizes, dtype)
+    clean = passes(c)
+    e = 1
+    mine = (c["ids"] == e).any(1)
+    assert mine.any() and not mine.all()
+    bad = dict(c, b=c["b"].clone())
+    bad["b"][e, 3, 0], bad["b"][e, 10, -1], bad["b"][e, 11, 1], bad["b"][e, -1, 2] = INF, NAN, -INF, INF
+    y, served, _ = passes(bad)
+    for got, was in ((y, clean[0]), (served, clean[1])):
+        assert torch.equal(got[~mine], was[~mine])
+        check_forward(bad, got)
+    bad = dict(c, a=c["a"].clone())
+    bad["a"][e, 0, 5], bad["a"][e, -1, 8], bad["a"][e, 1, -1] = INF, NAN, -INF
+    dx = passes(bad)[2]
+    assert torch.equal(dx[~mine], clean[2][~mine])
+    check_dx(bad, dx)
