@@ -67,6 +67,16 @@ __device__ inline bool all_finite(const vec8<T>& v) {
   return ((carry(d.x) | carry(d.y) | carry(d.z) | carry(d.w)) & 0x80008000u) == 0;
 }
 
+// Whether every value's high part is finite: those from half a step above
+// bf16's largest on round to infinity, and the low part would be the infinity
+// of the other sign.
+__device__ inline bool splits(float v) { return (__float_as_uint(v) & 0x7fffffff) < 0x7f7f8000; }
+__device__ inline bool all_split(const f32x8& v) {
+  uint32_t most = 0;
+  for (int i = 0; i < 8; ++i) most = max(most, __float_as_uint(v[i]) & 0x7fffffff);
+  return most < 0x7f7f8000;
+}
+
 // acc += a * b with b given as floats split in two; an f16 operand is split
 // too (11 bits, exact in the pair), a bf16 one needs no low part.
 __device__ inline f32x4 mfma_split(bf16x8 a, bf16x8 hi, bf16x8 lo, f32x4 c) { return mfma(a, hi, mfma(a, lo, c)); }

@@ -26,6 +26,12 @@ __device__ inline void arrived_but(void) {
 // more product with the low halves costs little next to the main one, and
 // rounding u once to bf16 would be as large an error as rounding y.
 //
+// A row's zeros meet the columns of adapters that it does not use, so an
+// infinity or NaN among those would make NaN of it; and an infinity times the
+// two parts of a pair, or an infinite coefficient's parts, are infinities of
+// both signs. They are laid as zeros too, and what they add to the rows that do
+// use them is made by add_nonfinite.
+//
 // list_adapters runs under the main product's first loads and leaves in LDS the
 // adapters and, for up to KEPT choices, each row's and its coefficients; the
 // loads of one set of 64 ranks then go out together. 4096 x 1536 x 1536 with two
@@ -85,10 +91,10 @@ __device__ inline uint32_t adapter_of(const MatArgs& a, int64_t m0, const LowLis
   return a.kc <= KEPT ? l.id[s] : (uint32_t)a.ids[m0 * a.kc + s];
 }
 
-// The products that add_lowrank leaves out, those of infinities and NaN, for a
-// wavefront's TM x TN outputs: each row's own adapters alone, one output at a
-// time in float, through the wavefront's own LDS in two halves. -0 where there
-// is none, which changes no sum.
+// The products that add_lowrank leaves out, those of infinities and NaN and of
+// coefficients that make no finite pair, for a wavefront's TM x TN outputs: each
+// row's own adapters alone, one output at a time in float, through the
+// wavefront's own LDS in two halves. -0 where there is none, which changes no sum.
 template <class T, int BM, int TM, int TN>
 __device__ inline void add_nonfinite(const MatArgs& a, int64_t m0, uint32_t rows, uint32_t row0, uint32_t n0, float* own,
                                      const LowLists<BM>& l, uint32_t lane, f32x4 (&acc)[TN / 16][TM / 16]) {
@@ -104,11 +110,13 @@ __device__ inline void add_nonfinite(const MatArgs& a, int64_t m0, uint32_t rows
         if (e >= a.E) continue;
         const T* p = (const T*)a.p + e * a.ldpe + (int64_t)n * a.ldp;
         const float* u = a.u + (m0 * a.kc + s) * a.ru;
-        float d = 0;
+        float f = 0, d = 0;  // f: what add_lowrank took for this adapter's coefficient
+        for (uint32_t i = 0; i < a.kc; ++i)
+          if (adapter_of(a, m0, l, row * a.kc + i) == e) f += coefficient(a, m0, l, row * a.kc + i, e);
         bool any = false;
 #pragma unroll 1
         for (uint32_t q = 0; q < a.r; ++q)
-          if (!is_finite(p[q])) {
+          if (!is_finite(p[q]) || !splits(f * u[q])) {
             d = fmaf(u[q], (float)p[q], d);
             any = true;
           }
@@ -137,7 +145,7 @@ __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, u
   const uint32_t rows = (uint32_t)(mend - m0);
   const uint32_t each = (a.r + 7) / 8, chunks = l.count * each;  // chunks of 8 ranks
   const uint32_t piece = threadIdx.x % 8;                        // this thread's chunk of a set, in all its rows
-  bool odd = false;                                              // it has left out an infinity or NaN
+  bool odd = false;                                              // it has left something out
   for (uint32_t c0 = 0; c0 < chunks; c0 += 8) {
     const uint32_t c = c0 + piece, e = c < chunks ? l.list[c / each] : ~1u, r0 = c % each * 8;
     const bool whole = r0 + 8 <= a.r;
@@ -183,6 +191,10 @@ __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, u
       f32x8 x;
 #pragma unroll
       for (int q = 0; q < 8; ++q) x[q] = f[i] * (q < 4 ? u0[i] : u1[i])[q % 4];
+      if (!all_split(x)) {
+        odd = true;
+        for (int q = 0; q < 8; ++q) x[q] = splits(x[q]) ? x[q] : 0.0f;
+      }
       bf16x8 hi, lo;
       split8(x, hi, lo);
       *(bf16x8*)(xhi + at) = hi;

@@ -95,3 +95,41 @@ def test_a_bad_adapter_stays_with_its_tokens(sizes, dtype):
     dx = passes(bad)[2]
     assert torch.equal(dx[~mine], clean[2][~mine])
     check_dx(bad, dx)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes", SIZES)
+def test_infinite_coefficients(sizes, dtype):
+    """An infinite, or no, number in a token, in its weights or in what A makes of it: infinities where the definition has them."""
+    c = case(*sizes, dtype)
+    clean = passes(c)
+    t = len(c["x"])
+    touched = torch.zeros(t, dtype=torch.bool, device="cuda")
+    bad = dict(c, gate=c["gate"].clone(), x=c["x"].clone(), dy=c["dy"].clone())
+    for i, (what, value) in enumerate((("gate", INF), ("gate", -INF), ("gate", NAN), ("x", INF), ("x", NAN), ("dy", -INF), ("dy", NAN))):
+        bad[what][3 * i + 1, 0] = value
+        touched[3 * i + 1] = True
+    for got, was, check in zip(passes(bad), clean, (check_forward, check_forward, check_dx)):
+        assert torch.equal(got[~touched], was[~touched])
+        check(bad, got)
+    bad = dict(c, a=c["a"].clone())  # every token of one adapter has an infinite rank
+    bad["a"][1, 0, 5] = INF
+    for got in passes(bad)[:2]:
+        check_forward(bad, got)
+    bad = dict(c, b=c["b"].clone())
+    bad["b"][1, 3, 0] = -INF
+    check_dx(bad, passes(bad)[2])
+
+
+@pytest.mark.parametrize("sizes", SIZES)
+def test_coefficients_near_the_largest_float(sizes):
+    """Products of weight and coefficient at and beyond float's range, brought back by a small factor."""
+    c = case(*sizes, "bf16")
+    c["a"], c["b"] = c["a"] * 0.125, c["b"] * 0.125
+    c["gate"][::7] = 3e38
+    c["gate"][1::7] = -1.5e38
+    c["scale"][:] = 1
+    y, served, dx = passes(c)
+    check_forward(c, y)
+    check_forward(c, served)
+    check_dx(c, dx)
