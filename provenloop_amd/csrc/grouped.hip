@@ -268,21 +268,21 @@ __device__ inline void gate_grad(const GateGradArgs& a, uint32_t block) {
 // of 8 rank-16 adapters by 1536 columns each way take 17.6 us (50 MB of gathered
 // rows, 10 us at a copy's rate; 26 with one workgroup a CU) and 6 for adding the
 // partial sums.
-template <class T, int MR, bool ALIGNED>
-__global__ void __launch_bounds__(256) low_outer_kernel(LowOuterPair pair) {
+//
+// Where a sum is no finite number, the span is taken again with coefficients
+// that round to infinity as bf16's largest and the rest, and, if infinities or
+// NaN are left, once more by the high parts alone (mfma_high): a span has one
+// adapter, so its other sums and other adapters' do not change.
+//
+// One pass over a span: its 16 MR x 128 partial sums, or, after the first, those
+// of them that are no finite numbers yet. Whether there are any of those.
+template <class T, int MR, bool ALIGNED, int PASS>
+__device__ inline bool low_span(const LowOuterArgs& a, const GroupTile& g, uint32_t span, uint32_t c0, char* lds, uint32_t lane,
+                                uint32_t wave) {
   constexpr int BATCH = low_batch(MR), BN = 128, R = 16 * MR;
   constexpr int JOBS = BATCH / 16;  // 1 KiB loads (4 slots) per wavefront and batch
-  extern __shared__ __attribute__((aligned(1024))) char lds[];
   char *wide = lds, *low[2] = {wide + BATCH * BN * 2, wide + BATCH * BN * 2 + BATCH * R * 2};
   uint32_t* slot = (uint32_t*)low[1];  // until the low-rank rows come there
-  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  if (blockIdx.x >= pair.gate_from) return gate_grad(pair.gate, blockIdx.x - pair.gate_from);
-  const bool second = blockIdx.x >= pair.blocks;
-  const LowOuterArgs& a = pair.p[second];
-  const uint32_t block = blockIdx.x - (second ? pair.blocks : 0), ctiles = (a.cols + BN - 1) / BN;
-  const uint32_t c0 = block % ctiles * BN, span = block / ctiles;
-  const GroupTile g = find_group_tile(a.offsets, a.E, a.E, a.slots, a.span, span, lane);
-  if (g.begin >= g.end) return;
   const char* zero = (const char*)&mix_zero16;
   f32x4 acc[MR][2];
 #pragma unroll
@@ -325,7 +325,8 @@ __global__ void __launch_bounds__(256) low_outer_kernel(LowOuterPair pair) {
             if (q + x < (int)limit) v[x] = c * u[q + x];
         }
         bf16x8 hi, lo;
-        split8(v, hi, lo);
+        if constexpr (PASS == 0) split8(v, hi, lo);
+        else split8_any(v, hi, lo);
         const uint32_t at = threadIdx.x * (R * 2) + ((q / 8) ^ tr_swizzle<R>(threadIdx.x)) * 16;
         *(bf16x8*)(low[0] + at) = hi;
         *(bf16x8*)(low[1] + at) = lo;
@@ -342,11 +343,14 @@ __global__ void __launch_bounds__(256) low_outer_kernel(LowOuterPair pair) {
         const bf16x8 hi = tr_fragment<bf16_t, R>(low[0], m * 16, k, lane);
         const bf16x8 lo = tr_fragment<bf16_t, R>(low[1], m * 16, k, lane);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) acc[m][i] = mfma_split(wf[i], hi, lo, acc[m][i]);
+        for (int i = 0; i < 2; ++i)
+          if constexpr (PASS < 2) acc[m][i] = mfma_split(wf[i], hi, lo, acc[m][i]);
+          else acc[m][i] = mfma_high(wf[i], hi, acc[m][i]);
       }
     }
   }
   // a lane: row lane % 16 of the low-rank factor, 4 neighbouring columns
+  bool odd = false;
 #pragma unroll
   for (int m = 0; m < MR; ++m)
 #pragma unroll
@@ -354,13 +358,37 @@ __global__ void __launch_bounds__(256) low_outer_kernel(LowOuterPair pair) {
       const uint32_t q = m * 16 + lane % 16, c = c0 + wave * 32 + i * 16 + lane / 16 * 4;
       if (q >= a.r) continue;
       float* o = a.partial + ((int64_t)span * a.r + q) * a.cols + c;
-      if (c + 4 <= a.cols && a.cols % 4 == 0) {
+      if (PASS == 0 && c + 4 <= a.cols && a.cols % 4 == 0) {
         *(f32x4*)o = acc[m][i];
       } else {
         for (int x = 0; x < 4; ++x)
-          if (c + x < a.cols) o[x] = acc[m][i][x];
+          if (c + x < a.cols && (PASS == 0 || !isfinite(o[x]))) o[x] = acc[m][i][x];
       }
+      for (int x = 0; x < 4; ++x) odd |= !isfinite(acc[m][i][x]);
     }
+  // (__syncthreads_or would take LDS of its own, and the CU's second workgroup with it)
+  uint32_t* flag = (uint32_t*)wide;
+  odd = __ballot(odd);
+  __syncthreads();
+  if (lane == 0) flag[wave] = odd;
+  __syncthreads();
+  return flag[0] | flag[1] | flag[2] | flag[3];
+}
+
+template <class T, int MR, bool ALIGNED>
+__global__ void __launch_bounds__(256) low_outer_kernel(LowOuterPair pair) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  if (blockIdx.x >= pair.gate_from) return gate_grad(pair.gate, blockIdx.x - pair.gate_from);
+  const bool second = blockIdx.x >= pair.blocks;
+  const LowOuterArgs& a = pair.p[second];
+  const uint32_t block = blockIdx.x - (second ? pair.blocks : 0), ctiles = (a.cols + 127) / 128;
+  const uint32_t c0 = block % ctiles * 128, span = block / ctiles;
+  const GroupTile g = find_group_tile(a.offsets, a.E, a.E, a.slots, a.span, span, lane);
+  if (g.begin >= g.end) return;
+  if (low_span<T, MR, ALIGNED, 0>(a, g, span, c0, lds, lane, wave) &&
+      low_span<T, MR, ALIGNED, 1>(a, g, span, c0, lds, lane, wave))
+    low_span<T, MR, ALIGNED, 2>(a, g, span, c0, lds, lane, wave);
 }
 
 // Adds an adapter's partial sums, in slot order. A thread: 4 columns of a rank,

@@ -77,6 +77,19 @@ __device__ inline bool all_split(const f32x8& v) {
   return most < 0x7f7f8000;
 }
 
+// The same pair for any float: one that rounds to infinity is bf16's largest and
+// the rest, infinities and NaN are themselves with no low part.
+__device__ inline void split8_any(const f32x8& v, bf16x8& hi, bf16x8& lo) {
+  split8(v, hi, lo);
+  if (all_split(v)) return;
+  for (int i = 0; i < 8; ++i) {
+    if (splits(v[i])) continue;
+    const bool number = (__float_as_uint(v[i]) & 0x7fffffff) < 0x7f800000;
+    if (number) hi[i] = __builtin_bit_cast(bf16_t, (uint16_t)(v[i] < 0 ? 0xff7f : 0x7f7f));
+    lo[i] = number ? (bf16_t)(v[i] - (float)hi[i]) : (bf16_t)0.0f;
+  }
+}
+
 // acc += a * b with b given as floats split in two; an f16 operand is split
 // too (11 bits, exact in the pair), a bf16 one needs no low part.
 __device__ inline f32x4 mfma_split(bf16x8 a, bf16x8 hi, bf16x8 lo, f32x4 c) { return mfma(a, hi, mfma(a, lo, c)); }
@@ -94,6 +107,12 @@ __device__ inline SplitF16 widen(f16x8 v) {
 __device__ inline f32x4 mfma_split(const SplitF16& a, bf16x8 hi, bf16x8 lo, f32x4 c) {
   return mfma(a.hi, hi, mfma(a.hi, lo, mfma(a.lo, hi, c)));
 }
+
+// The high parts' product alone. Infinities times pairs may be infinities of both
+// signs or meet a zero low part; here they are what they are in the product of
+// the values themselves.
+__device__ inline f32x4 mfma_high(bf16x8 a, bf16x8 hi, f32x4 c) { return mfma(a, hi, c); }
+__device__ inline f32x4 mfma_high(const SplitF16& a, bf16x8 hi, f32x4 c) { return mfma(a.hi, hi, c); }
 
 // 8 elements at p of which the first `valid` exist; the rest read as zero.
 // whole: all 8 may be read at once at any alignment of an element.

@@ -133,3 +133,69 @@ def test_coefficients_near_the_largest_float(sizes):
     check_forward(c, y)
     check_forward(c, served)
     check_dx(c, dx)
+
+
+def adapter_gradients(c):
+    """(da, db) in 64 bits, and their magnitudes, from each adapter's own tokens."""
+    x, dy, gate = c["x"].cpu().double(), c["dy"].cpu().double(), c["gate"].cpu().double()
+    a, b, ids = c["a"].cpu().double(), c["b"].cpu().double(), c["ids"].cpu()
+    out = [torch.zeros_like(a), torch.zeros_like(b), torch.zeros_like(a), torch.zeros_like(b)]
+    for e in range(a.shape[0]):
+        for j in range(ids.shape[1]):
+            rows = torch.nonzero(ids[:, j] == e)[:, 0]
+            if len(rows):
+                cf = gate[rows, j][:, None] * float(c["scale"][e])
+                cv, cu = cf * (dy[rows] @ b[e]), cf * (x[rows] @ a[e].t())
+                out[0][e] += cv.t() @ x[rows]
+                out[1][e] += dy[rows].t() @ cu
+                out[2][e] += (cf.abs() * (dy[rows].abs() @ b[e].abs())).t() @ x[rows].abs()
+                out[3][e] += dy[rows].abs().t() @ (cf.abs() * (x[rows].abs() @ a[e].abs().t()))
+    return [v.cuda() for v in out]
+
+
+def gradients(c):
+    a, b = c["a"].clone().requires_grad_(), c["b"].clone().requires_grad_()
+    y = mixture.lora_linear(c["x"], c["w"], a, b, c["ids"], weights=c["gate"], scale=c["scale"])
+    return torch.autograd.grad(y, (a, b), c["dy"])
+
+
+def check_gradients(c, da, db):
+    ra, rb, sa, sb = adapter_gradients(c)
+    t, k = c["ids"].shape
+    agrees(da, ra, sa, c["dy"].shape[1] + t * k, sa)
+    agrees(db, rb, sb, c["x"].shape[1] + t * k, sb)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+@pytest.mark.parametrize("sizes", SIZES + [(900, 3, 1, 72, 264, 100)])
+def test_gradients_of_bad_tokens_and_adapters(sizes, dtype):
+    """Infinities in a token, its gradient, its weight or an adapter show in the gradients of the adapters concerned, as
+    infinities where the definition has them; the others' are bit for bit what they are without them."""
+    c = case(*sizes, dtype)
+    clean = gradients(c)
+    for what, at, value in (("x", (5, 3), INF), ("dy", (6, 2), -INF), ("x", (9, 0), NAN), ("gate", (11, 0), INF), ("a", (1, 0, 4), INF),
+                            ("b", (1, 7, 0), -INF), ("dy", (13, 1), NAN)):
+        bad = dict(c, **{what: c[what].clone()})
+        bad[what][at] = value
+        if what == "gate":
+            c["ids"][11, 0] = bad["ids"][11, 0] = 1
+            clean = gradients(c)
+        touched = {at[0]} if what in ("a", "b") else set(c["ids"][at[0]].tolist())
+        da, db = gradients(bad)
+        for e in range(len(c["a"])):
+            if e not in touched:
+                assert torch.equal(da[e], clean[0][e]) and torch.equal(db[e], clean[1][e])
+        check_gradients(bad, da, db)
+
+
+def test_gradients_of_coefficients_near_the_largest_float():
+    """A scaled coefficient between bf16's largest value and float's makes a finite gradient."""
+    c = case(600, 2, 1, 72, 88, 16, "bf16")
+    c["ids"][:] = 0
+    c["ids"][::3] = 1
+    c["x"][:], c["dy"][:], c["gate"][:], c["scale"][0] = 0, 2.0 ** -10, 1, 1.999
+    c["a"][0, 3, :], c["b"][0] = 0, 0
+    c["x"][1, 7], c["a"][0, 3, 7] = 1, 2.0 ** 127
+    da, db = gradients(c)
+    assert float(db[0, :, 3].abs().min()) > 1e35
+    check_gradients(c, da, db)
