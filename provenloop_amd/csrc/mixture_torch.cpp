@@ -10,8 +10,10 @@
 #include <ATen/hip/EmptyTensor.h>
 #include <ATen/hip/impl/HIPGuardImplMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/csrc/utils/pybind.h>
 
 #include "tensafe_he.h"
@@ -50,6 +52,21 @@ void on_gpu(const char* name, const Tensor& first, std::initializer_list<Tensor>
   NEED(first.is_cuda(), name, ": tensors must be on the GPU (there is no CPU path)");
   for (const Tensor& t : others)
     NEED(!t.defined() || t.device() == first.device(), name, ": all tensors must be on one device");
+}
+
+// These functions are not torch's dispatched operators: a trace would hold their
+// results as constants, and the results would have no tangents, which torch
+// reads as zeros.
+void not_traced(const char* name) {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  TORCH_CHECK_NOT_IMPLEMENTED(!torch::jit::tracer::isTracing() && !Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+                              name, ": cannot be traced");
+}
+bool has_tangent(const Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool has_tangent(const OptTensor& t) { return t && has_tangent(*t); }
+template <class... Tensors>
+void no_tangents(const char* name, const Tensors&... ts) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(has_tangent(ts) || ...), name, ": has no forward-mode derivative");
 }
 
 Tensor make(at::IntArrayRef size, at::ScalarType type, const Tensor& like) {
@@ -111,6 +128,7 @@ variable_list once(variable_list grads) {
 
 // ---------------------------------------------------------------- grouping and gate
 std::tuple<Tensor, Tensor, Tensor> group(const Tensor& given, int64_t n) {
+  not_traced("group");
   const Tensor experts = experts_of("group", given);
   on_gpu("group", experts);
   NEED(n >= 1 && n <= 1 << 30, "group: the number of groups must be positive");
@@ -159,6 +177,7 @@ struct Route : Function<Route> {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &logits = saved[0], &mask = saved[1];
     if (!grads[0].defined()) return variable_list(4);
+    no_tangents("route's gradient", grads[0]);
     const Tensor dweights = grads[0].contiguous();
     Guard guard(logits.device());
     Tensor dlogits = make(logits.sizes(), logits.scalar_type(), logits);
@@ -172,6 +191,8 @@ struct Route : Function<Route> {
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> route(const Tensor& given, int64_t k, const OptTensor& given_mask,
                                                  bool normalize) {
+  not_traced("route");
+  no_tangents("route", given);
   NEED(type_of(given) != 0, "route: logits must be bf16, f16 or f32");
   NEED(given.dim() == 2, "route: logits must be [T, E]");
   Tensor mask = given_mask ? *given_mask : Tensor();
@@ -233,6 +254,7 @@ struct GroupedMatmul : Function<GroupedMatmul> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1];
+    no_tangents("grouped_matmul's gradient", grads[0]);
     const Tensor dy = grads[0].contiguous();
     Guard guard(x.device());
     Tensor dx, dw;
@@ -250,6 +272,8 @@ struct GroupedMatmul : Function<GroupedMatmul> {
 
 Tensor grouped_matmul(const Tensor& given_x, const Tensor& given_w, const Tensor& experts, const Tensor& order,
                       const Tensor& offsets, int64_t n_groups) {
+  not_traced("grouped_matmul");
+  no_tangents("grouped_matmul", given_x, given_w);
   NEED(is_half(given_x), "grouped_matmul: x must be bf16 or f16");
   NEED(given_w.scalar_type() == given_x.scalar_type(), "grouped_matmul: x and w must have one type");
   const int64_t t = experts.size(0), k = experts.size(1);
@@ -333,6 +357,7 @@ struct LoraLinear : Function<LoraLinear> {
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
     const Lora l{s[0], s[4], s[5], s[1], s[2], s[6], s[3], s[7], s[8], s[9]};
+    no_tangents("lora_linear's gradient", grads[0]);
     const Tensor dy = rows(grads[0]);
     Guard guard(l.x.device());
     Tensor out[4];
@@ -353,6 +378,8 @@ struct LoraLinear : Function<LoraLinear> {
 Tensor lora_linear(const Tensor& x, const Tensor& weight, const Tensor& a, const Tensor& b, const Tensor& given_experts,
                    const OptTensor& weights, const OptTensor& scale, const OptTensor& bias, const OptTensor& order,
                    const OptTensor& offsets) {
+  not_traced("lora_linear");
+  no_tangents("lora_linear", x, weight, a, b, weights, scale, bias);
   NEED(is_half(x), "lora_linear: x must be bf16 or f16");
   const at::ScalarType type = x.scalar_type();
   NEED(weight.scalar_type() == type, "lora_linear: weight must have x's type");

@@ -12,8 +12,9 @@ training the adapters and their gate. Three operators that fit together:
 
 A slot is a (token, choice) pair, numbered token * k + choice; expert -1 means
 none. Work is queued on torch's current stream of the tensors' device, and
-nothing waits for it. All three are differentiable (see each for what in) and
-can be captured into a graph. Values are bf16 or f16 with sums in float; the
+nothing waits for it. All three are differentiable (see each for what in; in
+reverse mode, once) and can be captured into a graph; forward-mode derivatives
+and tracing are refused. Values are bf16 or f16 with sums in float; the
 gate's logits may be f32 too. The C entry points are in
 include/tensafe_he.h (th_route, th_group, th_grouped_matmul, th_lora_linear).
 
