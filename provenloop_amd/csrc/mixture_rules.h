@@ -12,6 +12,11 @@ constexpr uint32_t MIX_MAX_RANK = 128;      // eight 16-row tiles of an adapter 
 
 constexpr uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
+// Workgroups of a kernel whose workgroups each take every so-many-th piece of
+// work: a launch must have fewer than 2^32 threads, and 2^20 workgroups fill the
+// GPU many times over.
+constexpr uint32_t loop_blocks(uint64_t pieces) { return (uint32_t)(pieces < 1u << 20 ? pieces : 1u << 20); }
+
 // Tokens whose (token, choice) slots one workgroup of 1024 threads groups: 1024
 // to 4096 slots, as few as give a workgroup to each of the 256 CUs, and more
 // where there would be more than 1024 workgroups, each of which adds up the

@@ -334,37 +334,37 @@ __global__ void __launch_bounds__(THREADS) place_kernel(RouteArgs a) {
 // sum_j w_j dw_j), with p from the logits again. A wavefront per token.
 template <class T>
 __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a, const float* dweights, T* dlogits) {
-  const int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
   const uint32_t lane = threadIdx.x & 63;
-  if (t >= a.T) return;
-  float inner = 0;
-  for (uint32_t j = 0; j < a.k; ++j)
-    if (a.experts[t * a.k + j] >= 0) inner += a.weights[t * a.k + j] * dweights[t * a.k + j];
-  float big = -INFINITY, z = 0;
-  if (!a.normalize) {
-    for (uint32_t e = lane; e < a.E; e += 64) {
-      float l;
-      if (allowed_at<T>(a, t, e, l)) big = l != l || big != big ? NAN : fmaxf(big, l);
-    }
-    for (int d = 32; d; d >>= 1) {
-      const float o = __shfl_xor(big, d);
-      big = o != o || big != big ? NAN : fmaxf(big, o);
-    }
-    for (uint32_t e = lane; e < a.E; e += 64) {
-      float l;
-      if (allowed_at<T>(a, t, e, l)) z += expf(l - big);
-    }
-    for (int d = 32; d; d >>= 1) z += __shfl_xor(z, d);
-  }
-  for (uint32_t e = lane; e < a.E; e += 64) {
-    float grad = 0, l;
-    if (!a.normalize && allowed_at<T>(a, t, e, l)) grad = -(expf(l - big) / z) * inner;
+  for (int64_t t = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); t < a.T; t += (int64_t)gridDim.x * 4) {
+    float inner = 0;
     for (uint32_t j = 0; j < a.k; ++j)
-      if (a.experts[t * a.k + j] == (int32_t)e) {
-        const float w = a.weights[t * a.k + j], dw = dweights[t * a.k + j];
-        grad = a.normalize ? w * (dw - inner) : grad + w * dw;
+      if (a.experts[t * a.k + j] >= 0) inner += a.weights[t * a.k + j] * dweights[t * a.k + j];
+    float big = -INFINITY, z = 0;
+    if (!a.normalize) {
+      for (uint32_t e = lane; e < a.E; e += 64) {
+        float l;
+        if (allowed_at<T>(a, t, e, l)) big = l != l || big != big ? NAN : fmaxf(big, l);
       }
-    dlogits[t * a.E + e] = from_float<T>(grad);
+      for (int d = 32; d; d >>= 1) {
+        const float o = __shfl_xor(big, d);
+        big = o != o || big != big ? NAN : fmaxf(big, o);
+      }
+      for (uint32_t e = lane; e < a.E; e += 64) {
+        float l;
+        if (allowed_at<T>(a, t, e, l)) z += expf(l - big);
+      }
+      for (int d = 32; d; d >>= 1) z += __shfl_xor(z, d);
+    }
+    for (uint32_t e = lane; e < a.E; e += 64) {
+      float grad = 0, l;
+      if (!a.normalize && allowed_at<T>(a, t, e, l)) grad = -(expf(l - big) / z) * inner;
+      for (uint32_t j = 0; j < a.k; ++j)
+        if (a.experts[t * a.k + j] == (int32_t)e) {
+          const float w = a.weights[t * a.k + j], dw = dweights[t * a.k + j];
+          grad = a.normalize ? w * (dw - inner) : grad + w * dw;
+        }
+      dlogits[t * a.E + e] = from_float<T>(grad);
+    }
   }
 }
 
@@ -416,7 +416,7 @@ hipError_t launch_group(RouteArgs a, hipStream_t s) {
 
 hipError_t launch_route_backward(MixType type, const RouteArgs& a, const float* dweights, void* dlogits,
                                  hipStream_t s) {
-  const uint32_t blocks = (uint32_t)th::ceil_div(a.T, 4);
+  const uint32_t blocks = th::loop_blocks(th::ceil_div(a.T, 4));
   if (type == MIX_BF16) route_backward_kernel<bf16_t><<<blocks, 256, 0, s>>>(a, dweights, (bf16_t*)dlogits);
   else if (type == MIX_F16) route_backward_kernel<f16_t><<<blocks, 256, 0, s>>>(a, dweights, (f16_t*)dlogits);
   else route_backward_kernel<float><<<blocks, 256, 0, s>>>(a, dweights, (float*)dlogits);
