@@ -447,13 +447,14 @@ __global__ void __launch_bounds__(256) low_sum_kernel(LowOuterPair pair) {
 }
 
 template <class T, int MR>
-hipError_t run_low(const LowOuterPair& pair, uint32_t blocks, hipStream_t s) {
+hipError_t run_low(const LowOuterPair& pair, uint64_t blocks, hipStream_t s) {
   constexpr uint32_t bytes = low_batch(MR) * (128 * 2 + 2 * 16 * MR * 2);
   auto go = [&](auto kernel) {
     static const hipError_t ready =
         hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (ready != hipSuccess) return ready;
-    kernel<<<blocks, 256, bytes, s>>>(pair);
+    if (!th::launchable(blocks, 256)) return hipErrorInvalidConfiguration;
+    kernel<<<(uint32_t)blocks, 256, bytes, s>>>(pair);
     return hipGetLastError();
   };
   const bool aligned = pair.p[0].aligned && pair.p[1].aligned;
@@ -462,18 +463,19 @@ hipError_t run_low(const LowOuterPair& pair, uint32_t blocks, hipStream_t s) {
 
 template <class T>
 hipError_t low_outer_typed(LowOuterPair pair, hipStream_t s) {
-  uint32_t blocks = 0, rows = 0;
+  uint64_t blocks = 0;
+  uint32_t rows = 0;
   for (int i = 0; i < 2; ++i) {
     const LowOuterArgs& a = pair.p[i];
-    if (i == 1) pair.blocks = blocks;
+    if (i == 1) pair.blocks = (uint32_t)blocks;
     if (!a.out) continue;
-    blocks += (uint32_t)(th::ceil_div(a.cols, 128) * th::lowrank_spans(a.slots, a.E, a.span));
+    blocks += th::ceil_div(a.cols, 128) * th::lowrank_spans(a.slots, a.E, a.span);
     const uint64_t threads = a.transposed ? a.cols * th::ceil_div(a.r, 8) : a.r * th::ceil_div(a.cols, 4);
     rows = max(rows, (uint32_t)min(th::ceil_div(threads, 256), (uint64_t)1024));
   }
   const LowOuterArgs& a = pair.p[pair.p[0].out ? 0 : 1];
-  pair.gate_from = blocks;
-  if (pair.gate.out) blocks += (uint32_t)th::ceil_div(pair.gate.slots, 256);
+  pair.gate_from = (uint32_t)blocks;
+  if (pair.gate.out) blocks += th::ceil_div(pair.gate.slots, 256);
   if (blocks) {
     const hipError_t e = a.r <= 16   ? run_low<T, 1>(pair, blocks, s)
                          : a.r <= 32 ? run_low<T, 2>(pair, blocks, s)
@@ -504,17 +506,19 @@ __global__ void __launch_bounds__(256) transpose_kernel(TransposePair pair) {
     ((uint16_t*)a.out)[((int64_t)e * a.cols + c0 + i / tail) * a.out_ld + a.rows + i % tail] = 0;
 }
 
-// 8 values a thread.
+// 8 values a thread at a time.
 __global__ void __launch_bounds__(256) pad_kernel(PadSet set) {
   const uint32_t which = (blockIdx.x >= set.blocks[0]) + (blockIdx.x >= set.blocks[1]);
   const PadArgs& a = set.p[which];
-  const uint64_t i = (uint64_t)(blockIdx.x - (which ? set.blocks[which - 1] : 0)) * 256 + threadIdx.x;
+  const uint32_t first = which ? set.blocks[which - 1] : 0, many = (which < 2 ? set.blocks[which] : gridDim.x) - first;
   const uint32_t chunks = (a.cols + 7) / 8;
-  const uint64_t row = i / chunks;
-  if (row >= (uint64_t)a.rows * a.E) return;
-  const uint32_t c = (uint32_t)(i % chunks) * 8;
-  const bf16_t* p = (const bf16_t*)a.in + (int64_t)(row / a.rows) * a.lde + (int64_t)(row % a.rows) * a.ld + c;
-  ((bf16x8*)a.out)[i] = load8<bf16_t>(p, (int64_t)a.cols - c);
+  for (uint64_t i = (uint64_t)(blockIdx.x - first) * 256 + threadIdx.x;; i += (uint64_t)many * 256) {
+    const uint64_t row = i / chunks;
+    if (row >= (uint64_t)a.rows * a.E) return;
+    const uint32_t c = (uint32_t)(i % chunks) * 8;
+    const bf16_t* p = (const bf16_t*)a.in + (int64_t)(row / a.rows) * a.lde + (int64_t)(row % a.rows) * a.ld + c;
+    ((bf16x8*)a.out)[i] = load8<bf16_t>(p, (int64_t)a.cols - c);
+  }
 }
 
 // A thread: 8 columns of a token, or 1 where rows are no multiple of 8.
@@ -546,14 +550,12 @@ template <class T>
 static hipError_t outer_typed(const OuterArgs& a, hipStream_t s) {
   if (!a.aligned) {
     const uint64_t blocks = th::ceil_div(a.n, 128) * th::ceil_div(a.k, 128) * a.E;
-    unaligned_outer_kernel<T><<<(uint32_t)blocks, 256, 2 * 2 * 64 * 128 * 2, s>>>(a);
-    return hipGetLastError();
+    return launch<unaligned_outer_kernel<T>>(blocks, 256, 2 * 2 * 64 * 128 * 2, s, a);
   }
   constexpr uint32_t B = 128;
   const uint64_t nt = th::ceil_div(a.n, B), kt = th::ceil_div(a.k, B), gn = nt >= kt ? 4 : 2, gk = 8 / gn;
   const uint64_t blocks = 8 * th::ceil_div(nt, gn) * th::ceil_div(kt, gk) * a.E;
-  outer_kernel<T, B, 2, 4><<<(uint32_t)blocks, 512, 2 * 2 * B * 128, s>>>(a);
-  return hipGetLastError();
+  return launch<outer_kernel<T, B, 2, 4>>(blocks, 512, 2 * 2 * B * 128, s, a);
 }
 hipError_t launch_outer(MixType type, const OuterArgs& a, hipStream_t s) {
   return type == MIX_BF16 ? outer_typed<bf16_t>(a, s) : outer_typed<f16_t>(a, s);
@@ -564,24 +566,22 @@ hipError_t launch_low_outer(MixType type, const LowOuterPair& pair, hipStream_t 
 }
 
 hipError_t launch_transpose(TransposePair pair, hipStream_t s) {
-  uint32_t blocks = 0;
+  uint64_t blocks = 0;
   for (int i = 0; i < 2; ++i) {
     const TransposeArgs& a = pair.p[i];
-    if (i == 1) pair.blocks = blocks;
-    if (a.out) blocks += (uint32_t)(th::ceil_div(a.rows, 64) * th::ceil_div(a.cols, 64) * a.E);
+    if (i == 1) pair.blocks = (uint32_t)blocks;
+    if (a.out) blocks += th::ceil_div(a.rows, 64) * th::ceil_div(a.cols, 64) * a.E;
   }
-  if (blocks) transpose_kernel<<<blocks, 256, 0, s>>>(pair);
-  return hipGetLastError();
+  return blocks ? launch<transpose_kernel>(blocks, 256, 0, s, pair) : hipSuccess;
 }
 
 hipError_t launch_pad(PadSet set, hipStream_t s) {
-  uint64_t blocks = 0;
+  uint32_t blocks = 0;
   for (int i = 0; i < 3; ++i) {
-    if (i) set.blocks[i - 1] = (uint32_t)blocks;
-    if (set.p[i].out) blocks += th::ceil_div((uint64_t)set.p[i].rows * set.p[i].E * th::ceil_div(set.p[i].cols, 8), 256);
+    if (i) set.blocks[i - 1] = blocks;
+    if (set.p[i].out) blocks += th::pad_blocks(set.p[i].rows, set.p[i].E, set.p[i].cols);
   }
-  if (blocks) pad_kernel<<<(uint32_t)blocks, 256, 0, s>>>(set);
-  return hipGetLastError();
+  return blocks ? launch<pad_kernel>(blocks, 256, 0, s, set) : hipSuccess;
 }
 
 hipError_t launch_sum_choices(MixType type, const float* in, void* out, int64_t tokens, uint32_t k, uint32_t n,
@@ -598,6 +598,5 @@ hipError_t launch_sum_choices(MixType type, const float* in, void* out, int64_t 
 
 hipError_t launch_gate_grad(const GateGradArgs& a, hipStream_t s) {
   if (!a.slots) return hipSuccess;
-  gate_grad_kernel<<<(uint32_t)th::ceil_div(a.slots, 256), 256, 0, s>>>(a);
-  return hipGetLastError();
+  return launch<gate_grad_kernel>(th::ceil_div(a.slots, 256), 256, 0, s, a);
 }

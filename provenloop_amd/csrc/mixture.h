@@ -18,6 +18,14 @@ typedef _Float16 f16_t;
 
 enum MixType { MIX_BF16 = 1, MIX_F16 = 2, MIX_F32 = 3 };
 
+// A launch of `blocks` workgroups, or none if they are too many for one.
+template <auto Kernel, class... Args>
+hipError_t launch(uint64_t blocks, uint32_t threads, uint32_t lds, hipStream_t s, const Args&... args) {
+  if (!th::launchable(blocks, threads)) return hipErrorInvalidConfiguration;
+  Kernel<<<(uint32_t)blocks, threads, lds, s>>>(args...);
+  return hipGetLastError();
+}
+
 __device__ inline float to_float(bf16_t v) { return (float)v; }
 __device__ inline float to_float(f16_t v) { return (float)v; }
 __device__ inline float to_float(float v) { return v; }

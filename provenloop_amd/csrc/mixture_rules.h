@@ -12,9 +12,11 @@ constexpr uint32_t MIX_MAX_RANK = 128;      // eight 16-row tiles of an adapter 
 
 constexpr uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 
+// A launch has fewer than 2^32 threads along each axis; the runtime takes more
+// with their number wrapped round.
+constexpr bool launchable(uint64_t blocks, uint32_t threads) { return blocks < (1ull << 32) / threads; }
 // Workgroups of a kernel whose workgroups each take every so-many-th piece of
-// work: a launch must have fewer than 2^32 threads, and 2^20 workgroups fill the
-// GPU many times over.
+// work: 2^20 fill the GPU many times over.
 constexpr uint32_t loop_blocks(uint64_t pieces) { return (uint32_t)(pieces < 1u << 20 ? pieces : 1u << 20); }
 
 // Tokens whose (token, choice) slots one workgroup of 1024 threads groups: 1024
@@ -88,6 +90,10 @@ constexpr bool wide_square(uint64_t rows, uint32_t n, uint32_t groups) {
 // 203 -> 515, 1 row 8.6 / 12.1, 32 rows 10.3 / 12.4; 1427 rows of 1389 -> 544
 // 82 / 41): a short contraction of few rows does not pay for the launch.
 constexpr bool pad_operands(uint64_t rows, uint32_t k) { return rows > 32 || k >= 1024; }
+// The workgroups that make such a copy, 2048 values at a time.
+constexpr uint32_t pad_blocks(uint64_t rows, uint32_t E, uint32_t cols) {
+  return loop_blocks(ceil_div(rows * E * ceil_div(cols, 8), 256));
+}
 // Slots whose adapters a workgroup of the low-rank product looks through by
 // itself, which saves the launch that would group them.
 constexpr uint32_t NARROW_SCAN_SLOTS = 2048;

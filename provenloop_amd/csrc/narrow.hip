@@ -304,6 +304,7 @@ hipError_t run(const MatArgs& a, int transposed, hipStream_t s) {
     static const hipError_t ready =
         hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, most);
     if (ready != hipSuccess) return ready;
+    if (!th::launchable(blocks, 64 * WAVES)) return hipErrorInvalidConfiguration;
     const uint32_t bytes = a.scan ? most : narrow_lds<MT, NT, WAVES, S>();
     kernel<<<(uint32_t)blocks, 64 * WAVES, bytes, s>>>(a, shares);
     return hipGetLastError();

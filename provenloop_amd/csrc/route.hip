@@ -370,15 +370,13 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a, const 
 
 template <class T>
 hipError_t route_typed(const RouteArgs& a, uint32_t chunks, size_t lds, hipStream_t s) {
-  auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, dim3(chunks), dim3(THREADS), lds, s, a); };
-  if (a.E <= 8) go(route_kernel<T, 1>);
-  else if (a.E <= 16) go(route_kernel<T, 2>);
-  else if (a.E <= 32) go(route_kernel<T, 4>);
-  else if (a.E <= 64) go(route_kernel<T, 8>);
-  else if (a.E <= 128) go(route_kernel<T, 16>);
-  else if (a.E <= 256) go(route_kernel<T, 32>);
-  else go(route_kernel<T, 64>);
-  return hipGetLastError();
+  if (a.E <= 8) return launch<route_kernel<T, 1>>(chunks, THREADS, lds, s, a);
+  if (a.E <= 16) return launch<route_kernel<T, 2>>(chunks, THREADS, lds, s, a);
+  if (a.E <= 32) return launch<route_kernel<T, 4>>(chunks, THREADS, lds, s, a);
+  if (a.E <= 64) return launch<route_kernel<T, 8>>(chunks, THREADS, lds, s, a);
+  if (a.E <= 128) return launch<route_kernel<T, 16>>(chunks, THREADS, lds, s, a);
+  if (a.E <= 256) return launch<route_kernel<T, 32>>(chunks, THREADS, lds, s, a);
+  return launch<route_kernel<T, 64>>(chunks, THREADS, lds, s, a);
 }
 
 size_t group_lds(uint32_t E, bool chunks = false) { return (size_t)((chunks ? 2 : 1) * WAVES + 1) * (E + 1) * 4; }
@@ -388,8 +386,7 @@ hipError_t place(const RouteArgs& a, uint32_t chunks, hipStream_t s) {
   static const hipError_t ready = hipFuncSetAttribute((const void*)place_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
                                                       (int)group_lds(th::MIX_MAX_EXPERTS, true));
   if (ready != hipSuccess) return ready;
-  place_kernel<<<chunks, THREADS, group_lds(a.E, true), s>>>(a);
-  return hipGetLastError();
+  return launch<place_kernel>(chunks, THREADS, group_lds(a.E, true), s, a);
 }
 
 }  // namespace
@@ -409,16 +406,14 @@ hipError_t launch_route(MixType type, RouteArgs a, hipStream_t s) {
 hipError_t launch_group(RouteArgs a, hipStream_t s) {
   const uint32_t chunks = (uint32_t)th::group_chunks(a.T, a.k);
   a.chunk = (uint32_t)th::group_chunk_tokens(a.T, a.k);
-  count_kernel<<<chunks, THREADS, group_lds(a.E), s>>>(a);
-  const hipError_t e = hipGetLastError();
+  const hipError_t e = launch<count_kernel>(chunks, THREADS, group_lds(a.E), s, a);
   return e != hipSuccess ? e : place(a, chunks, s);
 }
 
 hipError_t launch_route_backward(MixType type, const RouteArgs& a, const float* dweights, void* dlogits,
                                  hipStream_t s) {
   const uint32_t blocks = th::loop_blocks(th::ceil_div(a.T, 4));
-  if (type == MIX_BF16) route_backward_kernel<bf16_t><<<blocks, 256, 0, s>>>(a, dweights, (bf16_t*)dlogits);
-  else if (type == MIX_F16) route_backward_kernel<f16_t><<<blocks, 256, 0, s>>>(a, dweights, (f16_t*)dlogits);
-  else route_backward_kernel<float><<<blocks, 256, 0, s>>>(a, dweights, (float*)dlogits);
-  return hipGetLastError();
+  if (type == MIX_BF16) return launch<route_backward_kernel<bf16_t>>(blocks, 256, 0, s, a, dweights, (bf16_t*)dlogits);
+  if (type == MIX_F16) return launch<route_backward_kernel<f16_t>>(blocks, 256, 0, s, a, dweights, (f16_t*)dlogits);
+  return launch<route_backward_kernel<float>>(blocks, 256, 0, s, a, dweights, (float*)dlogits);
 }

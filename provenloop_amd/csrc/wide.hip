@@ -141,6 +141,7 @@ hipError_t run(const MatArgs& a, hipStream_t s) {
     static const hipError_t ready =
         hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (ready != hipSuccess) return ready;
+    if (!th::launchable(tiles, 64 * WM * WN)) return hipErrorInvalidConfiguration;
     hipLaunchKernelGGL(kernel, dim3((uint32_t)tiles), dim3(64 * WM * WN), bytes, s, a);
     return hipGetLastError();
   };
