@@ -449,16 +449,8 @@ __global__ void __launch_bounds__(256) low_sum_kernel(LowOuterPair pair) {
 template <class T, int MR>
 hipError_t run_low(const LowOuterPair& pair, uint64_t blocks, hipStream_t s) {
   constexpr uint32_t bytes = low_batch(MR) * (128 * 2 + 2 * 16 * MR * 2);
-  auto go = [&](auto kernel) {
-    static const hipError_t ready =
-        hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (ready != hipSuccess) return ready;
-    if (!th::launchable(blocks, 256)) return hipErrorInvalidConfiguration;
-    kernel<<<(uint32_t)blocks, 256, bytes, s>>>(pair);
-    return hipGetLastError();
-  };
-  const bool aligned = pair.p[0].aligned && pair.p[1].aligned;
-  return aligned ? go(low_outer_kernel<T, MR, true>) : go(low_outer_kernel<T, MR, false>);
+  return pair.p[0].aligned && pair.p[1].aligned ? launch<low_outer_kernel<T, MR, true>, bytes>(blocks, 256, bytes, s, pair)
+                                                : launch<low_outer_kernel<T, MR, false>, bytes>(blocks, 256, bytes, s, pair);
 }
 
 template <class T>

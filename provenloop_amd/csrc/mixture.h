@@ -18,10 +18,17 @@ typedef _Float16 f16_t;
 
 enum MixType { MIX_BF16 = 1, MIX_F16 = 2, MIX_F32 = 3 };
 
-// A launch of `blocks` workgroups, or none if they are too many for one.
-template <auto Kernel, class... Args>
+// A launch of `blocks` workgroups with `lds` bytes, MOST at most where they can
+// be more than the 64 KiB that every kernel may have; or none if the workgroups
+// are too many for one.
+template <auto Kernel, uint32_t MOST = 65536, class... Args>
 hipError_t launch(uint64_t blocks, uint32_t threads, uint32_t lds, hipStream_t s, const Args&... args) {
   if (!th::launchable(blocks, threads)) return hipErrorInvalidConfiguration;
+  if constexpr (MOST > 65536) {
+    const hipError_t ready = th::once_for<Kernel>(
+        [] { return hipFuncSetAttribute((const void*)Kernel, hipFuncAttributeMaxDynamicSharedMemorySize, MOST); });
+    if (ready != hipSuccess) return ready;
+  }
   Kernel<<<(uint32_t)blocks, threads, lds, s>>>(args...);
   return hipGetLastError();
 }

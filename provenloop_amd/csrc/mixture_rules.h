@@ -15,6 +15,13 @@ constexpr uint64_t ceil_div(uint64_t a, uint64_t b) { return (a + b - 1) / b; }
 // A launch has fewer than 2^32 threads along each axis; the runtime takes more
 // with their number wrapped round.
 constexpr bool launchable(uint64_t blocks, uint32_t threads) { return blocks < (1ull << 32) / threads; }
+// What make() gives, asked for once per Kernel: kernels are functions, and many
+// of them have one type.
+template <auto Kernel, class Make>
+auto once_for(Make make) {
+  static const auto made = make();
+  return made;
+}
 // Workgroups of a kernel whose workgroups each take every so-many-th piece of
 // work: 2^20 fill the GPU many times over.
 constexpr uint32_t loop_blocks(uint64_t pieces) { return (uint32_t)(pieces < 1u << 20 ? pieces : 1u << 20); }

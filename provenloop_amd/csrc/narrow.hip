@@ -300,23 +300,13 @@ hipError_t run(const MatArgs& a, int transposed, hipStream_t s) {
     if (a.offsets) mtiles = a.rows / BM + (uint64_t)min((int64_t)a.E + 1, a.rows);
     blocks = mtiles * ntiles;
   }
-  auto go = [&](auto kernel) {
-    static const hipError_t ready =
-        hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, most);
-    if (ready != hipSuccess) return ready;
-    if (!th::launchable(blocks, 64 * WAVES)) return hipErrorInvalidConfiguration;
-    const uint32_t bytes = a.scan ? most : narrow_lds<MT, NT, WAVES, S>();
-    kernel<<<(uint32_t)blocks, 64 * WAVES, bytes, s>>>(a, shares);
-    return hipGetLastError();
+  const uint32_t bytes = a.scan ? most : narrow_lds<MT, NT, WAVES, S>();
+  auto go = [&]<bool TR, bool ALIGNED>() {
+    return a.u ? launch<narrow_kernel<T, MT, NT, WAVES, S, TR, ALIGNED, true>, most>(blocks, 64 * WAVES, bytes, s, a, shares)
+               : launch<narrow_kernel<T, MT, NT, WAVES, S, TR, ALIGNED, false>, most>(blocks, 64 * WAVES, bytes, s, a, shares);
   };
-  if (transposed)
-    return a.u ? go(narrow_kernel<T, MT, NT, WAVES, S, true, true, true>)
-               : go(narrow_kernel<T, MT, NT, WAVES, S, true, true, false>);
-  if (a.aligned)
-    return a.u ? go(narrow_kernel<T, MT, NT, WAVES, S, false, true, true>)
-               : go(narrow_kernel<T, MT, NT, WAVES, S, false, true, false>);
-  return a.u ? go(narrow_kernel<T, MT, NT, WAVES, S, false, false, true>)
-             : go(narrow_kernel<T, MT, NT, WAVES, S, false, false, false>);
+  if (transposed) return go.template operator()<true, true>();
+  return a.aligned ? go.template operator()<false, true>() : go.template operator()<false, false>();
 }
 
 template <class T>

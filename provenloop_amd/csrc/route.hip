@@ -20,6 +20,8 @@
 namespace {
 
 constexpr int THREADS = 1024, WAVES = THREADS / 64;
+constexpr uint32_t group_lds(uint32_t E, bool chunks = false) { return ((chunks ? 2 : 1) * WAVES + 1) * (E + 1) * 4; }
+constexpr uint32_t MOST = group_lds(th::MIX_MAX_EXPERTS), MOST_CHUNKS = group_lds(th::MIX_MAX_EXPERTS, true);
 
 // A logit as a whole number that orders candidates: its bits made to rise with
 // its value (NaN above +inf, as a comparison sort of the framework's users puts
@@ -369,7 +371,7 @@ __global__ void __launch_bounds__(256) route_backward_kernel(RouteArgs a, const 
 }
 
 template <class T>
-hipError_t route_typed(const RouteArgs& a, uint32_t chunks, size_t lds, hipStream_t s) {
+hipError_t route_typed(const RouteArgs& a, uint32_t chunks, uint32_t lds, hipStream_t s) {
   if (a.E <= 8) return launch<route_kernel<T, 1>>(chunks, THREADS, lds, s, a);
   if (a.E <= 16) return launch<route_kernel<T, 2>>(chunks, THREADS, lds, s, a);
   if (a.E <= 32) return launch<route_kernel<T, 4>>(chunks, THREADS, lds, s, a);
@@ -379,14 +381,9 @@ hipError_t route_typed(const RouteArgs& a, uint32_t chunks, size_t lds, hipStrea
   return launch<route_kernel<T, 64>>(chunks, THREADS, lds, s, a);
 }
 
-size_t group_lds(uint32_t E, bool chunks = false) { return (size_t)((chunks ? 2 : 1) * WAVES + 1) * (E + 1) * 4; }
-
 hipError_t place(const RouteArgs& a, uint32_t chunks, hipStream_t s) {
   if (chunks == 1) return hipSuccess;
-  static const hipError_t ready = hipFuncSetAttribute((const void*)place_kernel, hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                      (int)group_lds(th::MIX_MAX_EXPERTS, true));
-  if (ready != hipSuccess) return ready;
-  return launch<place_kernel>(chunks, THREADS, group_lds(a.E, true), s, a);
+  return launch<place_kernel, MOST_CHUNKS>(chunks, THREADS, group_lds(a.E, true), s, a);
 }
 
 }  // namespace
@@ -406,7 +403,7 @@ hipError_t launch_route(MixType type, RouteArgs a, hipStream_t s) {
 hipError_t launch_group(RouteArgs a, hipStream_t s) {
   const uint32_t chunks = (uint32_t)th::group_chunks(a.T, a.k);
   a.chunk = (uint32_t)th::group_chunk_tokens(a.T, a.k);
-  const hipError_t e = launch<count_kernel>(chunks, THREADS, group_lds(a.E), s, a);
+  const hipError_t e = launch<count_kernel, MOST>(chunks, THREADS, group_lds(a.E), s, a);
   return e != hipSuccess ? e : place(a, chunks, s);
 }
 

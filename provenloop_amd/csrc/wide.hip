@@ -137,16 +137,10 @@ hipError_t run(const MatArgs& a, hipStream_t s) {
   constexpr uint32_t bytes = wide_lds<T, BM, BN, S, LR>();
   const uint64_t groups = a.offsets ? (uint64_t)min((int64_t)a.E + 1, a.rows) : 0;
   const uint64_t tiles = (a.offsets ? a.rows / BM + groups : th::ceil_div(a.rows, BM)) * th::ceil_div(a.n, BN);
-  auto go = [&](auto kernel) {
-    static const hipError_t ready =
-        hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
-    if (ready != hipSuccess) return ready;
-    if (!th::launchable(tiles, 64 * WM * WN)) return hipErrorInvalidConfiguration;
-    hipLaunchKernelGGL(kernel, dim3((uint32_t)tiles), dim3(64 * WM * WN), bytes, s, a);
-    return hipGetLastError();
-  };
-  if constexpr (S > 0 && BM * BN > 128 * 128) return go(wide_kernel<T, BM, BN, WM, WN, S, TR, LR>);
-  else return go(unaligned_kernel<T, BM, BN, WM, WN, TR, LR>);
+  if constexpr (S > 0 && BM * BN > 128 * 128)
+    return launch<wide_kernel<T, BM, BN, WM, WN, S, TR, LR>, bytes>(tiles, 64 * WM * WN, bytes, s, a);
+  else
+    return launch<unaligned_kernel<T, BM, BN, WM, WN, TR, LR>, bytes>(tiles, 64 * WM * WN, bytes, s, a);
 }
 
 template <class T, bool TR, bool LR>
