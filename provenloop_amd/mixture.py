@@ -32,7 +32,11 @@ from . import _lib
 
 _lib.load()  # the library that the binding calls
 
-from . import _mixture_torch as _ext  # noqa: E402
+try:
+    from . import _mixture_torch as _ext  # noqa: E402
+except ImportError as e:
+    raise ImportError(f"the binding of the mixture operators cannot be loaded ({e}): build it against this torch with "
+                      "`make -C provenloop_amd/csrc mixture`") from e
 
 __all__ = ["Groups", "Routing", "group", "route", "grouped_matmul", "lora_linear"]
 
