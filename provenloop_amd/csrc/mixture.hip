@@ -118,7 +118,7 @@ void check_grouped(const th_grouped* d) {
   mix_type(d->dtype, false);
   need_slots(d->tokens, d->experts, d->choices);
   need(d->d_in >= 1 && d->d_out >= 1, "d_in and d_out must be positive");
-  need_rows(d->x, d->tokens, d->ldx, d->d_in, "x");
+  need_rows(d->x, d->x_per_slot ? d->tokens * d->choices : d->tokens, d->ldx, d->d_in, "x");
   need(d->w != nullptr, "null w");
   need(d->ldw >= d->d_in, "w: the row stride is shorter than a row");
   need(d->tokens == 0 || (d->order && d->offsets), "null groups");
@@ -354,7 +354,7 @@ int th_route_backward(int dtype, const void* logits, int64_t ld, int64_t tokens,
 int th_grouped_matmul(const th_grouped* d, void* y, int64_t ldy, void* stream) {
   return guarded([&] {
     check_grouped(d);
-    need_rows(y, d->tokens, ldy, d->d_out, "y");
+    need_rows(y, d->tokens * d->choices, ldy, d->d_out, "y");
     need_device();
     MatArgs m{};
     m.x = d->x;
@@ -390,7 +390,7 @@ int th_grouped_matmul_backward(const th_grouped* d, const void* dy, int64_t lddy
                                size_t work_bytes, void* stream) {
   return guarded([&] {
     check_grouped(d);
-    need_rows(dy, d->tokens, lddy, d->d_out, "dy");
+    need_rows(dy, d->tokens * d->choices, lddy, d->d_out, "dy");
     const MixType type = (MixType)d->dtype;
     const bool summed = !d->x_per_slot && d->choices > 1;
     Pieces p(work);
