@@ -199,3 +199,21 @@ def test_gradients_of_coefficients_near_the_largest_float():
     da, db = gradients(c)
     assert float(db[0, :, 3].abs().min()) > 1e35
     check_gradients(c, da, db)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f16"])
+def test_bad_values_in_unaligned_operands(dtype):
+    """The same in the kernels for operands and gradients that do not start on 16 bytes."""
+    c = case(32, 5, 3, 200, 33000, 12, dtype)
+    shift = lambda v: torch.cat([v.new_zeros(1), v.flatten()])[1:].view(v.shape)  # noqa: E731
+    c["x"] = shift(c["x"])
+    c["b"][1, 3, 0], c["b"][1, -1, 2], c["gate"][4, 0], c["x"][9, 0] = INF, NAN, -INF, INF
+    with torch.no_grad():
+        check_forward(c, mixture.lora_linear(c["x"], c["w"], c["a"], c["b"], c["ids"], weights=c["gate"], scale=c["scale"]))
+    c = case(700, 5, 2, 136, 264, 20, dtype)
+    c["dy"] = shift(c["dy"])
+    c["a"][1, 0, 5], c["a"][1, -1, 8], c["gate"][4, 0], c["dy"][9, 0] = INF, NAN, -INF, INF
+    assert c["dy"].data_ptr() % 16 != 0
+    check_dx(c, passes(c)[2])
+    c["a"] = c["a"].nan_to_num(0.5, 0.5, 0.5)
+    check_gradients(c, *gradients(c))
