@@ -217,3 +217,33 @@ def test_bad_values_in_unaligned_operands(dtype):
     check_dx(c, passes(c)[2])
     c["a"] = c["a"].nan_to_num(0.5, 0.5, 0.5)
     check_gradients(c, *gradients(c))
+
+
+@pytest.mark.parametrize("t", [40, 2100])
+def test_bad_values_of_slots_without_an_expert(t):
+    """Weights, gradients and rows of slots that have no expert are never read into anything."""
+    c = case(t, 5, 2, 72, 560, 16, "bf16")
+    none = c["ids"] < 0
+    assert none.any()
+    clean = [*passes(c), *gradients(c)]
+    bad = dict(c, gate=torch.where(none, torch.full_like(c["gate"], NAN), c["gate"]))
+    assert all(torch.equal(p, q) for p, q in zip([*passes(bad), *gradients(bad)], clean))
+    w = normal(gen(1), 5, 136, 72, dtype=torch.bfloat16).requires_grad_()
+    x = c["x"].clone()
+    x[none.all(1)] = NAN
+    groups = mixture.group(c["ids"], 5)
+    dy = normal(gen(2), t, 2, 136, dtype=torch.bfloat16)
+    results = []
+    for xs, d in ((c["x"], dy), (x, torch.where(none[..., None], torch.full_like(dy, INF), dy))):
+        xs = xs.clone().requires_grad_()
+        y = mixture.grouped_matmul(xs, w, groups)
+        results.append([y.detach(), *torch.autograd.grad(y, (xs, w), d)])
+    assert all(torch.equal(p, q) for p, q in zip(*results))
+    logits = normal(gen(3), t, 5).requires_grad_()
+    mask = torch.rand(t, 5, generator=gen(4), device="cuda") < 0.4
+    for normalize in (True, False):
+        r = mixture.route(logits, 3, mask=mask, normalize=normalize)
+        dw = normal(gen(5), t, 3)
+        want, = torch.autograd.grad(r.weights, logits, dw, retain_graph=True)
+        got, = torch.autograd.grad(r.weights, logits, torch.where(r.experts < 0, torch.full_like(dw, NAN), dw))
+        assert torch.equal(got, want) and (r.experts < 0).any()
