@@ -40,7 +40,7 @@ __device__ inline void arrived_but(void) {
 constexpr uint32_t KEPT = 4;
 template <int BM>
 struct LowLists {
-  uint32_t words[32];  // a bit per adapter
+  uint32_t words[32];  // a bit per adapter: used, and after the listing, whether something of it is left out
   uint32_t count;
   uint16_t list[th::MIX_MAX_EXPERTS];  // those used, rising
   uint32_t id[BM * KEPT];              // rows x choices; ~0: none
@@ -78,6 +78,7 @@ __device__ inline void list_adapters(const MatArgs& a, int64_t m0, int64_t mend,
     if (lane == 63) l.count = sum;
   }
   __syncthreads();
+  if (threadIdx.x < 32) l.words[threadIdx.x] = 0;
 }
 
 // Coefficient of choice `s` of the tile (row x choices + j), which uses adapter e.
@@ -92,22 +93,25 @@ __device__ inline uint32_t adapter_of(const MatArgs& a, int64_t m0, const LowLis
 }
 
 // The products that add_lowrank leaves out, those of infinities and NaN and of
-// coefficients that make no finite pair, for a wavefront's TM x TN outputs: each
-// row's own adapters alone, one output at a time in float, through the
-// wavefront's own LDS in two halves. -0 where there is none, which changes no sum.
+// coefficients that make no finite pair, for a wavefront's TM x 64 outputs: each
+// row's own adapters alone, a row at a time in float, through the wavefront's own
+// LDS in two halves. -0 where there is none, which changes no sum.
 template <class T, int BM, int TM, int TN>
 __device__ inline void add_nonfinite(const MatArgs& a, int64_t m0, uint32_t rows, uint32_t row0, uint32_t n0, float* own,
                                      const LowLists<BM>& l, uint32_t lane, f32x4 (&acc)[TN / 16][TM / 16]) {
+  static_assert(TN == 64);
   constexpr int SLAB = TM / 2;
+  const uint32_t n = min(n0 + lane, a.n - 1);
 #pragma unroll
   for (int s0 = 0; s0 < TM; s0 += SLAB) {
 #pragma unroll 1
-    for (uint32_t i = lane; i < SLAB * TN; i += 64) {
-      const uint32_t row = row0 + s0 + i / TN, n = n0 + i % TN;
+    for (uint32_t i = 0; i < SLAB; ++i) {
+      const uint32_t row = __builtin_amdgcn_readfirstlane(row0) + s0 + i;
       float sum = -0.0f;
-      for (uint32_t j = 0; row < rows && n < a.n && j < a.kc; ++j) {
-        const uint32_t s = row * a.kc + j, e = adapter_of(a, m0, l, s);
-        if (e >= a.E) continue;
+#pragma unroll 1
+      for (uint32_t j = 0; row < rows && j < a.kc; ++j) {
+        const uint32_t s = row * a.kc + j, e = __builtin_amdgcn_readfirstlane(adapter_of(a, m0, l, s));
+        if (e >= a.E || !(__builtin_amdgcn_readfirstlane(l.words[e / 32]) >> (e % 32) & 1)) continue;
         const T* p = (const T*)a.p + e * a.ldpe + (int64_t)n * a.ldp;
         const float* u = a.u + (m0 * a.kc + s) * a.ru;
         float f = 0, d = 0;  // f: what add_lowrank took for this adapter's coefficient
@@ -115,14 +119,20 @@ __device__ inline void add_nonfinite(const MatArgs& a, int64_t m0, uint32_t rows
           if (adapter_of(a, m0, l, row * a.kc + i) == e) f += coefficient(a, m0, l, row * a.kc + i, e);
         bool any = false;
 #pragma unroll 1
-        for (uint32_t q = 0; q < a.r; ++q)
-          if (!is_finite(p[q]) || !splits(f * u[q])) {
-            d = fmaf(u[q], (float)p[q], d);
-            any = true;
+        for (uint32_t r0 = 0; r0 < a.r; r0 += 8) {
+          const vec8<T> v = load8<T>(p + r0, (int64_t)a.r - r0);
+#pragma unroll
+          for (uint32_t q = 0; q < 8; ++q) {
+            const float x = r0 + q < a.r ? u[r0 + q] : 0.0f;
+            if (r0 + q < a.r && !(is_finite(v[q]) && splits(f * x))) {
+              d = fmaf(x, (float)v[q], d);
+              any = true;
+            }
           }
+        }
         if (any) sum += coefficient(a, m0, l, s, e) * d;
       }
-      own[i] = sum;
+      own[i * TN + lane] = sum;
     }
     __builtin_amdgcn_wave_barrier();
 #pragma unroll
@@ -136,7 +146,7 @@ __device__ inline void add_nonfinite(const MatArgs& a, int64_t m0, uint32_t rows
 
 template <class T, int BM, int BN, int WM, int WN>
 __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, uint32_t n0, char* lds,
-                                   const LowLists<BM>& l, f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
+                                   LowLists<BM>& l, f32x4 (&acc)[BN / WN / 16][BM / WM / 16]) {
   constexpr int THREADS = 64 * WM * WN, TM = BM / WM, TN = BN / WN;
   constexpr int XI = BM * 8 / THREADS, WI = BN * 8 / THREADS;   // 16-byte pieces of a thread
   constexpr bool PAIR = !std::is_same<T, bf16_t>::value;  // f16 operands are pairs too
@@ -145,7 +155,12 @@ __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, u
   const uint32_t rows = (uint32_t)(mend - m0);
   const uint32_t each = (a.r + 7) / 8, chunks = l.count * each;  // chunks of 8 ranks
   const uint32_t piece = threadIdx.x % 8;                        // this thread's chunk of a set, in all its rows
-  bool odd = false;                                              // it has left something out
+  bool odd = false;
+  // it leaves something of adapter e out
+  auto left_out = [&](uint32_t e) __attribute__((always_inline)) {
+    odd = true;
+    atomicOr(&l.words[e / 32], 1u << (e % 32));
+  };
   for (uint32_t c0 = 0; c0 < chunks; c0 += 8) {
     const uint32_t c = c0 + piece, e = c < chunks ? l.list[c / each] : ~1u, r0 = c % each * 8;
     const bool whole = r0 + 8 <= a.r;
@@ -192,7 +207,7 @@ __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, u
 #pragma unroll
       for (int q = 0; q < 8; ++q) x[q] = f[i] * (q < 4 ? u0[i] : u1[i])[q % 4];
       if (!all_split(x)) {
-        odd = true;
+        left_out(e);
         for (int q = 0; q < 8; ++q) x[q] = splits(x[q]) ? x[q] : 0.0f;
       }
       bf16x8 hi, lo;
@@ -204,7 +219,7 @@ __device__ inline void add_lowrank(const MatArgs& a, int64_t m0, int64_t mend, u
     for (int i = 0; i < WI; ++i) {
       const uint32_t row = i * (THREADS / 8) + threadIdx.x / 8, at = row * 128 + (piece ^ (row & 7)) * 16;
       if (!all_finite<T>(v[i])) {
-        odd = true;
+        left_out(e);
         for (int q = 0; q < 8; ++q) v[i][q] = is_finite(v[i][q]) ? v[i][q] : (T)0.0f;
       }
       if constexpr (PAIR) {
