@@ -443,7 +443,8 @@ int th_grouped_matmul_backward(const th_grouped* d, const void* dy, int64_t lddy
  * a: adapters matrices of rank x d_in; b: of d_out x rank (ranks up to 128;
  * shorter ones are padded with zeros). gate (tokens x choices) and scale (per
  * adapter) are floats, NULL for ones. order and offsets (th_group of
- * `experts`), or NULL: made in the workspace. */
+ * `experts`), or NULL: made in the workspace. Infinities and NaN of an adapter
+ * reach the rows of the tokens that use it, and no others. */
 typedef struct th_lora_linear_args {
   int dtype; /* TH_BF16 or TH_F16: x, weight, bias, a, b, y and their gradients */
   uint32_t choices;

@@ -7,8 +7,8 @@ using namespace mix;
 namespace {
 
 // Slots whose rows a workgroup of low_outer_kernel holds in LDS: 64 KiB of the
-// wide operand and up to 64 KiB of ranks, 80 KiB in all up to rank 16, so that a
-// CU holds two.
+// wide operand and 16 to 64 KiB of ranks, or, above rank 64, 32 KiB and 64. Up
+// to rank 16 that is 80 KiB in all, so that a CU holds two.
 constexpr int low_batch(int mr) { return mr <= 4 ? 256 : 128; }
 
 // ---------------------------------------------------------------- weight gradients
@@ -265,7 +265,7 @@ __device__ inline void gate_grad(const GateGradArgs& a, uint32_t block) {
 // BATCH slots at a time. Few flops and short contractions: what bounds it is the
 // chain slot -> row -> product, so a batch's loads all go out together, and the
 // CU's other workgroups run meanwhile. Both gradients, and the gate's, share a launch: 8192 slots
-// of 8 rank-16 adapters by 1536 columns each way take 17.6 us (50 MB of gathered
+// of 8 rank-16 adapters by 1536 columns each way take 17 us (50 MB of gathered
 // rows, 10 us at a copy's rate; 26 with one workgroup a CU) and 6 for adding the
 // partial sums.
 //

@@ -83,7 +83,7 @@ constexpr bool narrow_product(uint64_t rows, uint32_t n, uint32_t k, uint32_t gr
 }
 // The wide products' tile: 256 x 256 or 256 x 128. A CU holds one workgroup of
 // either, and a square tile takes 1.75 times as long as the other (1.72 and
-// 0.97 us per 64 steps at 8192 x 8192 x 8192, 1288 and 1113 TFLOP/s), so it is
+// 0.97 us per 64 steps at 8192 x 8192 x 8192, in turn in short series), so it is
 // better where the number of rounds over the 256 CUs allows it: 8192 x 3584 x
 // 3584 takes 204 us with squares and 249 with halves, 4096 x 1536 x 1536 36 and
 // 24.5.

@@ -12,9 +12,10 @@
 // Both read their input once and write 12 bytes a slot; what bounds them is
 // the latency of the chain of dependent steps, at small sizes the launch.
 // Candidates are single numbers in a lane's registers, sorted once, and lanes
-// compare by DPP: 65536 tokens over 64 experts, 8 chosen, take 12.3 us for the
-// gate (19 MB to move, 4 us at a copy's rate: about 450 instructions a token's
-// lane are what it takes) and 10 us for the slots' places.
+// compare by DPP: 65536 tokens over 64 experts, 8 chosen, take 12.8 us for the
+// gate and 10 us for the slots' places. The gate moves 19 MB, 4 us at a copy's
+// rate; about 450 instructions a token's lane are some 6 us, and the rest is loads
+// that a workgroup's rounds of tokens wait for one after the other.
 #include "mixture.h"
 
 namespace {

@@ -35,7 +35,7 @@ __device__ inline void arrived_but(void) {
 // list_adapters runs under the main product's first loads and leaves in LDS the
 // adapters and, for up to KEPT choices, each row's and its coefficients; the
 // loads of one set of 64 ranks then go out together. 4096 x 1536 x 1536 with two
-// of 8 rank-16 adapters a token takes 35 us, 24.5 without adapters; with the
+// of 8 rank-16 adapters a token takes 37 us, 24.5 without adapters; with the
 // lists made after the main product and pieces loaded one by one it took 50.
 constexpr uint32_t KEPT = 4;
 template <int BM>
@@ -341,14 +341,15 @@ __device__ inline void put(const Out& out, f32x4 (&acc)[TN / 16][TM / 16], char*
 // steps, or, for y = x w, 64 rows of BN columns read through the transposing
 // LDS read.
 //
-// The matrix cores bound it: 8192 x 8192 x 8192 in bf16 runs at 1288 TFLOP/s
-// (y = x w: 1229), 95 % of what the library's product reaches on the card (1355,
-// at the clock the power leaves). 256 x 256 needs 64 KiB a tile, so two of them
-// and one workgroup of 8 wavefronts a CU; 4 wavefronts of 128 x 128 outputs did
-// not fit the registers, 128 x 128 tiles reach 924. Interleaving LDS reads, loads
-// and products in 8 pieces a half took 8192 x 3584 x 3584 from 231 to 215 us. What
-// is left there (204 us, floor 159) is 448 tiles on 256 CUs, two rounds of which
-// the second is three quarters full, and 4 us a round of stores.
+// The matrix cores bound it: 8192 x 8192 x 8192 in bf16 runs at 1452 TFLOP/s in a
+// long series (y = x w: 1331), 90 % of what the library's product reaches on the
+// card (1621, at the clock the power leaves). 256 x 256 needs 64 KiB a tile, so
+// two of them and one workgroup of 8 wavefronts a CU; 4 wavefronts of 128 x 128
+// outputs did not fit the registers, 128 x 128 tiles reach 924 in a short series.
+// Interleaving LDS reads, loads and products in 8 pieces a half took 8192 x 3584 x
+// 3584 from 231 to 215 us. What is left there (164 us in a long series, floor 130)
+// is 448 tiles on 256 CUs, two rounds of which the second is three quarters full,
+// and 4 us a round of stores.
 template <class T, int BM, int BN, int WM, int WN, int S, bool TR, bool LR>
 __global__ void __launch_bounds__(64 * WM * WN) wide_kernel(MatArgs a) {
   constexpr int WAVES = WM * WN, TM = BM / WM, TN = BN / WN;

@@ -15,7 +15,8 @@ none. Work is queued on torch's current stream of the tensors' device, and
 nothing waits for it. All three are differentiable (see each for what in; in
 reverse mode, once) and can be captured into a graph; forward-mode derivatives
 and tracing are refused. Values are bf16 or f16 with sums in float; the
-gate's logits may be f32 too. The C entry points are in
+gate's logits may be f32 too. At most 1024 experts or adapters (512 for a gate),
+32 choices a token and rank 128. The C entry points are in
 include/tensafe_he.h (th_route, th_group, th_grouped_matmul, th_lora_linear).
 
 The reference applies a single adapter to a single hidden state in the clear
