@@ -476,6 +476,52 @@ int th_lora_linear_backward_workspace(const th_lora_linear_args* d, size_t* byte
 int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const void* dy, int64_t lddy, void* dx,
                             void* da, void* db, float* dgate, void* work, size_t work_bytes, void* stream);
 
+/* ---------------------------------------------------------------- 4-bit weights */
+/* Frozen weights of the products above in 4 bits (no counterpart in the
+ * reference). A weight is the value scale * (code - zero) rounded to dtype, with
+ * codes and zeros in 0 .. 15 and a scale (and zero) of each row's `group`
+ * neighbouring columns; without zeros, zero is 8. Every call multiplies with
+ * exactly these values. `data` holds all of it in the layout that the products
+ * read (th_weight4_bytes bytes on a multiple of 16); what may be relied on is
+ * that these calls agree on it. A scale that is not a finite number, or for bf16
+ * above 2^120, makes its group's values NaN. */
+typedef struct th_weight4 {
+  int dtype; /* TH_BF16 or TH_F16: scales and values */
+  uint32_t matrices, d_out, d_in;
+  uint32_t group; /* columns of a scale: a power of two, 32 to 2^30 */
+  int zeros;      /* whether groups have zeros */
+  void* data;
+} th_weight4;
+int th_weight4_bytes(const th_weight4* w, size_t* bytes);
+/* Fills data from given codes (a byte each, the low 4 bits; matrices of d_out
+ * rows), scales (matrices x d_out x ceil(d_in / group), contiguous, of dtype) and
+ * zeros (the same in bytes; NULL without). */
+int th_pack4(const th_weight4* w, const uint8_t* codes, int64_t ldc, int64_t ldc_matrix, const void* scales,
+             const uint8_t* zeros, void* stream);
+/* Fills data from values of dtype. Without zeros, scale = max |w| / 7 and codes 1
+ * .. 15; with zeros, scale = (max - min) / 15 over the group's values and 0, and
+ * zero = -min / scale; both rounded to dtype before the codes are, ties to even.
+ * A group with an infinity or NaN becomes NaN. */
+int th_quantize4(const th_weight4* w, const void* values, int64_t ldv, int64_t ldv_matrix, void* stream);
+/* The values (matrices of d_out rows). */
+int th_dequantize4(const th_weight4* w, void* values, int64_t ldv, int64_t ldv_matrix, void* stream);
+/* th_grouped_matmul and th_lora_linear with 4-bit weights (of the descriptor's
+ * dtype and sizes) in place of d->w (ldw, ldwe) and d->weight (ldw), which are not
+ * read. The weights are frozen: there is no gradient of theirs. */
+int th_grouped_matmul4_workspace(const th_grouped* d, const th_weight4* w, size_t* bytes);
+int th_grouped_matmul4(const th_grouped* d, const th_weight4* w, void* y, int64_t ldy, void* work, size_t work_bytes,
+                       void* stream);
+int th_grouped_matmul4_backward_workspace(const th_grouped* d, const th_weight4* w, size_t* bytes);
+int th_grouped_matmul4_backward(const th_grouped* d, const th_weight4* w, const void* dy, int64_t lddy, void* dx,
+                                void* work, size_t work_bytes, void* stream);
+int th_lora_linear4_workspace(const th_lora_linear_args* d, const th_weight4* w, int keep_u, size_t* bytes);
+int th_lora_linear4(const th_lora_linear_args* d, const th_weight4* w, void* y, int64_t ldy, float* u, void* work,
+                    size_t work_bytes, void* stream);
+int th_lora_linear4_backward_workspace(const th_lora_linear_args* d, const th_weight4* w, size_t* bytes);
+int th_lora_linear4_backward(const th_lora_linear_args* d, const th_weight4* w, const float* u, const void* dy,
+                             int64_t lddy, void* dx, void* da, void* db, float* dgate, void* work, size_t work_bytes,
+                             void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -50,6 +50,12 @@ class LoraLinear(C.Structure):
                 ("experts", VP), ("gate", VP), ("scale", VP), ("order", VP), ("offsets", VP)]
 
 
+class Weight4(C.Structure):
+    """th_weight4"""
+    _fields_ = [("dtype", I32), ("matrices", U32), ("d_out", U32), ("d_in", U32), ("group", U32), ("zeros", I32),
+                ("data", VP)]
+
+
 _SIGS = {
     "th_last_error": (C.c_char_p, []),
     "th_version": (C.c_char_p, []),
@@ -120,6 +126,19 @@ _SIGS = {
     "th_lora_linear": (I32, [C.POINTER(LoraLinear), VP, I64, VP, VP, SZ, VP]),
     "th_lora_linear_backward_workspace": (I32, [C.POINTER(LoraLinear), C.POINTER(SZ)]),
     "th_lora_linear_backward": (I32, [C.POINTER(LoraLinear), VP, VP, I64, VP, VP, VP, VP, VP, SZ, VP]),
+    "th_weight4_bytes": (I32, [C.POINTER(Weight4), C.POINTER(SZ)]),
+    "th_pack4": (I32, [C.POINTER(Weight4), VP, I64, I64, VP, VP, VP]),
+    "th_quantize4": (I32, [C.POINTER(Weight4), VP, I64, I64, VP]),
+    "th_dequantize4": (I32, [C.POINTER(Weight4), VP, I64, I64, VP]),
+    "th_grouped_matmul4_workspace": (I32, [C.POINTER(Grouped), C.POINTER(Weight4), C.POINTER(SZ)]),
+    "th_grouped_matmul4": (I32, [C.POINTER(Grouped), C.POINTER(Weight4), VP, I64, VP, SZ, VP]),
+    "th_grouped_matmul4_backward_workspace": (I32, [C.POINTER(Grouped), C.POINTER(Weight4), C.POINTER(SZ)]),
+    "th_grouped_matmul4_backward": (I32, [C.POINTER(Grouped), C.POINTER(Weight4), VP, I64, VP, VP, SZ, VP]),
+    "th_lora_linear4_workspace": (I32, [C.POINTER(LoraLinear), C.POINTER(Weight4), I32, C.POINTER(SZ)]),
+    "th_lora_linear4": (I32, [C.POINTER(LoraLinear), C.POINTER(Weight4), VP, I64, VP, VP, SZ, VP]),
+    "th_lora_linear4_backward_workspace": (I32, [C.POINTER(LoraLinear), C.POINTER(Weight4), C.POINTER(SZ)]),
+    "th_lora_linear4_backward": (I32, [C.POINTER(LoraLinear), C.POINTER(Weight4), VP, VP, I64, VP, VP, VP, VP, VP, SZ,
+                                       VP]),
     "th_ntt_time": (I32, [VP, VP, SZ, U32, I32, I32, C.POINTER(C.c_float)]),
 }
 

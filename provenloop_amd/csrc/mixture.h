@@ -3,6 +3,8 @@
 //   narrow.hip    matrix products of few output tiles
 //   wide.hip      large ones, of ragged groups or with low-rank adapters added
 //   grouped.hip   weight gradients of groups and of low-rank factors
+//   four.hip      4-bit weights: quantizing, laying out, their values
+//   narrow4.hip   products of few output tiles with them
 //   mixture.hip   argument checks, workspaces and the C entry points
 // They know nothing of a CKKS context: each call runs on the stream it is
 // given, in memory its caller owns.
@@ -56,6 +58,34 @@ hipError_t launch_group(RouteArgs a, hipStream_t s);
 hipError_t launch_route_backward(MixType type, const RouteArgs& a, const float* dweights, void* dlogits,
                                  hipStream_t s);
 
+// 4-bit weights (mixture_rules.h): scale * (code - zero) rounded to the type.
+struct FourArgs {
+  const uint8_t* codes;  // null: a product's weights are not of 4 bits
+  const void* scales;
+  const uint8_t* zeros;  // null: 8 everywhere
+  th::FourLayout at;
+};
+// `data` of `matrices` weights in its three parts.
+inline FourArgs four_args(const void* data, const th::FourLayout& f, uint32_t matrices, bool zeros) {
+  const uint8_t* p = (const uint8_t*)data;
+  const uint8_t* s = p + matrices * f.codes();
+  return FourArgs{p, s, zeros ? s + matrices * f.scales() * 2 : nullptr, f};
+}
+// Rows of 2-byte values, or of codes, to 4-bit weights and back.
+struct FourRows {
+  const void* in;         // E matrices of rows x cols: values to quantize, or codes of a byte each
+  const void* scales;     // of codes: E x rows x scale_cols, contiguous
+  const uint8_t* zeros;   // of codes: the same, or null
+  void* out;              // the values, from 4-bit weights
+  FourArgs four;          // what is written, or read for the values
+  int64_t ld, lde;        // of `in` or `out`
+  uint32_t E, rows, cols, scale_cols;
+  uint32_t out_cols;      // values: columns written, zeros from cols on
+};
+hipError_t launch_quantize4(MixType type, const FourRows& a, hipStream_t s);
+hipError_t launch_pack4(MixType type, const FourRows& a, hipStream_t s);
+hipError_t launch_dequantize4(MixType type, const FourRows& a, hipStream_t s);
+
 // Rows of a matrix product. Without groups, row i of `x` gives row i of `y`.
 // With them, slot order[i] (offsets[g] <= i < offsets[g + 1]) reads row
 // slot / div of x, multiplies by matrix g of w and writes row slot of y; slots
@@ -82,10 +112,12 @@ struct MatArgs {
   const float* scale;      // null, or per adapter
   int64_t ldp, ldpe;
   uint32_t r, ru, kc;
+  FourArgs four;  // in place of w
 };
 // w is n x k (transposed = 0: y = x w^T) or k x n (1: y = x w).
 hipError_t launch_mat(MixType type, const MatArgs& a, int transposed, hipStream_t s);
 hipError_t launch_narrow(MixType type, const MatArgs& a, int transposed, hipStream_t s);  // launch_mat's choice
+hipError_t launch_narrow4(MixType type, const MatArgs& a, hipStream_t s);  // y = x w^T with a.four for w
 
 // out[g] = sum over the slots s of group g of left[s] (outer) right[s / div]:
 // n x k per group, with left row s of dy (n values), right row s / div of x (k).

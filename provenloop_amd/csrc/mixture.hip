@@ -112,15 +112,68 @@ void make_copies(Stack& a, Stack& b, Stack& c, hipStream_t s) {
   HIPCHK(launch_pad(set, s));
 }
 
+// ---------------------------------------------------------------- 4-bit weights
+th::FourLayout check_weight4(const th_weight4* w, bool data = true) {
+  need(w != nullptr, "null weight");
+  mix_type(w->dtype, false);
+  need(w->matrices >= 1 && w->d_in >= 1 && w->d_out >= 1, "matrices, d_in and d_out must be positive");
+  need(w->d_in <= 1u << 30 && w->d_out <= 1u << 30, "d_in and d_out must be at most 2^30");
+  need(w->group >= th::FOUR_MIN_GROUP && w->group <= th::FOUR_MAX_GROUP && (w->group & (w->group - 1)) == 0,
+       "group must be a power of two from 32 to 2^30");
+  if (data) {
+    need(w->data != nullptr, "null data of a 4-bit weight");
+    need(((uintptr_t)w->data & 15) == 0, "the data of a 4-bit weight must start on a multiple of 16 bytes");
+  }
+  return th::four_layout(w->d_out, w->d_in, w->group);
+}
+FourArgs four_of(const th_weight4* w) {
+  return four_args(w->data, th::four_layout(w->d_out, w->d_in, w->group), w->matrices, w->zeros != 0);
+}
+// The 4-bit weight of a product, or null.
+void check_operand4(const th_weight4* w, int dtype, uint32_t matrices, uint32_t d_out, uint32_t d_in) {
+  check_weight4(w);
+  need(w->dtype == dtype, "the 4-bit weight must have the other operands' dtype");
+  need(w->matrices == matrices && w->d_out == d_out && w->d_in == d_in, "the 4-bit weight has other sizes");
+}
+FourRows four_rows(const th_weight4* w, int64_t ld, int64_t ld_matrix) {
+  FourRows a{};
+  a.four = four_of(w);
+  a.ld = ld;
+  a.lde = ld_matrix;
+  a.E = w->matrices;
+  a.rows = w->d_out;
+  a.cols = w->d_in;
+  a.out_cols = w->d_in;
+  a.scale_cols = (uint32_t)th::ceil_div(w->d_in, w->group);
+  return a;
+}
+// The place of its values in a workspace, as a stack of rows of a multiple of 8.
+Stack values4(Pieces& p, const th_weight4* w) {
+  Stack t{nullptr, 0, 0, w->matrices, w->d_in, w->d_out, nullptr};
+  t.lay(p, true);
+  return t;
+}
+void make_values4(Stack& t, const th_weight4* w, hipStream_t s) {
+  t.use_copy();
+  FourRows a = four_rows(w, t.ld, t.lde);
+  a.out = t.copy;
+  a.out_cols = t.cols;
+  HIPCHK(launch_dequantize4((MixType)w->dtype, a, s));
+}
+
 // ---------------------------------------------------------------- grouped products
-void check_grouped(const th_grouped* d) {
+void check_grouped(const th_grouped* d, const th_weight4* four = nullptr) {
   need(d != nullptr, "null descriptor");
   mix_type(d->dtype, false);
   need_slots(d->tokens, d->experts, d->choices);
   need(d->d_in >= 1 && d->d_out >= 1, "d_in and d_out must be positive");
   need_rows(d->x, d->x_per_slot ? d->tokens * d->choices : d->tokens, d->ldx, d->d_in, "x");
-  need(d->w != nullptr, "null w");
-  need(d->ldw >= d->d_in, "w: the row stride is shorter than a row");
+  if (four) {
+    check_operand4(four, d->dtype, d->experts, d->d_out, d->d_in);
+  } else {
+    need(d->w != nullptr, "null w");
+    need(d->ldw >= d->d_in, "w: the row stride is shorter than a row");
+  }
   need(d->tokens == 0 || (d->order && d->offsets), "null groups");
 }
 
@@ -128,6 +181,29 @@ struct GroupedWork {
   Stack x{}, w{}, dy{};
   float* part = nullptr;  // a token's choices, to be summed
 };
+// y = w x of a product with 4-bit weights: whether small tiles take the codes
+// themselves; larger products go through the values.
+bool four_narrow(const th_grouped* d) {
+  return th::four_narrow(d->tokens * d->choices, d->d_out, d->d_in, d->experts);
+}
+bool four_narrow(const th_lora_linear_args* d) { return th::four_narrow(d->tokens, d->d_out, d->d_in, 1); }
+
+GroupedWork lay_grouped4(Pieces& p, const th_grouped* d, const th_weight4* w) {
+  GroupedWork g;
+  g.x = Stack{d->x, d->ldx, 0, 1, d->d_in, d->x_per_slot ? d->tokens * d->choices : d->tokens, nullptr};
+  g.x.lay(p, !g.x.ready());
+  if (!four_narrow(d)) g.w = values4(p, w);
+  return g;
+}
+GroupedWork lay_grouped4_backward(Pieces& p, const th_grouped* d, const th_weight4* w, const void* dy, int64_t lddy) {
+  GroupedWork g;
+  const int64_t slots = d->tokens * d->choices;
+  g.w = values4(p, w);
+  g.dy = Stack{dy, lddy, 0, 1, d->d_out, slots, nullptr};
+  g.dy.lay(p, d->d_out % 8 != 0);  // the workspace's size does not depend on where dy lies
+  if (!d->x_per_slot && d->choices > 1) g.part = p.take<float>((uint64_t)slots * d->d_in);
+  return g;
+}
 GroupedWork lay_grouped_backward(Pieces& p, const th_grouped* d, const void* dy, int64_t lddy) {
   GroupedWork g;
   const int64_t slots = d->tokens * d->choices;
@@ -140,16 +216,42 @@ GroupedWork lay_grouped_backward(Pieces& p, const th_grouped* d, const void* dy,
   return g;
 }
 
+// dx of grouped products, a token's choices summed.
+void grouped_dx(const th_grouped* d, const GroupedWork& g, void* dx, hipStream_t s) {
+  const int64_t slots = d->tokens * d->choices;
+  const bool summed = !d->x_per_slot && d->choices > 1;
+  MatArgs m{};
+  m.x = g.dy.p;
+  m.ldx = g.dy.ld;
+  m.w = g.w.p;
+  m.ldw = g.w.ld;
+  m.ldwe = g.w.lde;
+  m.y = summed ? (void*)g.part : dx;
+  m.y_float = summed;
+  m.ldy = d->d_in;
+  m.order = d->order;
+  m.offsets = d->offsets;
+  m.rows = slots;
+  m.n = d->d_in;
+  m.k = d->d_out;
+  m.E = d->experts;
+  m.div = 1;
+  m.aligned = g.dy.ready() && g.w.ready();
+  HIPCHK(launch_mat((MixType)d->dtype, m, 1, s));
+  if (summed) HIPCHK(launch_sum_choices((MixType)d->dtype, g.part, dx, d->tokens, d->choices, d->d_in, s));
+}
+
 // ---------------------------------------------------------------- shared projection with adapters
-void check_lora(const th_lora_linear_args* d) {
+void check_lora(const th_lora_linear_args* d, const th_weight4* four = nullptr) {
   need(d != nullptr, "null descriptor");
   mix_type(d->dtype, false);
   need_slots(d->tokens, d->adapters, d->choices);
   need(d->d_in >= 1 && d->d_out >= 1, "d_in and d_out must be positive");
   need(d->rank >= 1 && d->rank <= th::MIX_MAX_RANK, "rank must be in [1, " + std::to_string(th::MIX_MAX_RANK) + "]");
   need_rows(d->x, d->tokens, d->ldx, d->d_in, "x");
-  need(d->weight && d->a && d->b, "null weight or adapter");
-  need(d->ldw >= d->d_in, "weight: the row stride is shorter than a row");
+  need((four || d->weight) && d->a && d->b, "null weight or adapter");
+  if (four) check_operand4(four, d->dtype, 1, d->d_out, d->d_in);
+  else need(d->ldw >= d->d_in, "weight: the row stride is shorter than a row");
   need(d->lda >= d->d_in, "a: the row stride is shorter than a row");
   need(d->ldb >= d->rank, "b: the row stride is shorter than a row");
   need(d->tokens == 0 || d->experts, "null experts");
@@ -180,16 +282,22 @@ LoraWork lay_groups(Pieces& p, const th_lora_linear_args* d, bool own_lists = fa
   }
   return w;
 }
-LoraWork lay_forward(Pieces& p, const th_lora_linear_args* d, bool keep_u) {
+LoraWork lay_forward(Pieces& p, const th_lora_linear_args* d, bool keep_u, const th_weight4* four = nullptr) {
   LoraWork w = lay_groups(p, d, scans(d, keep_u));
-  for (Stack* t : {&w.x, &w.weight, &w.a}) t->lay(p, th::pad_operands(d->tokens, d->d_in) && !t->ready());
+  const bool pad = four || th::pad_operands(d->tokens, d->d_in);
+  for (Stack* t : {&w.x, &w.a}) t->lay(p, pad && !t->ready());
+  if (!four) w.weight.lay(p, pad && !w.weight.ready());
+  else if (!four_narrow(d)) w.weight = values4(p, four);
   if (!keep_u) w.u = p.take<float>((uint64_t)d->tokens * d->choices * padded_rank(d->rank));
   return w;
 }
-LoraWork lay_backward(Pieces& p, const th_lora_linear_args* d, const void* dy, int64_t lddy) {
+LoraWork lay_backward(Pieces& p, const th_lora_linear_args* d, const void* dy, int64_t lddy,
+                      const th_weight4* four = nullptr) {
   LoraWork w = lay_groups(p, d);
   w.dy = Stack{dy, lddy, 0, 1, d->d_out, d->tokens, nullptr};
-  for (Stack* t : {&w.x, &w.weight}) t->lay(p, !t->ready());
+  w.x.lay(p, !w.x.ready());
+  if (four) w.weight = values4(p, four);
+  else w.weight.lay(p, !w.weight.ready());
   w.dy.lay(p, d->d_out % 8 != 0);  // the workspace's size does not depend on where dy lies
   const uint64_t slots = (uint64_t)d->tokens * d->choices;
   w.v = p.take<float>(slots * padded_rank(d->rank));
@@ -259,6 +367,131 @@ void set_lowrank(MatArgs& m, const th_lora_linear_args* d, const float* u, const
   m.ru = padded_rank(d->rank);
   m.kc = d->choices;
   m.E = d->adapters;
+}
+
+// ---------------------------------------------------------------- the shared projection, its weight of 16 or 4 bits
+void lora_workspace(const th_lora_linear_args* d, const th_weight4* four, int keep_u, size_t* bytes) {
+  need(bytes != nullptr, "null output");
+  check_lora(d, four);
+  Pieces p(nullptr);
+  lay_forward(p, d, keep_u != 0, four);
+  *bytes = p.used();
+}
+void lora_forward(const th_lora_linear_args* d, const th_weight4* four, void* y, int64_t ldy, float* u, void* work,
+                  size_t work_bytes, void* stream) {
+  check_lora(d, four);
+  need_rows(y, d->tokens, ldy, d->d_out, "y");
+  Pieces p(work);
+  LoraWork w = lay_forward(p, d, u != nullptr, four);
+  need_work(work, work_bytes, p.used());
+  need_device();
+  if (d->tokens == 0) return;
+  const hipStream_t s = (hipStream_t)stream;
+  float* low = u ? u : w.u;
+  if (!scans(d, u != nullptr)) make_groups(d, w, s);
+  const bool codes = four && four_narrow(d);  // the product takes the codes, with no values of them in memory
+  Stack none{};
+  make_copies(w.x, four ? none : w.weight, w.a, s);
+  if (four && !codes) make_values4(w.weight, four, s);
+  shrink(d, w, w.x, w.a, low, s);
+  MatArgs m{};
+  m.x = w.x.p;
+  m.ldx = w.x.ld;
+  m.w = w.weight.p;
+  m.ldw = w.weight.ld;
+  m.y = y;
+  m.ldy = ldy;
+  m.bias = d->bias;
+  m.rows = d->tokens;
+  m.n = d->d_out;
+  m.k = w.x.cols;
+  m.div = 1;
+  m.aligned = w.x.ready() && (codes || w.weight.ready());
+  set_lowrank(m, d, low, d->b, d->ldb, d->ldb_adapter);
+  if (codes) {
+    m.four = four_of(four);
+    HIPCHK(launch_narrow4((MixType)d->dtype, m, s));
+  } else {
+    HIPCHK(launch_mat((MixType)d->dtype, m, 0, s));
+  }
+}
+void lora_backward_workspace(const th_lora_linear_args* d, const th_weight4* four, size_t* bytes) {
+  need(bytes != nullptr, "null output");
+  check_lora(d, four);
+  Pieces p(nullptr);
+  lay_backward(p, d, nullptr, d->d_out, four);
+  *bytes = p.used();
+}
+void lora_backward(const th_lora_linear_args* d, const th_weight4* four, const float* u, const void* dy, int64_t lddy,
+                   void* dx, void* da, void* db, float* dgate, void* work, size_t work_bytes, void* stream) {
+  check_lora(d, four);
+  need_rows(dy, d->tokens, lddy, d->d_out, "dy");
+  need(d->tokens == 0 || u != nullptr || !(db || dgate), "null u");
+  Pieces p(work);
+  LoraWork w = lay_backward(p, d, dy, lddy, four);
+  need_work(work, work_bytes, p.used());
+  need_device();
+  const hipStream_t s = (hipStream_t)stream;
+  const MixType type = (MixType)d->dtype;
+  const uint32_t ru = padded_rank(d->rank);
+  const int64_t slots = d->tokens * d->choices;
+  make_groups(d, w, s);
+  Stack none{};
+  if (slots) make_copies(w.x, four ? none : w.weight, w.dy, s);
+  if (slots && (dx || da || dgate)) {
+    TransposePair t{};
+    t.p[0] = TransposeArgs{d->b, w.bt, d->ldb, d->ldb_adapter, d->adapters, d->d_out, d->rank, w.dy.padded()};
+    if (dx) t.p[1] = TransposeArgs{d->a, w.at, d->lda, d->lda_adapter, d->adapters, d->rank, d->d_in, d->rank};
+    HIPCHK(launch_transpose(t, s));
+    const uint32_t n = w.dy.padded();
+    shrink(d, w, w.dy, Stack{w.bt, n, (int64_t)n * d->rank, d->adapters, n, d->rank, nullptr}, w.v, s);
+  }
+  if (slots && dx) {
+    if (four) make_values4(w.weight, four, s);
+    MatArgs m{};
+    m.x = w.dy.p;
+    m.ldx = w.dy.ld;
+    m.w = w.weight.p;
+    m.ldw = w.weight.ld;
+    m.y = dx;
+    m.ldy = d->d_in;
+    m.rows = d->tokens;
+    m.n = d->d_in;
+    m.k = d->d_out;
+    m.div = 1;
+    m.aligned = w.dy.ready() && w.weight.ready();
+    set_lowrank(m, d, w.v, w.at, d->rank, (int64_t)d->d_in * d->rank);
+    HIPCHK(launch_mat(type, m, 1, s));
+  }
+  GateGradArgs gate{u, w.v, d->experts, d->scale, dgate, slots, d->rank, ru, d->adapters};
+  if (da || db) {
+    LowOuterPair pair{};
+    pair.gate = gate;
+    for (int which = 0; which < 2; ++which) {
+      LowOuterArgs& o = pair.p[which];
+      o.low = which ? u : w.v;
+      const Stack& wide = which ? w.dy : w.x;
+      o.wide = wide.p;
+      o.ldwide = wide.ld;
+      o.cols = which ? d->d_out : d->d_in;
+      o.out = which ? db : da;
+      o.partial = w.partial[which];
+      o.order = w.order;
+      o.offsets = w.offsets;
+      o.gate = d->gate;
+      o.scale = d->scale;
+      o.slots = slots;
+      o.r = d->rank;
+      o.ru = ru;
+      o.E = d->adapters;
+      o.div = d->choices;
+      o.span = th::lowrank_span(slots, o.cols);
+      o.aligned = !o.out || wide.ready();
+      o.transposed = which;
+    }
+    HIPCHK(launch_low_outer(type, pair, s));
+  }
+  if (dgate && !(da || db)) HIPCHK(launch_gate_grad(gate, s));
 }
 
 }  // namespace
@@ -392,7 +625,6 @@ int th_grouped_matmul_backward(const th_grouped* d, const void* dy, int64_t lddy
     check_grouped(d);
     need_rows(dy, d->tokens * d->choices, lddy, d->d_out, "dy");
     const MixType type = (MixType)d->dtype;
-    const bool summed = !d->x_per_slot && d->choices > 1;
     Pieces p(work);
     GroupedWork g = lay_grouped_backward(p, d, dy, lddy);
     need_work(work, work_bytes, p.used());
@@ -400,27 +632,7 @@ int th_grouped_matmul_backward(const th_grouped* d, const void* dy, int64_t lddy
     const hipStream_t s = (hipStream_t)stream;
     const int64_t slots = d->tokens * d->choices;
     if (slots) make_copies(g.x, g.w, g.dy, s);
-    if (dx) {
-      MatArgs m{};
-      m.x = g.dy.p;
-      m.ldx = g.dy.ld;
-      m.w = g.w.p;
-      m.ldw = g.w.ld;
-      m.ldwe = g.w.lde;
-      m.y = summed ? (void*)g.part : dx;
-      m.y_float = summed;
-      m.ldy = d->d_in;
-      m.order = d->order;
-      m.offsets = d->offsets;
-      m.rows = slots;
-      m.n = d->d_in;
-      m.k = d->d_out;
-      m.E = d->experts;
-      m.div = 1;
-      m.aligned = g.dy.ready() && g.w.ready();
-      HIPCHK(launch_mat(type, m, 1, s));
-      if (summed) HIPCHK(launch_sum_choices(type, g.part, dx, d->tokens, d->choices, d->d_in, s));
-    }
+    if (dx) grouped_dx(d, g, dx, s);
     if (dw) {
       OuterArgs o{};
       o.dy = g.dy.p;
@@ -443,127 +655,179 @@ int th_grouped_matmul_backward(const th_grouped* d, const void* dy, int64_t lddy
 }
 
 int th_lora_linear_workspace(const th_lora_linear_args* d, int keep_u, size_t* bytes) {
+  return guarded([&] { lora_workspace(d, nullptr, keep_u, bytes); });
+}
+int th_lora_linear4_workspace(const th_lora_linear_args* d, const th_weight4* w, int keep_u, size_t* bytes) {
   return guarded([&] {
-    need(bytes != nullptr, "null output");
-    check_lora(d);
-    Pieces p(nullptr);
-    lay_forward(p, d, keep_u != 0);
-    *bytes = p.used();
+    check_weight4(w);
+    lora_workspace(d, w, keep_u, bytes);
   });
 }
 
 int th_lora_linear(const th_lora_linear_args* d, void* y, int64_t ldy, float* u, void* work, size_t work_bytes,
                    void* stream) {
+  return guarded([&] { lora_forward(d, nullptr, y, ldy, u, work, work_bytes, stream); });
+}
+int th_lora_linear4(const th_lora_linear_args* d, const th_weight4* w, void* y, int64_t ldy, float* u, void* work,
+                    size_t work_bytes, void* stream) {
   return guarded([&] {
-    check_lora(d);
-    need_rows(y, d->tokens, ldy, d->d_out, "y");
-    Pieces p(work);
-    LoraWork w = lay_forward(p, d, u != nullptr);
-    need_work(work, work_bytes, p.used());
-    need_device();
-    if (d->tokens == 0) return;
-    const hipStream_t s = (hipStream_t)stream;
-    float* low = u ? u : w.u;
-    if (!scans(d, u != nullptr)) make_groups(d, w, s);
-    make_copies(w.x, w.weight, w.a, s);
-    shrink(d, w, w.x, w.a, low, s);
-    MatArgs m{};
-    m.x = w.x.p;
-    m.ldx = w.x.ld;
-    m.w = w.weight.p;
-    m.ldw = w.weight.ld;
-    m.y = y;
-    m.ldy = ldy;
-    m.bias = d->bias;
-    m.rows = d->tokens;
-    m.n = d->d_out;
-    m.k = w.x.cols;
-    m.div = 1;
-    m.aligned = w.x.ready() && w.weight.ready();
-    set_lowrank(m, d, low, d->b, d->ldb, d->ldb_adapter);
-    HIPCHK(launch_mat((MixType)d->dtype, m, 0, s));
+    check_weight4(w);
+    lora_forward(d, w, y, ldy, u, work, work_bytes, stream);
   });
 }
 
 int th_lora_linear_backward_workspace(const th_lora_linear_args* d, size_t* bytes) {
+  return guarded([&] { lora_backward_workspace(d, nullptr, bytes); });
+}
+int th_lora_linear4_backward_workspace(const th_lora_linear_args* d, const th_weight4* w, size_t* bytes) {
   return guarded([&] {
-    need(bytes != nullptr, "null output");
-    check_lora(d);
-    Pieces p(nullptr);
-    lay_backward(p, d, nullptr, d->d_out);
-    *bytes = p.used();
+    check_weight4(w);
+    lora_backward_workspace(d, w, bytes);
   });
 }
 
 int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const void* dy, int64_t lddy, void* dx,
                             void* da, void* db, float* dgate, void* work, size_t work_bytes, void* stream) {
+  return guarded([&] { lora_backward(d, nullptr, u, dy, lddy, dx, da, db, dgate, work, work_bytes, stream); });
+}
+int th_lora_linear4_backward(const th_lora_linear_args* d, const th_weight4* w, const float* u, const void* dy,
+                             int64_t lddy, void* dx, void* da, void* db, float* dgate, void* work, size_t work_bytes,
+                             void* stream) {
   return guarded([&] {
-    check_lora(d);
-    need_rows(dy, d->tokens, lddy, d->d_out, "dy");
-    need(d->tokens == 0 || u != nullptr || !(db || dgate), "null u");
+    check_weight4(w);
+    lora_backward(d, w, u, dy, lddy, dx, da, db, dgate, work, work_bytes, stream);
+  });
+}
+
+// ---------------------------------------------------------------- 4-bit weights
+int th_weight4_bytes(const th_weight4* w, size_t* bytes) {
+  return guarded([&] {
+    need(bytes != nullptr, "null output");
+    const th::FourLayout f = check_weight4(w, false);
+    *bytes = th::four_bytes(f, w->matrices, w->zeros != 0);
+  });
+}
+
+int th_pack4(const th_weight4* w, const uint8_t* codes, int64_t ldc, int64_t ldc_matrix, const void* scales,
+             const uint8_t* zeros, void* stream) {
+  return guarded([&] {
+    check_weight4(w);
+    need_rows(codes, w->d_out, ldc, w->d_in, "codes");
+    need(scales != nullptr, "null scales");
+    need((zeros != nullptr) == (w->zeros != 0), "zeros are given exactly for a weight that has them");
+    need_device();
+    FourRows a = four_rows(w, ldc, ldc_matrix);
+    a.in = codes;
+    a.scales = scales;
+    a.zeros = zeros;
+    HIPCHK(launch_pack4((MixType)w->dtype, a, (hipStream_t)stream));
+  });
+}
+
+int th_quantize4(const th_weight4* w, const void* values, int64_t ldv, int64_t ldv_matrix, void* stream) {
+  return guarded([&] {
+    check_weight4(w);
+    need_rows(values, w->d_out, ldv, w->d_in, "values");
+    need_device();
+    FourRows a = four_rows(w, ldv, ldv_matrix);
+    a.in = values;
+    HIPCHK(launch_quantize4((MixType)w->dtype, a, (hipStream_t)stream));
+  });
+}
+
+int th_dequantize4(const th_weight4* w, void* values, int64_t ldv, int64_t ldv_matrix, void* stream) {
+  return guarded([&] {
+    check_weight4(w);
+    need_rows(values, w->d_out, ldv, w->d_in, "values");
+    need_device();
+    FourRows a = four_rows(w, ldv, ldv_matrix);
+    a.out = values;
+    HIPCHK(launch_dequantize4((MixType)w->dtype, a, (hipStream_t)stream));
+  });
+}
+
+int th_grouped_matmul4_workspace(const th_grouped* d, const th_weight4* w, size_t* bytes) {
+  return guarded([&] {
+    need(bytes != nullptr, "null output");
+    check_weight4(w);
+    check_grouped(d, w);
+    Pieces p(nullptr);
+    lay_grouped4(p, d, w);
+    *bytes = p.used();
+  });
+}
+
+int th_grouped_matmul4(const th_grouped* d, const th_weight4* w, void* y, int64_t ldy, void* work, size_t work_bytes,
+                       void* stream) {
+  return guarded([&] {
+    check_weight4(w);
+    check_grouped(d, w);
+    const int64_t slots = d->tokens * d->choices;
+    need_rows(y, slots, ldy, d->d_out, "y");
     Pieces p(work);
-    LoraWork w = lay_backward(p, d, dy, lddy);
+    GroupedWork g = lay_grouped4(p, d, w);
     need_work(work, work_bytes, p.used());
     need_device();
+    if (slots == 0) return;
     const hipStream_t s = (hipStream_t)stream;
-    const MixType type = (MixType)d->dtype;
-    const uint32_t ru = padded_rank(d->rank);
+    const bool codes = four_narrow(d);
+    Stack none{};
+    make_copies(g.x, none, none, s);
+    if (!codes) make_values4(g.w, w, s);
+    MatArgs m{};
+    m.x = g.x.p;
+    m.ldx = g.x.ld;
+    m.w = g.w.p;
+    m.ldw = g.w.ld;
+    m.ldwe = g.w.lde;
+    m.y = y;
+    m.ldy = ldy;
+    m.order = d->order;
+    m.offsets = d->offsets;
+    m.rows = slots;
+    m.n = d->d_out;
+    m.k = g.x.cols;
+    m.E = d->experts;
+    m.div = d->x_per_slot ? 1 : d->choices;
+    m.aligned = 1;
+    if (codes) {
+      m.four = four_of(w);
+      HIPCHK(launch_narrow4((MixType)d->dtype, m, s));
+    } else {
+      HIPCHK(launch_mat((MixType)d->dtype, m, 0, s));
+    }
+  });
+}
+
+int th_grouped_matmul4_backward_workspace(const th_grouped* d, const th_weight4* w, size_t* bytes) {
+  return guarded([&] {
+    need(bytes != nullptr, "null output");
+    check_weight4(w);
+    check_grouped(d, w);
+    Pieces p(nullptr);
+    lay_grouped4_backward(p, d, w, nullptr, d->d_out);
+    *bytes = p.used();
+  });
+}
+
+int th_grouped_matmul4_backward(const th_grouped* d, const th_weight4* w, const void* dy, int64_t lddy, void* dx,
+                                void* work, size_t work_bytes, void* stream) {
+  return guarded([&] {
+    check_weight4(w);
+    check_grouped(d, w);
     const int64_t slots = d->tokens * d->choices;
-    make_groups(d, w, s);
-    if (slots) make_copies(w.x, w.weight, w.dy, s);
-    if (slots && (dx || da || dgate)) {
-      TransposePair t{};
-      t.p[0] = TransposeArgs{d->b, w.bt, d->ldb, d->ldb_adapter, d->adapters, d->d_out, d->rank, w.dy.padded()};
-      if (dx) t.p[1] = TransposeArgs{d->a, w.at, d->lda, d->lda_adapter, d->adapters, d->rank, d->d_in, d->rank};
-      HIPCHK(launch_transpose(t, s));
-      const uint32_t n = w.dy.padded();
-      shrink(d, w, w.dy, Stack{w.bt, n, (int64_t)n * d->rank, d->adapters, n, d->rank, nullptr}, w.v, s);
-    }
-    if (slots && dx) {
-      MatArgs m{};
-      m.x = w.dy.p;
-      m.ldx = w.dy.ld;
-      m.w = w.weight.p;
-      m.ldw = w.weight.ld;
-      m.y = dx;
-      m.ldy = d->d_in;
-      m.rows = d->tokens;
-      m.n = d->d_in;
-      m.k = d->d_out;
-      m.div = 1;
-      m.aligned = w.dy.ready() && w.weight.ready();
-      set_lowrank(m, d, w.v, w.at, d->rank, (int64_t)d->d_in * d->rank);
-      HIPCHK(launch_mat(type, m, 1, s));
-    }
-    GateGradArgs gate{u, w.v, d->experts, d->scale, dgate, slots, d->rank, ru, d->adapters};
-    if (da || db) {
-      LowOuterPair pair{};
-      pair.gate = gate;
-      for (int which = 0; which < 2; ++which) {
-        LowOuterArgs& o = pair.p[which];
-        o.low = which ? u : w.v;
-        const Stack& wide = which ? w.dy : w.x;
-        o.wide = wide.p;
-        o.ldwide = wide.ld;
-        o.cols = which ? d->d_out : d->d_in;
-        o.out = which ? db : da;
-        o.partial = w.partial[which];
-        o.order = w.order;
-        o.offsets = w.offsets;
-        o.gate = d->gate;
-        o.scale = d->scale;
-        o.slots = slots;
-        o.r = d->rank;
-        o.ru = ru;
-        o.E = d->adapters;
-        o.div = d->choices;
-        o.span = th::lowrank_span(slots, o.cols);
-        o.aligned = !o.out || wide.ready();
-        o.transposed = which;
-      }
-      HIPCHK(launch_low_outer(type, pair, s));
-    }
-    if (dgate && !(da || db)) HIPCHK(launch_gate_grad(gate, s));
+    need_rows(dy, slots, lddy, d->d_out, "dy");
+    need(slots == 0 || dx != nullptr, "null dx");
+    Pieces p(work);
+    GroupedWork g = lay_grouped4_backward(p, d, w, dy, lddy);
+    need_work(work, work_bytes, p.used());
+    need_device();
+    if (slots == 0) return;
+    const hipStream_t s = (hipStream_t)stream;
+    Stack none{};
+    make_copies(none, none, g.dy, s);
+    make_values4(g.w, w, s);
+    grouped_dx(d, g, dx, s);
   });
 }
 

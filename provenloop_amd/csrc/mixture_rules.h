@@ -101,6 +101,42 @@ constexpr bool pad_operands(uint64_t rows, uint32_t k) { return rows > 32 || k >
 constexpr uint32_t pad_blocks(uint64_t rows, uint32_t E, uint32_t cols) {
   return loop_blocks(ceil_div(rows * E * ceil_div(cols, 8), 256));
 }
+// 4-bit weights as they lie in memory: the codes of all matrices, then their
+// scales, then their zeros if they have any.
+//   codes   512 bytes for each 16 rows by 64 columns, such blocks along a strip
+//           of 16 rows, then strip after strip. Lane l of a wavefront has 8 bytes
+//           of a block at 8 l, row l % 16: a word for columns (l / 16) * 8 .. + 8
+//           and one for the same columns 32 on, which are its operands of two
+//           matrix instructions. Columns 2 i and 2 i + 1 of a word are its bits
+//           4 i .. + 4 and 16 + 4 i .. + 4: a shift and a mask leave a pair.
+//   scales  of a group of columns for every row, rows rounded up to 16, group
+//           after group (2 bytes each); zeros the same (a byte each).
+// Rows and columns beyond the matrix's have code 8; its groups and rows beyond
+// have scale 0. The columns of a scale are a power of two, so that a group's
+// number is a shift.
+constexpr uint32_t FOUR_MIN_GROUP = 32;       // the columns of a matrix instruction
+constexpr uint32_t FOUR_MAX_GROUP = 1u << 30;
+struct FourLayout {
+  uint32_t strips, blocks, groups, shift;     // strips of 16 rows, blocks of 64 columns, groups of 2^shift
+  constexpr uint64_t codes() const { return (uint64_t)strips * blocks * 512; }  // of one matrix
+  constexpr uint64_t scales() const { return (uint64_t)groups * strips * 16; }
+};
+constexpr FourLayout four_layout(uint32_t d_out, uint32_t d_in, uint32_t group) {
+  FourLayout f{(uint32_t)ceil_div(d_out, 16), (uint32_t)ceil_div(d_in, 64), 0, 0};
+  while ((1u << f.shift) < group) ++f.shift;
+  f.groups = (uint32_t)ceil_div((uint64_t)f.blocks * 64, group);
+  return f;
+}
+constexpr uint64_t four_bytes(const FourLayout& f, uint32_t matrices, bool zeros) {
+  return matrices * (f.codes() + f.scales() * (zeros ? 3 : 2));
+}
+
+// Whether a product with 4-bit weights goes by their codes in small tiles; a
+// larger one goes by their values, written to a workspace.
+constexpr bool four_narrow(uint64_t rows, uint32_t n, uint32_t k, uint32_t groups) {
+  return narrow_product(rows, n, k, groups);
+}
+
 // Slots whose adapters a workgroup of the low-rank product looks through by
 // itself, which saves the launch that would group them.
 constexpr uint32_t NARROW_SCAN_SLOTS = 2048;

@@ -213,6 +213,95 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> route(const Tensor& given, int64_t k,
   return {out[0], out[1], out[2], out[3]};
 }
 
+// ---------------------------------------------------------------- 4-bit weights
+// What provenloop_amd.mixture.Weight4 holds.
+struct Four {
+  Tensor data;
+  th_weight4 w{};
+
+  Four() = default;
+  Four(const char* name, const Tensor& given, int64_t dtype, const std::vector<int64_t>& shape, int64_t group, bool zeros)
+      : data(given) {
+    NEED(shape.size() == 2 || shape.size() == 3, name, ": a 4-bit weight is [d_out, d_in] or [E, d_out, d_in]");
+    for (const int64_t n : shape) NEED(n >= 1 && n <= 1 << 30, name, ": a 4-bit weight's sizes must be in [1, 2^30]");
+    NEED(group >= 1 && group <= 1 << 30, name, ": group_size must be a power of two from 32 to 2^30");
+    const size_t at = shape.size() - 2;
+    w.dtype = (int)dtype;
+    w.matrices = at ? (uint32_t)shape[0] : 1;
+    w.d_out = (uint32_t)shape[at];
+    w.d_in = (uint32_t)shape[at + 1];
+    w.group = (uint32_t)group;
+    w.zeros = zeros;
+    if (!data.defined()) return;
+    NEED(data.scalar_type() == at::kByte && data.is_contiguous() && (uint64_t)data.numel() == bytes(),
+         name, ": a 4-bit weight must be what pack4 or quantize4 returns");
+    w.data = data.data_ptr();
+  }
+  size_t bytes() const {
+    size_t n;
+    check(th_weight4_bytes(&w, &n));  // refuses what is out of range
+    return n;
+  }
+  // as saved with a graph's node
+  std::vector<int64_t> numbers() const { return {w.dtype, w.matrices, w.d_out, w.d_in, w.group, w.zeros}; }
+  Four(const Tensor& saved, const std::vector<int64_t>& n) : data(saved) {
+    w = th_weight4{(int)n[0], (uint32_t)n[1], (uint32_t)n[2], (uint32_t)n[3], (uint32_t)n[4], (int)n[5], data.data_ptr()};
+  }
+};
+at::ScalarType scalar_type(int dtype) { return dtype == TH_BF16 ? at::kBFloat16 : at::kHalf; }
+
+// Stride from matrix to matrix of [d_out, d_in] or [E, d_out, d_in].
+int64_t ld_matrix(const Tensor& t) { return t.dim() == 3 ? t.stride(0) : 0; }
+
+Tensor quantize4(const Tensor& given, int64_t group, bool zeros) {
+  not_traced("quantize4");
+  no_tangents("quantize4", given);
+  NEED(is_half(given), "quantize4: weight must be bf16 or f16");
+  const Four shape("quantize4", Tensor(), type_of(given), given.sizes().vec(), group, zeros);
+  const size_t bytes = shape.bytes();
+  on_gpu("quantize4", given);
+  Guard guard(given.device());
+  const Tensor values = rows(given);
+  Tensor data = make({(int64_t)bytes}, at::kByte, values);
+  th_weight4 w = shape.w;
+  w.data = data.data_ptr();
+  check(th_quantize4(&w, ptr(values), ld(values), ld_matrix(values), stream(values)));
+  return data;
+}
+
+Tensor pack4(const Tensor& given, const Tensor& given_scales, int64_t group, const OptTensor& given_zeros) {
+  not_traced("pack4");
+  no_tangents("pack4", given_scales);
+  NEED(given.scalar_type() == at::kByte, "pack4: codes must be uint8");
+  NEED(is_half(given_scales), "pack4: scales must be bf16 or f16");
+  NEED(!given_zeros || given_zeros->scalar_type() == at::kByte, "pack4: zeros must be uint8");
+  const Four shape("pack4", Tensor(), type_of(given_scales), given.sizes().vec(), group, given_zeros.has_value());
+  const size_t bytes = shape.bytes();
+  std::vector<int64_t> want = given.sizes().vec();
+  want.back() = (want.back() + group - 1) / group;
+  NEED(given_scales.sizes() == want, "pack4: scales must have a value per row and group of columns");
+  NEED(!given_zeros || given_zeros->sizes() == want, "pack4: zeros must be shaped as scales");
+  on_gpu("pack4", given, {given_scales, given_zeros ? *given_zeros : Tensor()});
+  Guard guard(given.device());
+  const Tensor codes = rows(given), scales = given_scales.contiguous();
+  const Tensor zeros = given_zeros ? given_zeros->contiguous() : Tensor();
+  Tensor data = make({(int64_t)bytes}, at::kByte, codes);
+  th_weight4 w = shape.w;
+  w.data = data.data_ptr();
+  check(th_pack4(&w, ptr<uint8_t>(codes), ld(codes), ld_matrix(codes), ptr(scales), ptr<uint8_t>(zeros), stream(codes)));
+  return data;
+}
+
+Tensor dequantize4(const Tensor& data, int64_t dtype, const std::vector<int64_t>& shape, int64_t group, bool zeros) {
+  not_traced("dequantize4");
+  const Four four("dequantize4", data, dtype, shape, group, zeros);
+  on_gpu("dequantize4", data);
+  Guard guard(data.device());
+  Tensor out = make(shape, scalar_type(four.w.dtype), data);
+  check(th_dequantize4(&four.w, ptr(out), four.w.d_in, (int64_t)four.w.d_out * four.w.d_in, stream(data)));
+  return out;
+}
+
 // ---------------------------------------------------------------- grouped products
 th_grouped grouped_args(const Tensor& x, const Tensor& w, int64_t t, int64_t k, const Tensor& order,
                         const Tensor& offsets) {
@@ -270,38 +359,118 @@ struct GroupedMatmul : Function<GroupedMatmul> {
   }
 };
 
+// x and the groups of a grouped product with contraction length d.
+void check_grouped(const Tensor& given_x, const Tensor& w, int64_t d, const Tensor& experts, const Tensor& order,
+                   const Tensor& offsets, int64_t n_groups) {
+  const int64_t t = experts.size(0), k = experts.size(1);
+  NEED((given_x.dim() == 2 && given_x.size(0) == t && given_x.size(1) == d) ||
+           (given_x.dim() == 3 && given_x.size(0) == t && given_x.size(1) == k && given_x.size(2) == d),
+       "grouped_matmul: x must be [T, d_in] or [T, k, d_in]");
+  on_gpu("grouped_matmul", given_x, {w, order, offsets});
+  NEED(order.scalar_type() == at::kInt && order.is_contiguous() && order.numel() == t * k &&
+           offsets.scalar_type() == at::kInt && offsets.is_contiguous() && offsets.numel() == n_groups + 1,
+       "grouped_matmul: groups must be what group or route returns");
+}
+
 Tensor grouped_matmul(const Tensor& given_x, const Tensor& given_w, const Tensor& experts, const Tensor& order,
                       const Tensor& offsets, int64_t n_groups) {
   not_traced("grouped_matmul");
   no_tangents("grouped_matmul", given_x, given_w);
   NEED(is_half(given_x), "grouped_matmul: x must be bf16 or f16");
   NEED(given_w.scalar_type() == given_x.scalar_type(), "grouped_matmul: x and w must have one type");
-  const int64_t t = experts.size(0), k = experts.size(1);
   NEED(given_w.dim() == 3 && given_w.size(0) == n_groups, "grouped_matmul: w must be [n_groups, d_out, d_in]");
-  const int64_t d = given_w.size(2);
-  NEED((given_x.dim() == 2 && given_x.size(0) == t && given_x.size(1) == d) ||
-           (given_x.dim() == 3 && given_x.size(0) == t && given_x.size(1) == k && given_x.size(2) == d),
-       "grouped_matmul: x must be [T, d_in] or [T, k, d_in]");
-  on_gpu("grouped_matmul", given_x, {given_w, order, offsets});
-  NEED(order.scalar_type() == at::kInt && order.is_contiguous() && order.numel() == t * k &&
-           offsets.scalar_type() == at::kInt && offsets.is_contiguous() && offsets.numel() == n_groups + 1,
-       "grouped_matmul: groups must be what group or route returns");
+  check_grouped(given_x, given_w, given_w.size(2), experts, order, offsets, n_groups);
+  const int64_t t = experts.size(0), k = experts.size(1);
   const Tensor x = given_x.dim() == 3 ? given_x.contiguous() : rows(given_x), w = rows(given_w);
   if ((x.requires_grad() || w.requires_grad()) && at::GradMode::is_enabled())
     return GroupedMatmul::apply(x, w, t, k, order, offsets);
   return grouped_forward(x, w, t, k, order, offsets);
 }
 
+// The same with 4-bit weights, which are frozen.
+th_grouped grouped4_args(const Tensor& x, const Four& four, int64_t t, int64_t k, const Tensor& order,
+                         const Tensor& offsets) {
+  th_grouped d{};
+  d.dtype = type_of(x);
+  d.x_per_slot = x.dim() == 3;
+  d.tokens = t;
+  d.choices = (uint32_t)k;
+  d.experts = four.w.matrices;
+  d.d_in = four.w.d_in;
+  d.d_out = four.w.d_out;
+  d.x = ptr(x);
+  d.ldx = ld(x);
+  d.order = ptr<int32_t>(order);
+  d.offsets = ptr<int32_t>(offsets);
+  return d;
+}
+
+Tensor grouped4_forward(const Tensor& x, const Four& four, int64_t t, int64_t k, const Tensor& order,
+                        const Tensor& offsets) {
+  Guard guard(x.device());
+  Tensor y = make({t, k, four.w.d_out}, x.scalar_type(), x);
+  const th_grouped d = grouped4_args(x, four, t, k, order, offsets);
+  size_t bytes;
+  check(th_grouped_matmul4_workspace(&d, &four.w, &bytes));
+  const Work wk = work(bytes, x);
+  check(th_grouped_matmul4(&d, &four.w, ptr(y), four.w.d_out, wk.p, wk.bytes, stream(x)));
+  return y;
+}
+
+struct GroupedMatmul4 : Function<GroupedMatmul4> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Four& four, int64_t t, int64_t k,
+                        const Tensor& order, const Tensor& offsets) {
+    ctx->save_for_backward({four.data, order, offsets});
+    ctx->saved_data["four"] = four.numbers();
+    ctx->saved_data["x"] = x.sizes();
+    ctx->saved_data["k"] = k;
+    return grouped4_forward(x, four, t, k, order, offsets);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const variable_list saved = ctx->get_saved_variables();
+    no_tangents("grouped_matmul's gradient", grads[0]);
+    const Tensor dy = grads[0].contiguous();
+    Guard guard(dy.device());
+    const Four four(saved[0], ctx->saved_data["four"].toIntVector());
+    Tensor dx = make(ctx->saved_data["x"].toIntVector(), dy.scalar_type(), dy);
+    const th_grouped d = grouped4_args(dx, four, dx.size(0), ctx->saved_data["k"].toInt(), saved[1], saved[2]);
+    size_t bytes;
+    check(th_grouped_matmul4_backward_workspace(&d, &four.w, &bytes));
+    const Work wk = work(bytes, dy);
+    check(th_grouped_matmul4_backward(&d, &four.w, ptr(dy), four.w.d_out, ptr(dx), wk.p, wk.bytes, stream(dy)));
+    return once({dx, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()});
+  }
+};
+
+Tensor grouped_matmul4(const Tensor& given_x, const Tensor& data, int64_t dtype, const std::vector<int64_t>& shape,
+                       int64_t group, bool zeros, const Tensor& experts, const Tensor& order, const Tensor& offsets,
+                       int64_t n_groups) {
+  not_traced("grouped_matmul");
+  no_tangents("grouped_matmul", given_x);
+  NEED(is_half(given_x), "grouped_matmul: x must be bf16 or f16");
+  NEED(dtype == type_of(given_x), "grouped_matmul: x and w must have one type");
+  NEED(shape.size() == 3 && shape[0] == n_groups, "grouped_matmul: w must be [n_groups, d_out, d_in]");
+  const Four four("grouped_matmul", data, dtype, shape, group, zeros);
+  check_grouped(given_x, data, shape[2], experts, order, offsets, n_groups);
+  const Tensor x = given_x.dim() == 3 ? given_x.contiguous() : rows(given_x);
+  const int64_t t = experts.size(0), k = experts.size(1);
+  if (x.requires_grad() && at::GradMode::is_enabled()) return GroupedMatmul4::apply(x, four, t, k, order, offsets);
+  return grouped4_forward(x, four, t, k, order, offsets);
+}
+
 // ---------------------------------------------------------------- shared projection with adapters
 struct Lora {
+  Four four;  // in place of weight, if it has data
   Tensor x, weight, bias, a, b, experts, gate, scale, order, offsets;
+  bool has4() const { return four.data.defined(); }
+  int64_t d_out() const { return has4() ? four.w.d_out : weight.size(0); }
   th_lora_linear_args args() const {
     th_lora_linear_args d{};
     d.dtype = type_of(x);
     d.choices = (uint32_t)experts.size(1);
     d.tokens = experts.size(0);
     d.d_in = (uint32_t)x.size(1);
-    d.d_out = (uint32_t)weight.size(0);
+    d.d_out = (uint32_t)d_out();
     d.rank = (uint32_t)a.size(1);
     d.adapters = (uint32_t)a.size(0);
     d.x = ptr(x);
@@ -310,7 +479,7 @@ struct Lora {
     d.a = ptr(a);
     d.b = ptr(b);
     d.ldx = ld(x);
-    d.ldw = ld(weight);
+    d.ldw = has4() ? 0 : ld(weight);
     d.lda = ld(a);
     d.lda_adapter = a.stride(0);
     d.ldb = ld(b);
@@ -326,13 +495,15 @@ struct Lora {
 
 Tensor lora_forward(const Lora& l, const Tensor& u) {
   Guard guard(l.x.device());
-  const int64_t n = l.weight.size(0);
+  const int64_t n = l.d_out();
   Tensor y = make({l.x.size(0), n}, l.x.scalar_type(), l.x);
   const th_lora_linear_args d = l.args();
   size_t bytes;
-  check(th_lora_linear_workspace(&d, u.defined(), &bytes));
+  check(l.has4() ? th_lora_linear4_workspace(&d, &l.four.w, u.defined(), &bytes)
+                 : th_lora_linear_workspace(&d, u.defined(), &bytes));
   const Work w = work(bytes, l.x);
-  check(th_lora_linear(&d, ptr(y), n, ptr<float>(u), w.p, w.bytes, stream(l.x)));
+  check(l.has4() ? th_lora_linear4(&d, &l.four.w, ptr(y), n, ptr<float>(u), w.p, w.bytes, stream(l.x))
+                 : th_lora_linear(&d, ptr(y), n, ptr<float>(u), w.p, w.bytes, stream(l.x)));
   return y;
 }
 
@@ -351,12 +522,17 @@ struct LoraLinear : Function<LoraLinear> {
     }
     // u rows: the rank rounded up to 4
     Tensor u = make({l.experts.numel(), (a.size(1) + 3) / 4 * 4}, at::kFloat, x);
-    ctx->save_for_backward({x, a, b, l.gate, l.weight, l.bias, l.experts, l.scale, l.order, l.offsets, u});
+    ctx->save_for_backward(
+        {x, a, b, l.gate, l.has4() ? l.four.data : l.weight, l.bias, l.experts, l.scale, l.order, l.offsets, u});
+    if (l.has4()) ctx->saved_data["four"] = l.four.numbers();
     return lora_forward(l, u);
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list s = ctx->get_saved_variables();
-    const Lora l{s[0], s[4], s[5], s[1], s[2], s[6], s[3], s[7], s[8], s[9]};
+    const auto numbers = ctx->saved_data.find("four");
+    const bool has4 = numbers != ctx->saved_data.end();
+    const Lora l{has4 ? Four(s[4], numbers->second.toIntVector()) : Four(), s[0], has4 ? Tensor() : s[4], s[5], s[1], s[2],
+                 s[6], s[3], s[7], s[8], s[9]};
     no_tangents("lora_linear's gradient", grads[0]);
     const Tensor dy = rows(grads[0]);
     Guard guard(l.x.device());
@@ -365,31 +541,34 @@ struct LoraLinear : Function<LoraLinear> {
       if (s[i].defined() && ctx->needs_input_grad(i)) out[i] = make(s[i].sizes(), s[i].scalar_type(), l.x);
     const th_lora_linear_args d = l.args();
     size_t bytes;
-    check(th_lora_linear_backward_workspace(&d, &bytes));
+    check(has4 ? th_lora_linear4_backward_workspace(&d, &l.four.w, &bytes) : th_lora_linear_backward_workspace(&d, &bytes));
     const Work w = work(bytes, l.x);
-    check(th_lora_linear_backward(&d, ptr<float>(s[10]), ptr(dy), ld(dy), ptr(out[0]), ptr(out[1]), ptr(out[2]),
-                                  ptr<float>(out[3]), w.p, w.bytes, stream(l.x)));
+    check(has4 ? th_lora_linear4_backward(&d, &l.four.w, ptr<float>(s[10]), ptr(dy), ld(dy), ptr(out[0]), ptr(out[1]),
+                                          ptr(out[2]), ptr<float>(out[3]), w.p, w.bytes, stream(l.x))
+               : th_lora_linear_backward(&d, ptr<float>(s[10]), ptr(dy), ld(dy), ptr(out[0]), ptr(out[1]), ptr(out[2]),
+                                         ptr<float>(out[3]), w.p, w.bytes, stream(l.x)));
     variable_list result(5);
     for (int i = 0; i < 4; ++i) result[i] = out[i];
     return once(std::move(result));
   }
 };
 
-Tensor lora_linear(const Tensor& x, const Tensor& weight, const Tensor& a, const Tensor& b, const Tensor& given_experts,
-                   const OptTensor& weights, const OptTensor& scale, const OptTensor& bias, const OptTensor& order,
-                   const OptTensor& offsets) {
-  not_traced("lora_linear");
+// weight: 16 bits, undefined if four has data
+Tensor lora_any(const Tensor& x, const Tensor& weight, const Four& four, const Tensor& a, const Tensor& b,
+                const Tensor& given_experts, const OptTensor& weights, const OptTensor& scale, const OptTensor& bias,
+                const OptTensor& order, const OptTensor& offsets) {
   no_tangents("lora_linear", x, weight, a, b, weights, scale, bias);
   NEED(is_half(x), "lora_linear: x must be bf16 or f16");
   const at::ScalarType type = x.scalar_type();
-  NEED(weight.scalar_type() == type, "lora_linear: weight must have x's type");
+  const bool has4 = four.data.defined();
+  NEED(has4 ? four.w.dtype == type_of(x) : weight.scalar_type() == type, "lora_linear: weight must have x's type");
   NEED(a.scalar_type() == type, "lora_linear: lora_a must have x's type");
   NEED(b.scalar_type() == type, "lora_linear: lora_b must have x's type");
   NEED(!bias || bias->scalar_type() == type, "lora_linear: bias must have x's type");
-  NEED(x.dim() == 2 && weight.dim() == 2 && weight.size(1) == x.size(1),
+  NEED(x.dim() == 2 && (has4 ? four.w.d_in == x.size(1) : weight.dim() == 2 && weight.size(1) == x.size(1)),
        "lora_linear: x must be [T, d_in] and weight [d_out, d_in]");
   NEED(a.dim() == 3 && a.size(2) == x.size(1), "lora_linear: lora_a must be [n, rank, d_in]");
-  const int64_t n = a.size(0), d_out = weight.size(0);
+  const int64_t n = a.size(0), d_out = has4 ? four.w.d_out : weight.size(0);
   NEED(b.dim() == 3 && b.size(0) == n && b.size(1) == d_out && b.size(2) == a.size(1),
        "lora_linear: lora_b must be [n, d_out, rank]");
   const Tensor experts = experts_of("lora_linear", given_experts);
@@ -415,9 +594,10 @@ Tensor lora_linear(const Tensor& x, const Tensor& weight, const Tensor& a, const
     l.order = *order;
     l.offsets = *offsets;
   }
-  on_gpu("lora_linear", x, {weight, a, b, experts, l.gate, l.scale, l.bias, l.order, l.offsets});
+  on_gpu("lora_linear", x, {weight, four.data, a, b, experts, l.gate, l.scale, l.bias, l.order, l.offsets});
   l.x = rows(x);
-  l.weight = rows(weight);
+  if (has4) l.four = four;
+  else l.weight = rows(weight);
   l.a = rows(a);
   l.b = rows(b);
   l.experts = experts;
@@ -431,6 +611,21 @@ Tensor lora_linear(const Tensor& x, const Tensor& weight, const Tensor& a, const
   return lora_forward(l, Tensor());
 }
 
+Tensor lora_linear(const Tensor& x, const Tensor& weight, const Tensor& a, const Tensor& b, const Tensor& experts,
+                   const OptTensor& weights, const OptTensor& scale, const OptTensor& bias, const OptTensor& order,
+                   const OptTensor& offsets) {
+  not_traced("lora_linear");
+  return lora_any(x, weight, Four(), a, b, experts, weights, scale, bias, order, offsets);
+}
+Tensor lora_linear4(const Tensor& x, const Tensor& data, int64_t dtype, const std::vector<int64_t>& shape, int64_t group,
+                    bool zeros, const Tensor& a, const Tensor& b, const Tensor& experts, const OptTensor& weights,
+                    const OptTensor& scale, const OptTensor& bias, const OptTensor& order, const OptTensor& offsets) {
+  not_traced("lora_linear");
+  NEED(shape.size() == 2, "lora_linear: x must be [T, d_in] and weight [d_out, d_in]");
+  return lora_any(x, Tensor(), Four("lora_linear", data, dtype, shape, group, zeros), a, b, experts, weights, scale, bias,
+                  order, offsets);
+}
+
 }  // namespace
 
 PYBIND11_MODULE(_mixture_torch, m) {
@@ -438,4 +633,9 @@ PYBIND11_MODULE(_mixture_torch, m) {
   m.def("route", &route);
   m.def("grouped_matmul", &grouped_matmul);
   m.def("lora_linear", &lora_linear);
+  m.def("quantize4", &quantize4);
+  m.def("pack4", &pack4);
+  m.def("dequantize4", &dequantize4);
+  m.def("grouped_matmul4", &grouped_matmul4);
+  m.def("lora_linear4", &lora_linear4);
 }

@@ -10,6 +10,11 @@ training the adapters and their gate. Three operators that fit together:
   lora_linear    a frozen shared projection with the adapters of many requests,
                  or a gated mixture of them, in one pass
 
+The experts of grouped_matmul and the projection of lora_linear may have 4 bits
+a weight (`Weight4`): `quantize4` makes them of bf16 or f16 ones, `pack4` lays out
+a checkpoint's codes and scales, `dequantize4` gives the values that they stand
+for. They are frozen: the products have gradients of everything else.
+
 A slot is a (token, choice) pair, numbered token * k + choice; expert -1 means
 none. Work is queued on torch's current stream of the tensors' device, and
 nothing waits for it. All three are differentiable (see each for what in; in
@@ -39,7 +44,8 @@ except ImportError as e:
     raise ImportError(f"the binding of the mixture operators cannot be loaded ({e}): build it against this torch with "
                       "`make -C provenloop_amd/csrc mixture`") from e
 
-__all__ = ["Groups", "Routing", "group", "route", "grouped_matmul", "lora_linear"]
+__all__ = ["Groups", "Routing", "Weight4", "group", "route", "quantize4", "pack4", "dequantize4", "grouped_matmul",
+           "lora_linear"]
 
 
 class Groups(NamedTuple):
@@ -55,6 +61,63 @@ class Routing(NamedTuple):
     weights: torch.Tensor  # [T, k] float32
     experts: torch.Tensor  # [T, k] int32
     groups: Groups
+
+
+class Weight4(NamedTuple):
+    """Frozen weights of 4 bits: the values scale * (code - zero), rounded to dtype,
+    with a scale (and a zero) for each row's group_size neighbouring columns.
+
+    Made by `quantize4` and `pack4`; used in place of a weight by `grouped_matmul`
+    and `lora_linear`. data is the layout that the kernels read, half a byte a
+    weight and 2 (with zeros 3) bytes a group, and is all that a copy to another
+    device or a checkpoint has to take along: w._replace(data=w.data.to(device)).
+    """
+
+    data: torch.Tensor   # uint8
+    shape: tuple         # (d_out, d_in) or (E, d_out, d_in)
+    dtype: torch.dtype   # bf16 or f16, of the scales and values and of the products' other operands
+    group_size: int
+    zeros: bool
+
+
+# ---------------------------------------------------------------- 4-bit weights
+_TYPES = {torch.bfloat16: 1, torch.float16: 2}  # TH_BF16, TH_F16
+
+
+def quantize4(weight, group_size: int = 128, zeros: bool = False) -> Weight4:
+    """weight [d_out, d_in] or [E, d_out, d_in] (bf16 or f16) to 4 bits.
+
+    group_size: columns of a scale, a power of two from 32 on (one that reaches
+    d_in: a scale a row). Without zeros, scale = max |w| / 7 of the group and the
+    codes stand for -7 .. 7 scales; with zeros, scale = (max - min) / 15 over the
+    group's values and 0, and zero = -min / scale. Scales are rounded to the
+    weight's type first, codes to the nearest value (ties to even). A group with
+    an infinity or NaN becomes NaN. Has no gradient.
+    """
+    return Weight4(_ext.quantize4(weight, group_size, zeros), tuple(weight.shape), weight.dtype, group_size, bool(zeros))
+
+
+def pack4(codes, scales, group_size: int, zeros=None) -> Weight4:
+    """A checkpoint's 4-bit weights for the products here.
+
+    codes [d_out, d_in] or [E, d_out, d_in] uint8, a code (the low 4 bits) a byte;
+    scales [..., d_out, ceil(d_in / group_size)] bf16 or f16, which gives the
+    values' type; zeros like scales in uint8 (0 .. 15), or None: 8 everywhere.
+    Scales of infinity or NaN, for bf16 also above 2^120, make their group NaN.
+    """
+    return Weight4(_ext.pack4(codes, scales, group_size, zeros), tuple(codes.shape), scales.dtype, group_size,
+                   zeros is not None)
+
+
+def dequantize4(weight: Weight4):
+    """The values of 4-bit weights: exactly those that the products multiply with."""
+    return _ext.dequantize4(*_four(weight))
+
+
+def _four(w):
+    if w.dtype not in _TYPES:
+        raise ValueError("a 4-bit weight's dtype must be bf16 or f16")
+    return w.data, _TYPES[w.dtype], w.shape, w.group_size, w.zeros
 
 
 # ---------------------------------------------------------------- grouping and gate
@@ -84,8 +147,11 @@ def grouped_matmul(x, w, groups: Groups):
 
     x [T, d_in], or [T, k, d_in] with a row per slot; w [E, d_out, d_in];
     groups from `route` or `group` with E groups. Returns [T, k, d_out], zero
-    for slots without an expert. Differentiable in x and w.
+    for slots without an expert. Differentiable in x and w. w may be a `Weight4`
+    of shape (E, d_out, d_in), which has no gradient.
     """
+    if isinstance(w, Weight4):
+        return _ext.grouped_matmul4(x, *_four(w), *groups)
     return _ext.grouped_matmul(x, w, *groups)
 
 
@@ -94,7 +160,8 @@ def lora_linear(x, weight, lora_a, lora_b, experts, weights=None, scale=None, bi
                 groups: Optional[Groups] = None):
     """y[t] = weight @ x[t] + bias + sum_j weights[t, j] scale[e] B[e] @ (A[e] @ x[t]), e = experts[t, j].
 
-    x [T, d_in]; weight [d_out, d_in] and bias [d_out] frozen; lora_a
+    x [T, d_in]; weight [d_out, d_in] (or a `Weight4` of it) and bias [d_out]
+    frozen; lora_a
     [n, rank, d_in] and lora_b [n, d_out, rank] (PEFT's layout; rank <= 128,
     shorter adapters padded with zeros); experts [T] or [T, k] int32, outside
     [0, n) none: each request's adapter, or `route`'s choice; weights [T, k]
@@ -103,4 +170,6 @@ def lora_linear(x, weight, lora_a, lora_b, experts, weights=None, scale=None, bi
     them. Differentiable in x, lora_a, lora_b and weights.
     """
     order, offsets = (None, None) if groups is None else groups[1:3]
+    if isinstance(weight, Weight4):
+        return _ext.lora_linear4(x, *_four(weight), lora_a, lora_b, experts, weights, scale, bias, order, offsets)
     return _ext.lora_linear(x, weight, lora_a, lora_b, experts, weights, scale, bias, order, offsets)
