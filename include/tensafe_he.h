@@ -416,6 +416,32 @@ int th_route_backward(int dtype, const void* logits, int64_t ld, int64_t tokens,
                       const uint8_t* mask, int64_t mask_ld, uint32_t choices, int normalize, const float* weights,
                       const int32_t* experts, const float* dweights, void* dlogits, void* stream);
 
+/* The same gate with balanced choices. score: TH_SOFTMAX, s = exp(l - max) / sum
+ * over the allowed experts, or TH_SIGMOID, s = 1 / (1 + exp(-l)). The experts of
+ * largest s + bias are chosen (bias NULL: of largest l; an expert whose bias is
+ * -inf is not chosen). With nodes > 1 the experts lie on that many nodes, in
+ * order and equally many each, and only those of the top_nodes nodes of largest
+ * value may be chosen; a node's value is its largest s + bias, or the sum of its
+ * node_best = 2 largest. Ties go to the lowest number. The choice is that of s
+ * and s + bias in 64 bits. weights = scale s / sum of the chosen s (normalize), or
+ * scale s. bias: a float per expert, which takes part in the choice alone. */
+enum { TH_SOFTMAX = 0, TH_SIGMOID = 1 };
+typedef struct th_gate_args {
+  int dtype; /* of the logits: TH_BF16, TH_F16 or TH_F32 */
+  int score, normalize;
+  uint32_t n_experts, choices;
+  uint32_t nodes, top_nodes, node_best; /* 1, 1, 1: no nodes */
+  int64_t tokens, ld, mask_ld;
+  const void* logits;
+  const uint8_t* mask;
+  const float* bias;
+  float scale; /* positive */
+} th_gate_args;
+int th_gate(const th_gate_args* d, float* weights, int32_t* experts, int32_t* order, int32_t* offsets, void* work,
+            size_t work_bytes, void* stream);
+int th_gate_backward(const th_gate_args* d, const float* weights, const int32_t* experts, const float* dweights,
+                     void* dlogits, void* stream);
+
 /* Products grouped by expert: y[slot] = w[expert of slot] x[token of slot]
  * (x_per_slot == 0: tokens rows of x) or x[slot] (tokens x choices rows); rows
  * of slots without an expert are zero. w: experts matrices of d_out x d_in. */

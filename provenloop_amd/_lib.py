@@ -50,6 +50,13 @@ class LoraLinear(C.Structure):
                 ("experts", VP), ("gate", VP), ("scale", VP), ("order", VP), ("offsets", VP)]
 
 
+class Gate(C.Structure):
+    """th_gate_args"""
+    _fields_ = [("dtype", I32), ("score", I32), ("normalize", I32), ("n_experts", U32), ("choices", U32), ("nodes", U32),
+                ("top_nodes", U32), ("node_best", U32), ("tokens", I64), ("ld", I64), ("mask_ld", I64), ("logits", VP),
+                ("mask", VP), ("bias", VP), ("scale", C.c_float)]
+
+
 class Weight4(C.Structure):
     """th_weight4"""
     _fields_ = [("dtype", I32), ("matrices", U32), ("d_out", U32), ("d_in", U32), ("group", U32), ("zeros", I32),
@@ -119,6 +126,8 @@ _SIGS = {
     "th_group": (I32, [VP, I64, U32, U32, VP, VP, VP, SZ, VP]),
     "th_route": (I32, [I32, VP, I64, I64, U32, VP, I64, U32, I32, VP, VP, VP, VP, VP, SZ, VP]),
     "th_route_backward": (I32, [I32, VP, I64, I64, U32, VP, I64, U32, I32, VP, VP, VP, VP, VP]),
+    "th_gate": (I32, [C.POINTER(Gate), VP, VP, VP, VP, VP, SZ, VP]),
+    "th_gate_backward": (I32, [C.POINTER(Gate), VP, VP, VP, VP, VP]),
     "th_grouped_matmul": (I32, [C.POINTER(Grouped), VP, I64, VP]),
     "th_grouped_matmul_backward_workspace": (I32, [C.POINTER(Grouped), C.POINTER(SZ)]),
     "th_grouped_matmul_backward": (I32, [C.POINTER(Grouped), VP, I64, VP, VP, VP, SZ, VP]),

@@ -1,5 +1,6 @@
 // Shared declarations of the plain (unencrypted) mixture-of-adapters operators:
 //   route.hip     softmax gate with top-k, grouping of slots by expert
+//   balance.hip   gate with sigmoid scores, a bias or nodes of experts
 //   narrow.hip    matrix products of few output tiles
 //   wide.hip      large ones, of ragged groups or with low-rank adapters added
 //   grouped.hip   weight gradients of groups and of low-rank factors
@@ -52,8 +53,21 @@ struct RouteArgs {
   int32_t* order;     // T k
   int32_t* offsets;   // E + 1
   uint32_t* hist;     // chunks x (E + 1), with more than one chunk
+  // a balanced gate's (balance.hip); the plain one has softmax scores, no bias, one node and scale 1
+  const float* bias;  // null, or per expert
+  float scale = 1.0f;
+  int sigmoid = 0;
+  uint32_t nodes = 1, top_nodes = 1, node_best = 1;
 };
+// 8 logits of a token, and their mask bytes, can be loaded at once.
+inline bool whole_loads(MixType type, const RouteArgs& a) {
+  return (uintptr_t)a.logits % 16 == 0 && (a.T == 1 || a.ld * (type == MIX_F32 ? 4 : 2) % 16 == 0) &&
+         (!a.mask || ((uintptr_t)a.mask % 8 == 0 && a.mask_ld % 8 == 0));
+}
 hipError_t launch_route(MixType type, RouteArgs a, hipStream_t s);
+hipError_t launch_balanced(MixType type, const RouteArgs& a, uint32_t chunks, hipStream_t s);  // launch_route's choice
+hipError_t launch_balanced_backward(MixType type, const RouteArgs& a, const float* dweights, void* dlogits, hipStream_t s);
+hipError_t launch_place(const RouteArgs& a, uint32_t chunks, hipStream_t s);  // of the slots of several chunks
 hipError_t launch_group(RouteArgs a, hipStream_t s);
 hipError_t launch_route_backward(MixType type, const RouteArgs& a, const float* dweights, void* dlogits,
                                  hipStream_t s);

@@ -112,6 +112,66 @@ void make_copies(Stack& a, Stack& b, Stack& c, hipStream_t s) {
   HIPCHK(launch_pad(set, s));
 }
 
+// ---------------------------------------------------------------- gates
+th_gate_args plain_gate(int dtype, const void* logits, int64_t ld, int64_t tokens, uint32_t n_experts,
+                        const uint8_t* mask, int64_t mask_ld, uint32_t choices, int normalize) {
+  return th_gate_args{dtype, TH_SOFTMAX, normalize, n_experts, choices, 1, 1, 1, tokens, ld, mask_ld, logits, mask, nullptr, 1.0f};
+}
+RouteArgs check_gate(const th_gate_args& d) {
+  mix_type(d.dtype, true);
+  need_slots(d.tokens, d.n_experts, d.choices);
+  need(d.n_experts <= 512, "a gate has at most 512 experts");
+  need(d.choices <= d.n_experts, "choices must not exceed the number of experts");
+  need_rows(d.logits, d.tokens, d.ld, d.n_experts, "logits");
+  need(!d.mask || d.mask_ld == 0 || d.mask_ld >= d.n_experts, "mask: the row stride is shorter than a row");
+  need(d.score == TH_SOFTMAX || d.score == TH_SIGMOID, "score must be TH_SOFTMAX or TH_SIGMOID");
+  need(d.nodes >= 1 && d.n_experts % d.nodes == 0, "the experts must lie on the nodes equally");
+  need(d.top_nodes >= 1 && d.top_nodes <= d.nodes, "top_nodes must be in [1, nodes]");
+  need(d.choices <= d.n_experts / d.nodes * d.top_nodes, "choices must not exceed the experts of top_nodes nodes");
+  need(d.node_best == 1 || d.node_best == 2, "node_best must be 1 or 2");
+  need(d.scale > 0 && d.scale < INFINITY, "scale must be a positive number");
+  RouteArgs a{};
+  a.logits = d.logits;
+  a.mask = d.mask;
+  a.T = d.tokens;
+  a.ld = d.ld;
+  a.mask_ld = d.mask_ld;
+  a.E = d.n_experts;
+  a.k = d.choices;
+  a.normalize = d.normalize;
+  a.bias = d.bias;
+  a.scale = d.scale;
+  a.sigmoid = d.score == TH_SIGMOID;
+  // every node kept is no choice of nodes
+  a.nodes = d.top_nodes < d.nodes ? d.nodes : 1;
+  a.top_nodes = d.top_nodes < d.nodes ? d.top_nodes : 1;
+  a.node_best = d.node_best;
+  return a;
+}
+void gate_forward(const th_gate_args& d, float* weights, int32_t* experts, int32_t* order, int32_t* offsets, void* work,
+                  size_t work_bytes, void* stream) {
+  RouteArgs a = check_gate(d);
+  need(offsets && (d.tokens == 0 || (weights && experts && order)), "null output");
+  need_work(work, work_bytes, hist_words(d.tokens, d.n_experts, d.choices) * 4);
+  need_device();
+  a.weights = weights;
+  a.experts = experts;
+  a.order = order;
+  a.offsets = offsets;
+  a.hist = (uint32_t*)work;
+  HIPCHK(launch_route((MixType)d.dtype, a, (hipStream_t)stream));
+}
+void gate_backward(const th_gate_args& d, const float* weights, const int32_t* experts, const float* dweights,
+                   void* dlogits, void* stream) {
+  RouteArgs a = check_gate(d);
+  need(d.tokens == 0 || (weights && experts && dweights && dlogits), "null argument");
+  need_device();
+  if (d.tokens == 0) return;
+  a.weights = const_cast<float*>(weights);
+  a.experts = const_cast<int32_t*>(experts);
+  HIPCHK(launch_route_backward((MixType)d.dtype, a, dweights, dlogits, (hipStream_t)stream));
+}
+
 // ---------------------------------------------------------------- 4-bit weights
 th::FourLayout check_weight4(const th_weight4* w, bool data = true) {
   need(w != nullptr, "null weight");
@@ -529,30 +589,15 @@ int th_route(int dtype, const void* logits, int64_t ld, int64_t tokens, uint32_t
              int64_t mask_ld, uint32_t choices, int normalize, float* weights, int32_t* experts, int32_t* order,
              int32_t* offsets, void* work, size_t work_bytes, void* stream) {
   return guarded([&] {
-    const MixType type = mix_type(dtype, true);
-    need_slots(tokens, n_experts, choices);
-    need(n_experts <= 512, "a gate has at most 512 experts");
-    need(choices <= n_experts, "choices must not exceed the number of experts");
-    need_rows(logits, tokens, ld, n_experts, "logits");
-    need(!mask || mask_ld == 0 || mask_ld >= n_experts, "mask: the row stride is shorter than a row");
-    need(offsets && (tokens == 0 || (weights && experts && order)), "null output");
-    need_work(work, work_bytes, hist_words(tokens, n_experts, choices) * 4);
-    need_device();
-    RouteArgs a{};
-    a.logits = logits;
-    a.mask = mask;
-    a.T = tokens;
-    a.ld = ld;
-    a.mask_ld = mask_ld;
-    a.E = n_experts;
-    a.k = choices;
-    a.normalize = normalize;
-    a.weights = weights;
-    a.experts = experts;
-    a.order = order;
-    a.offsets = offsets;
-    a.hist = (uint32_t*)work;
-    HIPCHK(launch_route(type, a, (hipStream_t)stream));
+    const th_gate_args d = plain_gate(dtype, logits, ld, tokens, n_experts, mask, mask_ld, choices, normalize);
+    gate_forward(d, weights, experts, order, offsets, work, work_bytes, stream);
+  });
+}
+int th_gate(const th_gate_args* d, float* weights, int32_t* experts, int32_t* order, int32_t* offsets, void* work,
+            size_t work_bytes, void* stream) {
+  return guarded([&] {
+    need(d != nullptr, "null descriptor");
+    gate_forward(*d, weights, experts, order, offsets, work, work_bytes, stream);
   });
 }
 
@@ -560,27 +605,15 @@ int th_route_backward(int dtype, const void* logits, int64_t ld, int64_t tokens,
                       const uint8_t* mask, int64_t mask_ld, uint32_t choices, int normalize, const float* weights,
                       const int32_t* experts, const float* dweights, void* dlogits, void* stream) {
   return guarded([&] {
-    const MixType type = mix_type(dtype, true);
-    need_slots(tokens, n_experts, choices);
-    need(n_experts <= 512, "a gate has at most 512 experts");
-    need(choices <= n_experts, "choices must not exceed the number of experts");
-    need_rows(logits, tokens, ld, n_experts, "logits");
-    need(!mask || mask_ld == 0 || mask_ld >= n_experts, "mask: the row stride is shorter than a row");
-    need(tokens == 0 || (weights && experts && dweights && dlogits), "null argument");
-    need_device();
-    if (tokens == 0) return;
-    RouteArgs a{};
-    a.logits = logits;
-    a.mask = mask;
-    a.T = tokens;
-    a.ld = ld;
-    a.mask_ld = mask_ld;
-    a.E = n_experts;
-    a.k = choices;
-    a.normalize = normalize;
-    a.weights = const_cast<float*>(weights);
-    a.experts = const_cast<int32_t*>(experts);
-    HIPCHK(launch_route_backward(type, a, dweights, dlogits, (hipStream_t)stream));
+    const th_gate_args d = plain_gate(dtype, logits, ld, tokens, n_experts, mask, mask_ld, choices, normalize);
+    gate_backward(d, weights, experts, dweights, dlogits, stream);
+  });
+}
+int th_gate_backward(const th_gate_args* d, const float* weights, const int32_t* experts, const float* dweights,
+                     void* dlogits, void* stream) {
+  return guarded([&] {
+    need(d != nullptr, "null descriptor");
+    gate_backward(*d, weights, experts, dweights, dlogits, stream);
   });
 }
 

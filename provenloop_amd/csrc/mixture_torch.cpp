@@ -147,57 +147,96 @@ int64_t mask_ld(const Tensor& mask) {
   return !mask.defined() || mask.dim() == 1 || mask.stride(0) == 0 ? 0 : ld(mask);
 }
 
-variable_list route_forward(const Tensor& logits, const Tensor& mask, int64_t k, bool normalize) {
+struct Gate {
+  Tensor logits, mask, bias;
+  int64_t k;
+  bool normalize, sigmoid;
+  double scale;
+  int64_t nodes, top_nodes, node_best;
+  th_gate_args args() const {
+    th_gate_args d{};
+    d.dtype = type_of(logits);
+    d.score = sigmoid ? TH_SIGMOID : TH_SOFTMAX;
+    d.normalize = normalize;
+    d.n_experts = (uint32_t)logits.size(1);
+    d.choices = (uint32_t)k;
+    d.nodes = (uint32_t)nodes;
+    d.top_nodes = (uint32_t)top_nodes;
+    d.node_best = (uint32_t)node_best;
+    d.tokens = logits.size(0);
+    d.ld = ld(logits);
+    d.mask_ld = mask_ld(mask);
+    d.logits = ptr(logits);
+    d.mask = ptr<uint8_t>(mask);
+    d.bias = ptr<float>(bias);
+    d.scale = (float)scale;
+    return d;
+  }
+};
+
+variable_list route_forward(const Gate& g) {
+  const Tensor& logits = g.logits;
   Guard guard(logits.device());
-  const int64_t t = logits.size(0), e = logits.size(1);
+  const int64_t t = logits.size(0), e = logits.size(1), k = g.k;
   NEED(k >= 1 && k <= e, "route: choices must be in [1, number of experts]");
   size_t bytes;
   check(th_group_workspace(t, (uint32_t)e, (uint32_t)k, &bytes));
   Tensor weights = make({t, k}, at::kFloat, logits), experts = make({t, k}, at::kInt, logits);
   Tensor order = make({t * k}, at::kInt, logits), offsets = make({e + 1}, at::kInt, logits);
   const Work w = work(bytes, logits);
-  check(th_route(type_of(logits), ptr(logits), ld(logits), t, (uint32_t)e, ptr<uint8_t>(mask), mask_ld(mask),
-                 (uint32_t)k, normalize, ptr<float>(weights), ptr<int32_t>(experts), ptr<int32_t>(order),
-                 ptr<int32_t>(offsets), w.p, w.bytes, stream(logits)));
+  const th_gate_args d = g.args();
+  check(th_gate(&d, ptr<float>(weights), ptr<int32_t>(experts), ptr<int32_t>(order), ptr<int32_t>(offsets), w.p, w.bytes,
+                stream(logits)));
   return {weights, experts, order, offsets};
 }
 
 struct Route : Function<Route> {
-  static variable_list forward(AutogradContext* ctx, const Tensor& logits, const OptTensor& given_mask, int64_t k,
-                               bool normalize) {
-    const Tensor mask = given_mask ? *given_mask : Tensor();
-    variable_list out = route_forward(logits, mask, k, normalize);
-    ctx->save_for_backward({logits, mask, out[0], out[1]});
-    ctx->saved_data["normalize"] = normalize;
+  // `g` holds all of it; its other tensors have no gradients
+  static variable_list forward(AutogradContext* ctx, const Tensor& logits, Gate g) {
+    g.logits = logits;
+    variable_list out = route_forward(g);
+    ctx->save_for_backward({logits, g.mask, out[0], out[1]});
+    ctx->saved_data["normalize"] = g.normalize;
+    ctx->saved_data["sigmoid"] = g.sigmoid;
+    ctx->saved_data["scale"] = g.scale;
     ctx->mark_non_differentiable({out[1], out[2], out[3]});
     ctx->set_materialize_grads(false);
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const variable_list saved = ctx->get_saved_variables();
-    const Tensor &logits = saved[0], &mask = saved[1];
-    if (!grads[0].defined()) return variable_list(4);
+    const Tensor& logits = saved[0];
+    if (!grads[0].defined()) return variable_list(2);
     no_tangents("route's gradient", grads[0]);
     const Tensor dweights = grads[0].contiguous();
     Guard guard(logits.device());
     Tensor dlogits = make(logits.sizes(), logits.scalar_type(), logits);
-    check(th_route_backward(type_of(logits), ptr(logits), ld(logits), logits.size(0), (uint32_t)logits.size(1),
-                            ptr<uint8_t>(mask), mask_ld(mask), (uint32_t)saved[2].size(1),
-                            ctx->saved_data["normalize"].toBool(), ptr<float>(saved[2]), ptr<int32_t>(saved[3]),
-                            ptr<float>(dweights), ptr(dlogits), stream(logits)));
-    return once({dlogits, Tensor(), Tensor(), Tensor()});
+    // which experts were chosen is given, so the bias and nodes have no part in it
+    const Gate g{logits, saved[1], Tensor(), saved[2].size(1), ctx->saved_data["normalize"].toBool(),
+                 ctx->saved_data["sigmoid"].toBool(), ctx->saved_data["scale"].toDouble(), 1, 1, 1};
+    const th_gate_args d = g.args();
+    check(th_gate_backward(&d, ptr<float>(saved[2]), ptr<int32_t>(saved[3]), ptr<float>(dweights), ptr(dlogits),
+                           stream(logits)));
+    return once({dlogits, Tensor()});
   }
 };
 
 std::tuple<Tensor, Tensor, Tensor, Tensor> route(const Tensor& given, int64_t k, const OptTensor& given_mask,
-                                                 bool normalize) {
+                                                 bool normalize, const std::string& score, const OptTensor& given_bias,
+                                                 double scale, int64_t nodes, int64_t top_nodes, int64_t node_best) {
   not_traced("route");
-  no_tangents("route", given);
+  no_tangents("route", given, given_bias);
   NEED(type_of(given) != 0, "route: logits must be bf16, f16 or f32");
   NEED(given.dim() == 2, "route: logits must be [T, E]");
-  Tensor mask = given_mask ? *given_mask : Tensor();
-  on_gpu("route", given, {mask});
+  NEED(score == "softmax" || score == "sigmoid", "route: score must be 'softmax' or 'sigmoid'");
+  Tensor mask = given_mask ? *given_mask : Tensor(), bias = given_bias ? *given_bias : Tensor();
   const int64_t t = given.size(0), e = given.size(1);
+  if (bias.defined()) {
+    NEED(bias.scalar_type() == at::kFloat && bias.dim() == 1 && bias.size(0) == e, "route: bias must be float32 [E]");
+    NEED(!bias.requires_grad() || !at::GradMode::is_enabled(), "route: bias takes part in the choice alone and has no gradient");
+  }
+  NEED(nodes >= 1 && nodes <= e && top_nodes >= 1 && top_nodes <= nodes, "route: top_nodes must be in [1, nodes], nodes in [1, number of experts]");
+  on_gpu("route", given, {mask, bias});
   if (mask.defined()) {
     NEED(mask.scalar_type() == at::kBool, "route: mask must be bool");
     NEED((mask.dim() == 2 && mask.size(0) == t && mask.size(1) == e) || (mask.dim() == 1 && mask.size(0) == e),
@@ -206,10 +245,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> route(const Tensor& given, int64_t k,
         (mask.dim() == 2 && t > 1 && mask.stride(0) > 0 && mask.stride(0) < e))
       mask = mask.contiguous();
   }
+  if (bias.defined()) bias = bias.contiguous();
   const Tensor logits = rows(given);
-  const variable_list out = logits.requires_grad() && at::GradMode::is_enabled()
-                                ? Route::apply(logits, optional(mask), k, normalize)
-                                : route_forward(logits, mask, k, normalize);
+  const Gate g{logits, mask, bias, k, normalize, score == "sigmoid", scale, nodes, top_nodes, node_best};
+  const variable_list out = logits.requires_grad() && at::GradMode::is_enabled() ? Route::apply(logits, g) : route_forward(g);
   return {out[0], out[1], out[2], out[3]};
 }
 

@@ -16,13 +16,11 @@
 // gate and 10 us for the slots' places. The gate moves 19 MB, 4 us at a copy's
 // rate; about 450 instructions a token's lane are some 6 us, and the rest is loads
 // that a workgroup's rounds of tokens wait for one after the other.
-#include "mixture.h"
+#include "route_device.h"
+
+using namespace mix;
 
 namespace {
-
-constexpr int THREADS = 1024, WAVES = THREADS / 64;
-constexpr uint32_t group_lds(uint32_t E, bool chunks = false) { return ((chunks ? 2 : 1) * WAVES + 1) * (E + 1) * 4; }
-constexpr uint32_t MOST = group_lds(th::MIX_MAX_EXPERTS), MOST_CHUNKS = group_lds(th::MIX_MAX_EXPERTS, true);
 
 // A logit as a whole number that orders candidates: its bits made to rise with
 // its value (NaN above +inf, as a comparison sort of the framework's users puts
@@ -58,101 +56,6 @@ struct Ranked<float> {
     return key == 0xffffffffu ? NAN : __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
   }
 };
-
-// The same value from a lane on the other side, of pairs, quads, 8, 16, 32 or
-// 64 lanes whose halves each agree on theirs.
-template <int D>
-__device__ inline uint32_t across(uint32_t v) {
-  if constexpr (D == 1) return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xf, 0xf, true);        // quad_perm 1 0 3 2
-  else if constexpr (D == 2) return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xf, 0xf, true);   // quad_perm 2 3 0 1
-  else if constexpr (D == 4) return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xf, 0xf, true);  // row_half_mirror
-  else if constexpr (D == 8) return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xf, 0xf, true);  // row_mirror
-  else return __shfl_xor(v, D);
-}
-template <int D>
-__device__ inline uint64_t across(uint64_t v) {
-  return (uint64_t)across<D>((uint32_t)(v >> 32)) << 32 | across<D>((uint32_t)v);
-}
-template <int G, class C, int D = 1>
-__device__ inline C group_max(C v) {
-  if constexpr (D < G) {
-    const C o = across<D>(v);
-    return group_max<G, C, 2 * D>(o > v ? o : v);
-  } else {
-    return v;
-  }
-}
-template <int G, int D = 1>
-__device__ inline float group_sum(float v) {
-  if constexpr (D < G) return group_sum<G, 2 * D>(v + __uint_as_float(across<D>(__float_as_uint(v))));
-  else return v;
-}
-
-template <class T>
-__device__ inline bool allowed_at(const RouteArgs& a, int64_t t, uint32_t e, float& l) {
-  l = to_float(((const T*)a.logits)[t * a.ld + e]);
-  const bool ok = !(l == -INFINITY) && (!a.mask || a.mask[t * a.mask_ld + e]);
-  return ok;
-}
-
-// Exclusive prefix of n words in LDS by the first wavefront.
-__device__ void prefix_words(uint32_t* v, uint32_t n) {
-  if (threadIdx.x < 64) {
-    uint32_t run = 0;
-    for (uint32_t at = 0; at < n; at += 64) {
-      const uint32_t i = at + threadIdx.x;
-      const uint32_t own = i < n ? v[i] : 0;
-      uint32_t sum = own;
-      for (int d = 1; d < 64; d <<= 1) {
-        const uint32_t up = __shfl_up(sum, d);
-        if ((int)threadIdx.x >= d) sum += up;
-      }
-      if (i < n) v[i] = run + sum - own;
-      run += __shfl(sum, 63);
-    }
-  }
-}
-
-// Positions of the slots [s0, s1) of one workgroup. `base` (LDS, E + 1 words)
-// holds where the workgroup's first slot of each expert goes; `counts` (LDS,
-// WAVES x (E + 1)). A wavefront ranks its 64 slots by matching the expert's
-// bits across its lanes; the wavefronts' counts are summed per expert.
-__device__ void place_slots(const int32_t* experts, int64_t s0, int64_t s1, uint32_t E, int32_t* order, uint32_t* base,
-                            uint32_t* counts) {
-  const uint32_t keys = E + 1, wave = threadIdx.x >> 6, lane = threadIdx.x & 63;
-  const int bits = 32 - __clz(E);
-  for (int64_t at = s0; at < s1; at += THREADS) {
-    for (uint32_t i = threadIdx.x; i < WAVES * keys; i += THREADS) counts[i] = 0;
-    __syncthreads();
-    const int64_t s = at + threadIdx.x;
-    const bool in = s < s1;
-    uint32_t key = E;
-    if (in) {
-      const uint32_t e = (uint32_t)experts[s];
-      key = e < E ? e : E;
-    }
-    uint64_t same = __ballot(in);
-    for (int b = 0; b < bits; ++b) {
-      const uint64_t set = __ballot((key >> b) & 1);
-      same &= (key >> b) & 1 ? set : ~set;
-    }
-    const uint32_t rank = __popcll(same & ((1ull << lane) - 1));
-    if (in && rank == 0) counts[wave * keys + key] = __popcll(same);
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < keys; i += THREADS) {
-      uint32_t run = base[i];
-      for (int w = 0; w < WAVES; ++w) {
-        const uint32_t c = counts[w * keys + i];
-        counts[w * keys + i] = run;
-        run += c;
-      }
-      base[i] = run;
-    }
-    __syncthreads();
-    if (in) order[counts[wave * keys + key] + rank] = (int32_t)s;
-    __syncthreads();
-  }
-}
 
 // base = where this chunk's slots start, per expert, from every chunk's counts
 // hist[chunk][key]; offsets written by chunk 0. A wavefront adds up every 16th
@@ -288,17 +191,7 @@ __global__ void __launch_bounds__(THREADS) route_kernel(RouteArgs a) {
   __syncthreads();
   const int64_t t0 = (int64_t)blockIdx.x * a.chunk, t1 = min(t0 + (int64_t)a.chunk, a.T);
   choose<T, G>(a, t0, t1, base);
-  __threadfence_block();
-  __syncthreads();
-  if (gridDim.x > 1) {
-    for (uint32_t i = threadIdx.x; i <= a.E; i += THREADS) a.hist[(size_t)blockIdx.x * (a.E + 1) + i] = base[i];
-    return;
-  }
-  prefix_words(base, a.E + 1);
-  __syncthreads();
-  for (uint32_t i = threadIdx.x; i <= a.E; i += THREADS) a.offsets[i] = (int32_t)base[i];
-  __syncthreads();
-  place_slots(a.experts, 0, a.T * a.k, a.E, a.order, base, counts);
+  end_chunk(a, base, counts);
 }
 
 // Counts of one chunk of given slots; a single chunk also places them.
@@ -382,34 +275,37 @@ hipError_t route_typed(const RouteArgs& a, uint32_t chunks, uint32_t lds, hipStr
   return launch<route_kernel<T, 64>>(chunks, THREADS, lds, s, a);
 }
 
-hipError_t place(const RouteArgs& a, uint32_t chunks, hipStream_t s) {
+}  // namespace
+
+hipError_t launch_place(const RouteArgs& a, uint32_t chunks, hipStream_t s) {
   if (chunks == 1) return hipSuccess;
   return launch<place_kernel, MOST_CHUNKS>(chunks, THREADS, group_lds(a.E, true), s, a);
 }
 
-}  // namespace
-
 hipError_t launch_route(MixType type, RouteArgs a, hipStream_t s) {
   const uint32_t chunks = (uint32_t)th::group_chunks(a.T, a.k);
   a.chunk = (uint32_t)th::group_chunk_tokens(a.T, a.k);
-  const uint32_t size = type == MIX_F32 ? 4 : 2;
-  a.vector = (uintptr_t)a.logits % 16 == 0 && (a.T == 1 || a.ld * size % 16 == 0) &&
-             (!a.mask || ((uintptr_t)a.mask % 8 == 0 && a.mask_ld % 8 == 0));
+  a.vector = whole_loads(type, a);
+  if (a.sigmoid || a.bias || a.nodes > 1 || a.scale != 1.0f) {
+    const hipError_t e = launch_balanced(type, a, chunks, s);
+    return e != hipSuccess ? e : launch_place(a, chunks, s);
+  }
   hipError_t e = type == MIX_BF16  ? route_typed<bf16_t>(a, chunks, group_lds(a.E), s)
                  : type == MIX_F16 ? route_typed<f16_t>(a, chunks, group_lds(a.E), s)
                                    : route_typed<float>(a, chunks, group_lds(a.E), s);
-  return e != hipSuccess ? e : place(a, chunks, s);
+  return e != hipSuccess ? e : launch_place(a, chunks, s);
 }
 
 hipError_t launch_group(RouteArgs a, hipStream_t s) {
   const uint32_t chunks = (uint32_t)th::group_chunks(a.T, a.k);
   a.chunk = (uint32_t)th::group_chunk_tokens(a.T, a.k);
   const hipError_t e = launch<count_kernel, MOST>(chunks, THREADS, group_lds(a.E), s, a);
-  return e != hipSuccess ? e : place(a, chunks, s);
+  return e != hipSuccess ? e : launch_place(a, chunks, s);
 }
 
 hipError_t launch_route_backward(MixType type, const RouteArgs& a, const float* dweights, void* dlogits,
                                  hipStream_t s) {
+  if (a.sigmoid || a.scale != 1.0f) return launch_balanced_backward(type, a, dweights, dlogits, s);
   const uint32_t blocks = th::loop_blocks(th::ceil_div(a.T, 4));
   if (type == MIX_BF16) return launch<route_backward_kernel<bf16_t>>(blocks, 256, 0, s, a, dweights, (bf16_t*)dlogits);
   if (type == MIX_F16) return launch<route_backward_kernel<f16_t>>(blocks, 256, 0, s, a, dweights, (f16_t*)dlogits);

@@ -4,8 +4,9 @@ The adapters that `zero_moai` serves under encryption, in the clear: for
 sessions that did not ask for encryption, for prefills and batches, and for
 training the adapters and their gate. Three operators that fit together:
 
-  route          softmax gate with top-k per token (`zero_moai.softmax_gate`
-                 for a whole batch, on the GPU), slots grouped by expert
+  route          gate with top-k per token (`zero_moai.softmax_gate` for a whole
+                 batch, on the GPU; also with sigmoid scores, a bias for balance
+                 and experts on nodes), slots grouped by expert
   grouped_matmul matrix products grouped by expert, with ragged group sizes
   lora_linear    a frozen shared projection with the adapters of many requests,
                  or a gated mixture of them, in one pass
@@ -127,8 +128,9 @@ def group(experts, n_groups: int) -> Groups:
     return Groups(*_ext.group(experts, n_groups), n_groups)
 
 
-def route(logits, k: int, mask=None, normalize: bool = True) -> Routing:
-    """Softmax gate with top-k.
+def route(logits, k: int, mask=None, normalize: bool = True, *, score: str = "softmax", bias=None, scale: float = 1.0,
+          nodes: int = 1, top_nodes: int = 1, node_best: int = 1) -> Routing:
+    """Gate with top-k, by softmax or sigmoid scores, balanced by a bias and by nodes.
 
     logits [T, E] (bf16, f16 or f32; E <= 512); mask [T, E] or [E] bool, False
     where a token must not use an expert (a logit of -inf says the same). The k
@@ -136,8 +138,18 @@ def route(logits, k: int, mask=None, normalize: bool = True) -> Routing:
     are exp(l - max) over their sum (normalize=True) or over the sum of all
     allowed experts. Tokens with fewer than k allowed experts have -1 and
     weight 0 there. Differentiable in the logits.
+
+    score: "softmax" as above, or "sigmoid", s = 1 / (1 + exp(-l)) and weights s,
+    or s over the sum of the chosen ones (normalize=True). scale: a positive number
+    that multiplies the weights. bias [E] float32, which takes part in the choice
+    alone: the k largest s + bias are chosen (an expert whose bias is -inf never
+    is). Balancing raises it for experts with few slots and lowers it for those
+    with many, as groups.offsets counts them. nodes: the experts lie in order on
+    that many nodes, E / nodes each, and a token uses those of top_nodes nodes
+    alone: of the nodes whose largest s + bias, or sum of the two largest
+    (node_best=2), is largest. What is chosen is decided in 64 bits.
     """
-    weights, experts, order, offsets = _ext.route(logits, k, mask, normalize)
+    weights, experts, order, offsets = _ext.route(logits, k, mask, normalize, score, bias, scale, nodes, top_nodes, node_best)
     return Routing(weights, experts, Groups(experts, order, offsets, logits.shape[1]))
 
 
