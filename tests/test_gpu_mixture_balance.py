@@ -109,6 +109,41 @@ def test_near_ties(score, e, nodes, top, best):
         assert np.array_equal(got[clear], ids[clear])
 
 
+@pytest.mark.parametrize("per", [2, 8, 12, 16, 64])
+def test_nodes_that_only_64_bits_tell_apart(per):
+    """Two nodes whose sums are equal in float, of experts that differ clearly: one is kept, the larger."""
+    logits = torch.full((9, 4 * per), -6.0, device="cuda")
+    logits[:, 0::per], logits[:, 1::per] = 2.0, 1.0
+    for first, second in ((1, 2), (2, 1), (3, 0)):
+        for more in (2.0 ** -25, -2.0 ** -26, 0.0):  # float's neighbours of 1/4
+            bias = torch.full((4 * per,), -0.5, device="cuda")
+            bias[first * per], bias[first * per + 1] = 0.25, 0.0
+            bias[second * per], bias[second * per + 1] = 0.0, 0.25 + more
+            for score, top in (("sigmoid", 1), ("softmax", 1)):
+                opts = dict(score=score, bias=bias, nodes=4, top_nodes=top, node_best=2)
+                got = mixture.route(logits, 2, **opts).experts.cpu().numpy()
+                if more:
+                    assert np.array_equal(got, oracle(logits, 2, **opts)[1])
+                else:  # (s + 1/4) + t and s + (t + 1/4): one number, and 64 bits round each to either side of it
+                    assert (got == [first * per, first * per + 1]).all() or (got == [second * per + 1, second * per]).all()
+
+
+def test_many_tokens_whose_nodes_come_near():
+    """A prefill's tokens, a few of which have nodes nearer than float tells apart."""
+    for seed, (e, nodes, top) in enumerate([(256, 8, 4), (256, 8, 4), (96, 8, 3), (512, 16, 4)] * 6):
+        g = gen(200 + seed)
+        logits = normal(g, 65536, e, dtype=torch.bfloat16, std=1.5)
+        bias = (torch.randn(e, generator=g, device="cuda") * 20).round() * 0.001
+        opts = dict(score="sigmoid", bias=bias, nodes=nodes, top_nodes=top, node_best=2)
+        r = mixture.route(logits, 8, **opts)
+        # the definition in 64 bits, on the GPU: the host's takes long
+        c = 1 / (1 + torch.exp(-logits.double())) + bias.double()
+        value = torch.sort(c.view(-1, nodes, e // nodes), dim=2, descending=True).values[:, :, :2].sum(2)
+        kept = torch.zeros_like(value, dtype=torch.bool).scatter_(1, torch.sort(value, dim=1, descending=True, stable=True).indices[:, :top], True)
+        c = c.masked_fill(~kept.repeat_interleave(e // nodes, 1), -float("inf"))
+        assert torch.equal(r.experts, torch.sort(c, dim=1, descending=True, stable=True).indices[:, :8].to(torch.int32))
+
+
 def test_extremes_and_bad_values():
     inf, nan = float("inf"), float("nan")
     z = torch.zeros(4, device="cuda")
