@@ -437,6 +437,7 @@ typedef struct th_gate_args {
   const float* bias;
   float scale; /* positive */
 } th_gate_args;
+int th_gate_workspace(const th_gate_args* d, size_t* bytes);
 int th_gate(const th_gate_args* d, float* weights, int32_t* experts, int32_t* order, int32_t* offsets, void* work,
             size_t work_bytes, void* stream);
 int th_gate_backward(const th_gate_args* d, const float* weights, const int32_t* experts, const float* dweights,

@@ -126,6 +126,7 @@ _SIGS = {
     "th_group": (I32, [VP, I64, U32, U32, VP, VP, VP, SZ, VP]),
     "th_route": (I32, [I32, VP, I64, I64, U32, VP, I64, U32, I32, VP, VP, VP, VP, VP, SZ, VP]),
     "th_route_backward": (I32, [I32, VP, I64, I64, U32, VP, I64, U32, I32, VP, VP, VP, VP, VP]),
+    "th_gate_workspace": (I32, [C.POINTER(Gate), C.POINTER(SZ)]),
     "th_gate": (I32, [C.POINTER(Gate), VP, VP, VP, VP, VP, SZ, VP]),
     "th_gate_backward": (I32, [C.POINTER(Gate), VP, VP, VP, VP, VP]),
     "th_grouped_matmul": (I32, [C.POINTER(Grouped), VP, I64, VP]),

@@ -12,22 +12,27 @@
 //
 // A choice by scores is a choice between numbers that were rounded. It is defined
 // by s and c in 64 bits. Those cost a token of 256 experts several times the rest
-// of its work, so the numbers are first made in float, and only a token two of
-// whose decisive numbers are nearer than float's errors can tell apart goes
-// through them again in double.
+// of its work, so its lanes first make the numbers in float, and only a token two
+// of whose decisive numbers are nearer than float's errors can tell apart is
+// decided again in double, by a whole wavefront, once the workgroup's others are
+// done: next to them double's registers would cost the loop that all go through.
 //
-// The lanes of a token, its slots' places and what bounds both are route.hip's.
+// Up to 16 lanes take a token, several chunks of 8 experts a lane. Chunks are put in
+// order in a lane's registers and merged there and then across the lanes, 8 numbers
+// with 8: the fewer lanes a token has, the fewer steps go across lanes, which cost
+// most. 65536 tokens of 256 experts on 8 nodes, 8 chosen: 47 us where no two numbers
+// come near, with 16 for the places (32 lanes a token and rounds that take the
+// largest of the lanes' first: 87), 67 where a few tokens are decided again: one of
+// these takes some 12 us, waiting for one step after the other, and nearly every
+// workgroup has one. A copy's rate would be 8 us; about 1300 instructions a
+// wavefront's 8 tokens are 14. One token takes 9.5 us: the chain of its steps.
 #include "route_device.h"
 
 using namespace mix;
 
 namespace {
 
-// A candidate as a number that orders like (value, lowest expert first), 0 for
-// none: the value's bits made to rise with it, NaN above +inf, over the expert's
-// number from the top.
-template <class V>
-struct Candidate;
+// A number's bits made to rise with its value, NaN above +inf, -0 with +0; never 0.
 __device__ inline uint32_t rising(float v) {
   const uint32_t b = __float_as_uint(v + 0.0f);
   return v != v ? 0xffffffffu : b & 0x80000000u ? ~b : b | 0x80000000u;
@@ -36,157 +41,17 @@ __device__ inline uint64_t rising(double v) {
   const uint64_t b = (uint64_t)__double_as_longlong(v + 0.0);
   return v != v ? ~0ull : b >> 63 ? ~b : b | 1ull << 63;
 }
-template <>
-struct Candidate<float> {
-  uint64_t v;
-  __device__ inline Candidate() : v(0) {}
-  __device__ inline Candidate(float c, uint32_t e) : v((uint64_t)rising(c) << 32 | (0xffffffffu - e)) {}
-  __device__ inline bool any() const { return v != 0; }
-  __device__ inline bool operator>(const Candidate& o) const { return v > o.v; }
-  __device__ inline bool operator==(const Candidate& o) const { return v == o.v; }
-  __device__ inline uint32_t expert() const { return 0xffffffffu - (uint32_t)v; }
-};
-template <>
-struct Candidate<double> {
-  uint64_t v;
-  uint32_t low;
-  __device__ inline Candidate() : v(0), low(0) {}
-  __device__ inline Candidate(double c, uint32_t e) : v(rising(c)), low(0xffffffffu - e) {}
-  __device__ inline bool any() const { return v != 0; }
-  __device__ inline bool operator>(const Candidate& o) const { return v > o.v || (v == o.v && low > o.low); }
-  __device__ inline bool operator==(const Candidate& o) const { return v == o.v && low == o.low; }
-  __device__ inline uint32_t expert() const { return 0xffffffffu - low; }
-};
-template <int D>
-__device__ inline Candidate<float> across(const Candidate<float>& c) {
-  Candidate<float> o;
-  o.v = mix::across<D>(c.v);
-  return o;
-}
-template <int D>
-__device__ inline Candidate<double> across(const Candidate<double>& c) {
-  Candidate<double> o;
-  o.v = mix::across<D>(c.v);
-  o.low = mix::across<D>(c.low);
-  return o;
-}
-template <int G, class V, int D = 1>
-__device__ inline Candidate<V> largest(const Candidate<V>& c) {
-  if constexpr (D < G) {
-    const Candidate<V> o = across<D>(c);
-    return largest<G, V, 2 * D>(o > c ? o : c);
-  } else {
-    return c;
-  }
-}
-// Over a token's lanes; NaN if any is.
-template <int G, int D = 1>
-__device__ inline float most(float v) {
-  if constexpr (D < G) {
-    const float o = __uint_as_float(mix::across<D>(__float_as_uint(v)));
-    return most<G, 2 * D>(o != o || v != v ? NAN : fmaxf(v, o));
-  } else {
-    return v;
-  }
-}
-template <int G, int D = 1>
-__device__ inline double sum(double v) {
-  if constexpr (D < G) return sum<G, 2 * D>(v + __longlong_as_double(mix::across<D>((uint64_t)__double_as_longlong(v))));
-  else return v;
-}
-template <int G>
-__device__ inline float sum(float v) {
-  return group_sum<G>(v);
+__device__ inline float value_of(uint32_t key) {
+  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
-// A token's lanes see what each has laid in LDS; they are in one wavefront, whose
-// LDS accesses are answered in order.
-__device__ inline void lanes_agree() {
-  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
-  __builtin_amdgcn_wave_barrier();
-  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
-}
-
-
-constexpr int keep(int G) { return G >= 32 ? 1 : G >= 4 ? 32 / G : 8; }  // choices that one lane can have to keep
-
-// A token's logits, 8 a lane, and which of them are allowed.
-struct Row {
-  float l[8];
-  uint32_t allowed;  // a bit each
-  float big;         // the largest allowed; NaN if one is
-};
-
-// Of a token's experts with numbers c those on the nodes that it may use. own: LDS
-// for the numbers.
-struct Kept {
-  uint32_t allowed;
-  float clear;  // by how much the least of the kept nodes is above the best of the others
-};
-template <int G, class V>
-__device__ inline Kept keep_nodes(const RouteArgs& a, uint32_t g, const V (&c)[8], uint32_t allowed, V* own) {
-  // a lane takes every G-th node: its value in place of its first expert's c,
-  // then whether it is kept
-  const uint32_t per = a.E / a.nodes, to_node = (1u << 20) / per + 1;  // e * to_node >> 20 = e / per, for e < 512
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (g * 8 + i < a.E) own[g * 8 + i] = allowed >> i & 1 ? c[i] : (V)-INFINITY;
-  lanes_agree();
-  for (uint32_t n = g; n < a.nodes; n += G) {
-    V one = -INFINITY, two = -INFINITY;
-    bool nan = false;
-    for (uint32_t i = 0; i < per; ++i) {
-      const V v = own[n * per + i];
-      nan |= v != v;
-      if (v > one) {
-        two = one;
-        one = v;
-      } else if (v > two) {
-        two = v;
-      }
-    }
-    if (a.node_best == 2 && two > (V)-INFINITY) one += two;
-    own[n * per] = nan ? (V)NAN : one;
-  }
-  lanes_agree();
-  uint32_t kept = 0, at = 0;
-  float least = INFINITY, above = -INFINITY;  // of the kept, of the others
-  for (uint32_t n = g; n < a.nodes; n += G, ++at) {
-    const V mine = own[n * per];
-    const Candidate<V> me(mine, n);
-    uint32_t before = 0;
-    for (uint32_t m = 0; m < a.nodes; ++m) before += Candidate<V>(own[m * per], m) > me;
-    if (before < a.top_nodes) {
-      kept |= 1u << at;
-      least = fminf(least, (float)mine);
-    } else {
-      above = fmaxf(above, (float)mine);
-    }
-  }
-  lanes_agree();
-  at = 0;
-  for (uint32_t n = g; n < a.nodes; n += G, ++at) own[n * per] = kept >> at & 1 ? (V)1 : (V)0;
-  lanes_agree();
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const uint32_t ex = g * 8 + i;
-    if (ex < a.E && own[(ex * to_node >> 20) * per] == (V)0) allowed &= ~(1u << i);
-  }
-  lanes_agree();  // before the next numbers are laid there
-  if constexpr (std::is_same<V, float>::value) {
-    above = most<G>(above);
-    return Kept{allowed, above > -INFINITY ? -most<G>(-least) - above : INFINITY};
-  }
-  return Kept{allowed, 0};
-}
-
-// The largest key of a token's lanes.
+// The largest of G lanes' words.
 template <int G>
 __device__ inline uint32_t most_key(uint32_t v) {
-  if constexpr (G > 1) v = max(v, mix::across<1>(v));
-  if constexpr (G > 2) v = max(v, mix::across<2>(v));
-  if constexpr (G > 4) v = max(v, mix::across<4>(v));
-  if constexpr (G > 8) v = max(v, mix::across<8>(v));
+  if constexpr (G > 1) v = max(v, across<1>(v));
+  if constexpr (G > 2) v = max(v, across<2>(v));
+  if constexpr (G > 4) v = max(v, across<4>(v));
+  if constexpr (G > 8) v = max(v, across<8>(v));
   if constexpr (G > 16) {
     const auto o = __builtin_amdgcn_permlane16_swap(v, v, false, false);
     v = max(o[0], o[1]);
@@ -197,306 +62,562 @@ __device__ inline uint32_t most_key(uint32_t v) {
   }
   return v;
 }
-__device__ inline float key_value(uint32_t key) {
-  return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
-}
-
-// Chooses by scores in float, or returns false where those are too near to tell.
-// A candidate is one word: its c made to rise, the lowest 3 bits its place among
-// the lane's 8, so that the lane's candidates are put in order by 38 maxima and
-// minima; equal c need no order of their own, since they are too near. The rounds
-// then take the largest of the lanes' first.
+// The largest of G lanes' numbers; NaN if any is.
 template <int G>
-__device__ inline bool pick_near(const RouteArgs& a, const Row& r, uint32_t g, float* own, int32_t (&e)[keep(G)]) {
-  constexpr float LOG2E = 1.44269504f;
-  float c[8];
-  // exp through exp2 of a rounded product: off by |l| 2^-24 of itself, which is
-  // below 2^-24 of the score's range since x exp(-x) < 1
-  if (a.sigmoid) {
+__device__ inline float most(float v) {
+  return value_of(most_key<G>(rising(v)));
+}
+
+// A wavefront's lanes see what each has laid in LDS, whose accesses are answered
+// in order.
+__device__ inline void lanes_agree() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
+}
+
+// ---------------------------------------------------------------- experts on lanes
+// Experts in chunks of 8, a node in chunks of its own (the last one's rest is
+// empty). Chunk i of a token's G lanes is the (i / G)-th of lane i % G.
+struct Chunks {
+  uint32_t per, chunks_per;  // experts and chunks of a node
+};
+__host__ __device__ inline Chunks chunks_of(uint32_t E, uint32_t nodes) {
+  const uint32_t per = E / nodes;
+  return Chunks{per, (per + 7) / 8};
+}
+
+// What decides: the scores, with a bias or as sums of two, or else the logits.
+__device__ inline bool by_scores(const RouteArgs& a) { return a.bias || (a.nodes > 1 && a.node_best == 2); }
+
+// LDS floats of a lane: two of each chunk, one of each node.
+constexpr uint32_t lane_space(int C) { return 3 * C; }
+
+// ---------------------------------------------------------------- 8 numbers in falling order
+// A candidate is a double: its c, which float's 24 bits leave 29 bits of, and below
+// these the expert's number, so that of equal c the lowest expert's is the larger.
+// -inf: none.
+__device__ inline double candidate(float c, uint32_t e) {
+  const uint64_t b = (uint64_t)__double_as_longlong((double)c);
+  const uint32_t low = c == -INFINITY ? 0 : c < 0 ? e : 511 - e;
+  return __longlong_as_double((long long)(b | low));
+}
+__device__ inline int32_t expert_of(double v) {
+  const uint32_t low = (uint32_t)(uint64_t)__double_as_longlong(v) & 511;
+  return v == -INFINITY ? -1 : (int32_t)(v < 0 ? low : 511 - low);
+}
+template <int I, int J>
+__device__ inline void order(double (&s)[8]) {
+  const double hi = fmax(s[I], s[J]), lo = fmin(s[I], s[J]);
+  s[I] = hi;
+  s[J] = lo;
+}
+__device__ inline void sort8(double (&s)[8]) {  // Batcher's odd-even merge
+  order<0, 1>(s), order<2, 3>(s), order<4, 5>(s), order<6, 7>(s), order<0, 2>(s), order<1, 3>(s), order<4, 6>(s);
+  order<5, 7>(s), order<1, 2>(s), order<5, 6>(s), order<0, 4>(s), order<1, 5>(s), order<2, 6>(s), order<3, 7>(s);
+  order<2, 4>(s), order<3, 5>(s), order<1, 2>(s), order<3, 4>(s), order<5, 6>(s);
+}
+// top = the 8 largest of both; rest: the largest of what was left out, if asked for.
+__device__ inline void merge8(double (&top)[8], const double (&s)[8], double& rest, bool ask) {
+  if (ask) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-LOG2E * r.l[i]));
+    for (int i = 0; i < 8; ++i) rest = fmax(rest, fmin(top[i], s[7 - i]));
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) top[i] = fmax(top[i], s[7 - i]);  // falls and rises: three steps put it in order
+  order<0, 4>(top), order<1, 5>(top), order<2, 6>(top), order<3, 7>(top);
+  order<0, 2>(top), order<1, 3>(top), order<4, 6>(top), order<5, 7>(top);
+  order<0, 1>(top), order<2, 3>(top), order<4, 5>(top), order<6, 7>(top);
+}
+// The 8 largest of G lanes' lists, in all of them.
+template <int G>
+__device__ inline void merge_lanes(double (&top)[8], double& rest, bool ask) {
+#pragma unroll 1
+  for (int d = 1; d < G; d *= 2) {
+    double s[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s[i] = __shfl_xor(top[i], d);
+    if (ask) rest = fmax(rest, __shfl_xor(rest, d));
+    merge8(top, s, rest, ask);
+  }
+}
+
+// ---------------------------------------------------------------- in float
+// c becomes -inf on the nodes that are not kept. Returns by how much the least of
+// the kept is above the best of the others. own: the token's LDS.
+template <int G, int C>
+__device__ inline float keep_nodes(const RouteArgs& a, uint32_t chunks_per, uint32_t g, float (&c)[8 * C], float* own) {
+  float* values = own + 2 * G * C;
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    float one = -INFINITY, two = -INFINITY;
+#pragma unroll
+    for (int r = 0; r < 8; ++r) {
+      two = fmaxf(two, fminf(one, c[8 * i + r]));
+      one = fmaxf(one, c[8 * i + r]);
+    }
+    *(float2*)&own[2 * (i * G + g)] = float2{one, two};
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  lanes_agree();
+#pragma unroll 1
+  for (uint32_t n = g; n < a.nodes; n += G) {
+    float one = -INFINITY, two = -INFINITY;
+    for (uint32_t q = n * chunks_per; q < (n + 1) * chunks_per; ++q) {
+      const float2 v = *(const float2*)&own[2 * q];
+      two = fmaxf(fminf(one, v.x), fmaxf(two, v.y));
+      one = fmaxf(one, v.x);
+    }
+    values[n] = a.node_best == 2 && two > -INFINITY ? one + two : one;
+  }
+  lanes_agree();
+  uint64_t kept = 0;  // a bit for each node
+  float least = INFINITY, above = -INFINITY;
+#pragma unroll 1
+  for (uint32_t at = 0; at < a.nodes; at += G) {  // the same rounds for all lanes, which vote in them
+    const uint32_t n = at + g;
+    const float mine = n < a.nodes ? values[n] : -INFINITY;
+    uint32_t before = n < a.nodes ? 0 : a.nodes;
+    for (uint32_t o = 0; o < a.nodes; ++o) {
+      const float v = values[o];
+      before += v > mine || (v == mine && o < n);
+    }
+    const bool is = before < a.top_nodes;
+    least = is ? fminf(least, mine) : least;
+    above = is ? above : fmaxf(above, mine);
+    const uint64_t all = __ballot(is) >> ((threadIdx.x & 63) & ~(uint32_t)(G - 1));
+    kept |= (all & ((1ull << G) - 1)) << at;
+  }
+  lanes_agree();  // before the next token's numbers are laid there
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const uint32_t n = min((i * G + g) / chunks_per, 63u);
+#pragma unroll
+    for (int r = 0; r < 8; ++r) c[8 * i + r] = kept >> n & 1 ? c[8 * i + r] : -INFINITY;
+  }
+  above = most<G>(above);
+  return above > -INFINITY ? -most<G>(-least) - above : INFINITY;
+}
+
+// ---------------------------------------------------------------- in double
+// The largest of a wavefront's lanes.
+__device__ inline uint64_t most_key64(uint64_t v) {
+  auto step = [&](uint64_t o) __attribute__((always_inline)) { v = o > v ? o : v; };
+  step(across<1>(v));
+  step(across<2>(v));
+  step(across<4>(v));
+  step(across<8>(v));
+  step(across<16>(v));
+  step(across<32>(v));
+  return v;
+}
+
+// The same choice of one token by a whole wavefront, EACH neighbouring experts a
+// lane; d: LDS for 64 EACH doubles. Lane j returns choice j. A few tokens go through
+// it, each once in a while, so what it takes is fetching its code and waiting for
+// one step after the other: there is one exp and one quotient, in a loop.
+template <class T, int EACH>
+__device__ inline int32_t pick_exactly(const RouteArgs& a, int64_t t, double* d) {
+  const uint32_t lane = threadIdx.x & 63, e0 = lane * EACH;
+  const bool scores = by_scores(a);
+  float l[EACH], b[EACH], big = -INFINITY;
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    const uint32_t e = min(e0 + i, a.E - 1);
+    l[i] = to_float(((const T*)a.logits)[t * a.ld + e]);
+    b[i] = a.bias ? a.bias[e] : 0.0f;
+    if (e0 + i >= a.E || (a.mask && !a.mask[t * a.mask_ld + e])) l[i] = -INFINITY;
+    big = l[i] != l[i] || big != big ? NAN : fmaxf(big, l[i]);
+  }
+  double c[EACH];
+  if (!scores) {
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) c[i] = l[i];
   } else {
-    float z = 0;
+    big = a.sigmoid ? 0.0f : most<64>(big);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      c[i] = r.allowed >> i & 1 ? __builtin_amdgcn_exp2f(LOG2E * (r.l[i] - r.big)) : 0.0f;
-      z += c[i];
+    for (int i = 0; i < EACH; ++i) d[e0 + i] = a.sigmoid ? -(double)l[i] : (double)l[i] - (double)big;
+    double z = 0;
+#pragma unroll 1
+    for (int i = 0; i < EACH; ++i) {
+      const double v = exp(d[e0 + i]);
+      d[e0 + i] = v;
+      z += v;
     }
-    z = __builtin_amdgcn_rcpf(group_sum<G>(z));
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] *= z;
-  }
-  if (a.bias) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] += g * 8 + i < a.E ? a.bias[g * 8 + i] : 0.0f;
-  }
-  uint32_t s[8], size = 0, allowed = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    if (!(r.allowed >> i & 1) || c[i] == -INFINITY) continue;
-    allowed |= 1u << i;
-    size = max(size, __float_as_uint(c[i]) & 0x7fffffffu);
-  }
-  // How near two decisive numbers may come. A sigmoid is off by up to 2^-22, a
-  // softmax's share by 2^-20 (a sum 14 additions deep), a sum with the bias by
-  // 2^-24 of its size, and the word leaves 2^-20 of it away; a node's sum of two
-  // twice all that, and so does a difference. NaN is near everything.
-  float clear = INFINITY;  // the least difference that decides something
-  const float near = (a.sigmoid ? 0x1p-20f : 0x1p-18f) + 0x1p-18f * __uint_as_float(most_key<G>(size));
-
-  // the lanes of a node: a power of two of them alone, or 0
-  const uint32_t per = a.E / a.nodes, lanes = a.nodes > 1 && per % 8 == 0 && __popc(per) == 1 ? per / 8 : 0;
-  if (a.nodes > 1 && !lanes) {
-    const Kept k = keep_nodes<G>(a, g, c, allowed, own);
-    allowed = k.allowed;
-    clear = k.clear;
-  }
-#pragma unroll
-  for (int i = 0; i < 8; ++i) s[i] = allowed >> i & 1 ? (rising(c[i]) & ~7u) | (7 - i) : 0;
-  auto order = [&](int i, int j) __attribute__((always_inline)) {
-    const uint32_t hi = max(s[i], s[j]), lo = min(s[i], s[j]);
-    s[i] = hi;
-    s[j] = lo;
-  };
-  order(0, 1), order(2, 3), order(4, 5), order(6, 7), order(0, 2), order(1, 3), order(4, 6), order(5, 7);
-  order(1, 2), order(5, 6), order(0, 4), order(1, 5), order(2, 6), order(3, 7), order(2, 4), order(3, 5);
-  order(1, 2), order(3, 4), order(5, 6);
-
-  if (lanes) {
-    // a node's two largest by all of its lanes
-    float one = s[0] ? key_value(s[0]) : -INFINITY, two = s[1] ? key_value(s[1]) : -INFINITY;
-    for (uint32_t d = 1; d < lanes; d *= 2) {
-      const float o1 = __shfl_xor(one, d), o2 = __shfl_xor(two, d);
-      two = fmaxf(fminf(one, o1), fmaxf(two, o2));
-      one = fmaxf(one, o1);
+    if (!a.sigmoid)
+#pragma unroll 1
+      for (int m = 1; m < 64; m *= 2) z += __shfl_xor(z, m);
+#pragma unroll 1
+    for (int i = 0; i < EACH; ++i) {
+      const double v = d[e0 + i];
+      d[e0 + i] = (a.sigmoid ? 1.0 : v) / (a.sigmoid ? 1.0 + v : z);
     }
-    const float mine = a.node_best == 2 && two > -INFINITY ? one + two : one;
-    if (g % lanes == 0) own[g / lanes] = mine;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) c[i] = l[i] == -INFINITY ? -INFINITY : d[e0 + i] + (double)b[i];
+  }
+  if (a.nodes > 1) {
+    // a node's value and then whether it is kept are laid in its first expert's place
+    const uint32_t per = a.E / a.nodes;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) d[e0 + i] = c[i];
     lanes_agree();
-    uint32_t before = 0;
-    for (uint32_t n = 0; n < a.nodes; ++n) before += own[n] > mine || (own[n] == mine && n < g / lanes);
-    const bool kept = before < a.top_nodes;
-    const float least = -most<G>(kept ? -mine : -INFINITY), above = most<G>(kept ? -INFINITY : mine);
-    if (above > -INFINITY) clear = least - above;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = kept ? s[i] : 0;
-    lanes_agree();  // before the next numbers are laid there
-  }
-
-  const uint32_t lane = threadIdx.x & 63, first_lane = lane & ~(uint32_t)(G - 1);
-  float last = INFINITY;
-  auto next = [&](int32_t& expert) __attribute__((always_inline)) {
-    const uint32_t best = most_key<G>(s[0]);
-    uint64_t here = __ballot(s[0] == best) >> first_lane;
-    if constexpr (G < 64) here &= (1ull << G) - 1;
-    const uint32_t from = G == 1 ? lane : first_lane + __ffsll((unsigned long long)here) - 1;
-    const bool out = lane == from;
-#pragma unroll
-    for (int i = 0; i < 7; ++i) s[i] = out ? s[i + 1] : s[i];
-    s[7] = out ? 0 : s[7];
-    const float value = key_value(best);
-    if (best) {
-      clear = fminf(clear, last - value);
-      last = value;
-    }
-    expert = best ? (int32_t)((from - first_lane) * 8 + 7 - (best & 7)) : -1;
-  };
-#pragma unroll
-  for (int q = 0; q < keep(G); ++q) {
-    e[q] = -1;
-    if (q * G < (int)a.k) {
-      for (uint32_t j = 0; j < G && q * G + j < a.k; ++j) {
-        int32_t expert;
-        next(expert);
-        if (g == j) e[q] = expert;
+#pragma unroll 1
+    for (uint32_t n = lane; n < a.nodes; n += 64) {
+      double one = -INFINITY, two = -INFINITY;
+      bool nan = false;
+#pragma unroll 4
+      for (uint32_t i = 0; i < per; ++i) {
+        const double v = d[n * per + i];
+        nan |= v != v;
+        two = fmax(two, fmin(one, v));
+        one = fmax(one, v);
       }
+      if (a.node_best == 2 && two > -INFINITY) one += two;
+      d[n * per] = nan ? NAN : one;
     }
+    lanes_agree();
+    uint32_t is = 0, at = 0;
+#pragma unroll 1
+    for (uint32_t n = lane; n < a.nodes; n += 64, ++at) {
+      const uint64_t mine = rising(d[n * per]);
+      uint32_t before = 0;
+#pragma unroll 4
+      for (uint32_t m = 0; m < a.nodes; ++m) {
+        const uint64_t v = rising(d[m * per]);
+        before += v > mine || (v == mine && m < n);
+      }
+      if (before < a.top_nodes) is |= 1u << at;
+    }
+    lanes_agree();
+    at = 0;
+#pragma unroll 1
+    for (uint32_t n = lane; n < a.nodes; n += 64, ++at) d[n * per] = is >> at & 1;
+    lanes_agree();
+#pragma unroll
+    for (int i = 0; i < EACH; ++i)
+      if (e0 + i < a.E && d[(e0 + i) / per * per] == 0) c[i] = -INFINITY;
+    lanes_agree();  // before the next token's numbers are laid there
   }
-  int32_t expert;
-  next(expert);  // the best that is not chosen has to be clearly less
-  return clear > near;
+  uint64_t key[EACH];
+#pragma unroll
+  for (int i = 0; i < EACH; ++i) {
+    // without a bias the experts go by their logits, and only the nodes by scores
+    key[i] = c[i] == -INFINITY ? 0 : rising(scores && !a.bias ? (double)l[i] : c[i]);
+  }
+  int32_t chosen = -1;  // of choice number `lane`
+#pragma unroll 1
+  for (uint32_t j = 0; j < a.k; ++j) {
+    uint64_t mine = 0;  // the largest of this lane's, the lowest of equals at `at`
+    uint32_t at = 0;
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) {
+      at = key[i] > mine ? i : at;
+      mine = key[i] > mine ? key[i] : mine;
+    }
+    const uint64_t best = most_key64(mine);
+    if (!best) break;
+    const uint32_t from = __ffsll((unsigned long long)__ballot(mine == best)) - 1;
+    at = __builtin_amdgcn_readlane(at, from);
+    if (lane == j) chosen = (int32_t)(from * EACH + at);
+#pragma unroll
+    for (int i = 0; i < EACH; ++i) key[i] = lane == from && i == (int)at ? 0 : key[i];
+  }
+  return chosen;
 }
 
-// Chooses a token's experts: lane j of its G lanes keeps choices j, j + G, ... in
-// e. V: the type of the decisive numbers, double for scores, float for logits.
-// own: LDS for the token's c, 8 a lane.
-template <class V, int G>
-__device__ inline void pick(const RouteArgs& a, const Row& r, uint32_t g, V* own, int32_t (&e)[keep(G)]) {
-  constexpr bool SCORES = std::is_same<V, double>::value;
-  V c[8];
+// ---------------------------------------------------------------- weights
+// The weights of the choices of one token, which its G lanes keep, from their
+// logits lc (-inf: none): normalized ones from the largest chosen logit where they
+// are a softmax, or sigmoids so small that they are exp(l). z_all: sum of exp(l -
+// big) over the allowed, of a softmax that is not normalized.
+template <int G, int KEEP>
+__device__ inline void weigh(const RouteArgs& a, const float (&lc)[KEEP], float big, float z_all, float (&w)[KEEP]) {
+  float top = -INFINITY;
+  if (a.normalize) {
 #pragma unroll
-  for (int i = 0; i < 8; ++i) c[i] = (V)r.l[i];
-  if constexpr (SCORES) {
-    if (a.sigmoid) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] = (V)1 / ((V)1 + exp(-c[i]));
-    } else {
-      V z = 0;
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        c[i] = exp(c[i] - (V)r.big);
-        z += r.allowed >> i & 1 ? c[i] : (V)0;
-      }
-      z = sum<G>(z);
-#pragma unroll
-      for (int i = 0; i < 8; ++i) c[i] /= z;
-    }
-    if (a.bias) {
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (g * 8 + i < a.E) c[i] += (V)a.bias[g * 8 + i];
-    }
-  }
-  uint32_t allowed = 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if ((r.allowed >> i & 1) && !(c[i] == (V)-INFINITY)) allowed |= 1u << i;
-
-  if (a.nodes > 1) allowed = keep_nodes<G>(a, g, c, allowed, own).allowed;
-
-  // without a bias the experts go by their logits, and only the nodes by scores
-  const bool by_scores = SCORES && a.bias;
-  Candidate<V> s[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-    if (allowed >> i & 1) s[i] = Candidate<V>(by_scores ? c[i] : (V)r.l[i], g * 8 + i);
-  // Batcher's odd-even merge of 8: 19 exchanges
-  auto order = [&](int i, int j) __attribute__((always_inline)) {
-    if (s[j] > s[i]) {
-      const Candidate<V> t = s[i];
-      s[i] = s[j];
-      s[j] = t;
-    }
-  };
-  order(0, 1), order(2, 3), order(4, 5), order(6, 7), order(0, 2), order(1, 3), order(4, 6), order(5, 7);
-  order(1, 2), order(5, 6), order(0, 4), order(1, 5), order(2, 6), order(3, 7), order(2, 4), order(3, 5);
-  order(1, 2), order(3, 4), order(5, 6);
-  // the next largest leaves its lane
-  auto next = [&]() __attribute__((always_inline)) {
-    const Candidate<V> best = largest<G>(s[0]);
-    if (best.any() && s[0] == best) {
-#pragma unroll
-      for (int i = 0; i < 7; ++i) s[i] = s[i + 1];
-      s[7] = Candidate<V>();
-    }
-    return best;
-  };
-#pragma unroll
-  for (int q = 0; q < keep(G); ++q) {
-    e[q] = -1;
-    if (q * G < (int)a.k) {
-      for (uint32_t j = 0; j < G && q * G + j < a.k; ++j) {
-        const Candidate<V> best = next();
-        if (g == j && best.any()) e[q] = (int32_t)best.expert();
-      }
-    }
-  }
-}
-
-// LDS for the numbers of a wavefront's tokens: a float for each of a lane's 8
-// experts, which are taken by one token at a time where it is doubles that they
-// have to hold.
-constexpr uint32_t space_of_wave(int G) { return G < 64 ? 64 * 8 * 4 : 64 * 8 * 8; }
-
-// One workgroup's tokens [t0, t1): G lanes a token, 8 experts a lane. Counts the
-// chosen experts in `base`.
-template <class T, int G, bool SCORES>
-__device__ void choose_balanced(const RouteArgs& a, int64_t t0, int64_t t1, uint32_t* base, char* space) {
-  const uint32_t g = threadIdx.x % G;
-  const bool whole = g * 8 + 8 <= a.E && a.vector;
-  char* wave_space = space + threadIdx.x / 64 * space_of_wave(G);
-  float* own = (float*)wave_space + (threadIdx.x & 63) / G * (G * 8);
-  for (int64_t at = t0; at < t1; at += THREADS / G) {
-    const int64_t t = at + threadIdx.x / G;
-    if (t >= t1) continue;  // whole groups of G lanes leave together
-    const T* row = (const T*)a.logits + t * a.ld;
-    const uint8_t* mask = a.mask ? a.mask + t * a.mask_ld + g * 8 : nullptr;
-    Row r;
-    r.allowed = 0;
-    T l[8];
-    uint64_t in = ~0ull;  // a byte per expert
-    if (whole) {
-      __builtin_memcpy(l, __builtin_assume_aligned(row + g * 8, 16), sizeof(l));
-      if (mask) __builtin_memcpy(&in, __builtin_assume_aligned(mask, 8), 8);
-    } else {
-      for (uint32_t i = 0; i < 8; ++i) {
-        const bool is = g * 8 + i < a.E;
-        l[i] = is ? row[g * 8 + i] : (T)0.0f;
-        if (!is || (mask && !mask[i])) in &= ~(0xffull << (8 * i));
-      }
-    }
-    r.big = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      r.l[i] = (float)l[i];
-      if ((in >> (8 * i) & 0xff) && !(r.l[i] == -INFINITY)) {
-        r.allowed |= 1u << i;
-        r.big = r.l[i] != r.l[i] || r.big != r.big ? NAN : fmaxf(r.big, r.l[i]);
-      }
-    }
-    r.big = most<G>(r.big);
-
-    int32_t e[keep(G)];
-    if constexpr (SCORES) {
-      const bool sure = pick_near<G>(a, r, g, own, e);
-      for (uint64_t left = __ballot(!sure); left;) {  // one token after the other
-        const uint32_t first = (uint32_t)(__ffsll((unsigned long long)left) - 1) / G;
-        if ((threadIdx.x & 63) / G == first) pick<double, G>(a, r, g, (double*)wave_space, e);
-        left &= G == 64 ? 0 : ~(((1ull << (G % 64)) - 1) << (first * G));
-      }
-    } else {
-      pick<float, G>(a, r, g, own, e);
-    }
-
-    // scores of the chosen; normalized ones from the largest chosen logit where
-    // they are a softmax, or sigmoids so small that they are exp(l)
-    float z = 1, p[keep(G)], lc[keep(G)], top = -INFINITY;
-#pragma unroll
-    for (int q = 0; q < keep(G); ++q) {
-      lc[q] = e[q] < 0 ? -INFINITY : (float)row[e[q]];
-      top = lc[q] != lc[q] || top != top ? NAN : fmaxf(top, lc[q]);
-    }
+    for (int q = 0; q < KEEP; ++q) top = lc[q] != lc[q] || top != top ? NAN : fmaxf(top, lc[q]);
     top = most<G>(top);
-    const bool by_exp = !a.sigmoid || (a.normalize && top < -40.0f);
-    const float from = a.normalize ? top : r.big;
-    if (a.normalize) {
-      z = 0;
-    } else if (!a.sigmoid) {
-      z = 0;
+  }
+  const bool by_exp = !a.sigmoid || (a.normalize && top < -40.0f);
+  const float from = a.normalize ? top : big;
+  float z = a.normalize ? 0 : a.sigmoid ? 1 : z_all;
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        if (r.allowed >> i & 1) z += expf(r.l[i] - from);
-      z = group_sum<G>(z);
-    }
+  for (int q = 0; q < KEEP; ++q) {
+    const float x = expf(by_exp ? lc[q] - from : -lc[q]);
+    w[q] = lc[q] == -INFINITY ? 0.0f : by_exp ? x : 1.0f / (1.0f + x);
+    if (a.normalize) z += w[q];
+  }
+  if (a.normalize) z = group_sum<G>(z);
 #pragma unroll
-    for (int q = 0; q < keep(G); ++q) {
-      p[q] = e[q] < 0 ? 0.0f : by_exp ? expf(lc[q] - from) : 1.0f / (1.0f + expf(-lc[q]));
-      if (a.normalize) z += p[q];
-    }
-    if (a.normalize) z = group_sum<G>(z);
+  for (int q = 0; q < KEEP; ++q) w[q] = lc[q] == -INFINITY ? 0.0f : a.scale * (w[q] / z);
+}
+
+// ---------------------------------------------------------------- tokens
+constexpr int32_t UNSURE = INT32_MIN;  // first choice of a token that is to be decided in double
+
+__device__ inline void put(const RouteArgs& a, int64_t t, uint32_t j, int32_t e, float w, uint32_t* base) {
+  a.experts[t * a.k + j] = e;
+  a.weights[t * a.k + j] = w;
+  atomicAdd(&base[e < 0 ? a.E : e], 1u);
+}
+
+// One workgroup's tokens [t0, t1): G lanes a token, C chunks a lane, up to P times 8
+// choices. Counts the chosen experts in `base`; space: LDS of the lanes; sbias: each
+// expert's bias in the chunks' order, 0 without. Says in `unsure` whether a token is.
+template <class T, int G, int C, int P>
+__device__ void choose_balanced(const RouteArgs& a, int64_t t0, int64_t t1, uint32_t* base, float* space,
+                                const float* sbias, float near, uint32_t* unsure) {
+  constexpr int W = G < 8 ? G : 8, EACH = 8 / W;  // lanes that keep choices, choices of a pass that each keeps
+  constexpr float LOG2E = 1.44269504f;
+  const uint32_t g = threadIdx.x % G;
+  const Chunks ch = chunks_of(a.E, a.nodes);
+  const bool whole = a.vector && ch.per % 8 == 0, scores = by_scores(a);
+  float* own = space + threadIdx.x / G * (G * lane_space(C));
+  uint32_t first[C], count[C];  // of the lane's chunks: first expert, how many
 #pragma unroll
-    for (int q = 0; q < keep(G); ++q) {
-      const uint32_t j = q * G + g;
-      if (j < a.k) {
-        a.experts[t * a.k + j] = e[q];
-        a.weights[t * a.k + j] = e[q] < 0 ? 0.0f : a.scale * (p[q] / z);
-        atomicAdd(&base[e[q] < 0 ? a.E : e[q]], 1u);
+  for (int i = 0; i < C; ++i) {
+    const uint32_t n = (i * G + g) / ch.chunks_per, in = (i * G + g) % ch.chunks_per * 8;
+    count[i] = n < a.nodes ? min(ch.per - in, 8u) : 0;
+    first[i] = n < a.nodes ? n * ch.per + in : 0;
+  }
+  // every lane of a wavefront stays in it: past the end, tokens are taken again and not written
+  const int64_t rounds = (t1 - t0 + THREADS / G - 1) / (THREADS / G);
+  for (int64_t round = 0; round < rounds; ++round) {
+    const int64_t here = t0 + round * (THREADS / G) + threadIdx.x / G, t = min(here, t1 - 1);
+    const T* row = (const T*)a.logits + t * a.ld;
+    const uint8_t* mask = a.mask ? a.mask + t * a.mask_ld : nullptr;
+    // nothing that is made from these is kept from token to token
+#pragma unroll
+    for (int i = 0; i < C; ++i) asm volatile("" : "+v"(first[i]), "+v"(count[i]));
+    // the logits, -inf where the expert is not allowed; one chunk after the other
+    // here and below: several at once do not fit the registers
+    float c[8 * C];
+    if (whole) {
+      T l[8 * C];
+#pragma unroll
+      for (int i = 0; i < C; ++i) __builtin_memcpy(l + 8 * i, __builtin_assume_aligned(row + first[i], 16), 8 * sizeof(T));
+#pragma unroll
+      for (int i = 0; i < C; ++i)
+#pragma unroll
+        for (int r = 0; r < 8; ++r) c[8 * i + r] = count[i] ? (float)l[8 * i + r] : -INFINITY;
+      if (mask) {
+#pragma unroll
+        for (int i = 0; i < C; ++i) {
+          uint64_t m;
+          __builtin_memcpy(&m, __builtin_assume_aligned(mask + first[i], 8), 8);
+#pragma unroll
+          for (int r = 0; r < 8; ++r) c[8 * i + r] = (m >> (8 * r) & 0xff) ? c[8 * i + r] : -INFINITY;
+        }
       }
+    } else {
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        uint8_t m[8];
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const uint32_t e = min(first[i] + r, a.E - 1);
+          c[8 * i + r] = (float)row[e];
+          m[r] = mask ? mask[e] : 1;
+        }
+#pragma unroll
+        for (int r = 0; r < 8; ++r) c[8 * i + r] = r < (int)count[i] && m[r] ? c[8 * i + r] : -INFINITY;
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    float big = -INFINITY, z = 0;  // of a softmax
+    if (!a.sigmoid) {
+      bool nan = false;
+#pragma unroll
+      for (int i = 0; i < 8 * C; ++i) {
+        big = fmaxf(big, c[i]);
+        nan |= c[i] != c[i];
+      }
+      big = most<G>(nan ? NAN : big);
+      if (scores || !a.normalize) {
+#pragma unroll
+        for (int i = 0; i < 8 * C; ++i) {
+          z += c[i] == -INFINITY ? 0.0f : __builtin_amdgcn_exp2f(LOG2E * (c[i] - big));
+          if (i % 8 == 7) __builtin_amdgcn_sched_barrier(0);
+        }
+        z = group_sum<G>(z);
+      }
+    }
+    if (scores) {
+      // exp through exp2 of a rounded product: off by |l| 2^-24 of itself, and
+      // |x| exp(-|x|) < 1
+      const float per_z = __builtin_amdgcn_rcpf(z);
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        const float* b = sbias + 8 * (i * G + g);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float l = c[8 * i + r], x = __builtin_amdgcn_exp2f(a.sigmoid ? -LOG2E * l : LOG2E * (l - big));
+          const float v = (a.sigmoid ? __builtin_amdgcn_rcpf(1.0f + x) : x * per_z) + b[r];
+          c[8 * i + r] = l == -INFINITY ? -INFINITY : v;
+        }
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    }
+    bool bad = false;  // a NaN or +inf, which the candidates cannot hold
+#pragma unroll
+    for (int i = 0; i < 8 * C; ++i) bad |= !(c[i] < INFINITY);
+    float clear = INFINITY;  // the least difference that decides something
+    if (a.nodes > 1) {
+      clear = keep_nodes<G, C>(a, ch.chunks_per, g, c, own);
+      if (!scores) clear = INFINITY;  // logits are what they are, and ties are in order
+    }
+
+    int32_t e[P * EACH];
+    double limit = INFINITY;  // the last pass's least
+    float last = INFINITY;
+#pragma unroll
+    for (int p = 0; p < P; ++p) {
+#pragma unroll
+      for (int q = 0; q < EACH; ++q) e[p * EACH + q] = -1;
+      if (p * 8 >= (int)a.k) break;
+      const bool ask = scores && (int)a.k == 8 * (p + 1);
+      double top[8], rest = -INFINITY;
+#pragma unroll
+      for (int i = 0; i < C; ++i) {
+        double s[8];
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          s[r] = candidate(c[8 * i + r], first[i] + r);
+          if (p) s[r] = s[r] < limit ? s[r] : -INFINITY;
+        }
+        sort8(s);
+        if (i == 0) {
+#pragma unroll
+          for (int r = 0; r < 8; ++r) top[r] = s[r];
+        } else {
+          merge8(top, s, rest, ask);
+        }
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      merge_lanes<G>(top, rest, ask);
+      __builtin_amdgcn_sched_barrier(0);
+      limit = top[7];
+      if (scores) {
+        float before = last;
+#pragma unroll
+        for (int r = 0; r < 8; ++r) {
+          const float v = (float)top[r];
+          if (p * 8 + r <= (int)a.k) clear = fminf(clear, v == -INFINITY ? INFINITY : before - v);
+          before = v;
+        }
+        last = before;
+        if (ask && rest > -INFINITY) clear = fminf(clear, before - (float)rest);
+      }
+#pragma unroll
+      for (int q = 0; q < EACH; ++q) {
+        double v = top[q * W];
+#pragma unroll
+        for (int o = 1; o < W; ++o) v = g == o ? top[q * W + o] : v;
+        e[p * EACH + q] = g < W && p * 8 + q * W + g < a.k ? expert_of(v) : -1;
+      }
+    }
+    const bool sure = clear > near && !most_key<G>(bad);
+
+    float lc[P * EACH], w[P * EACH];
+#pragma unroll
+    for (int q = 0; q < P * EACH; ++q) lc[q] = e[q] < 0 ? -INFINITY : (float)row[e[q]];
+    weigh<G>(a, lc, big, z, w);
+    if (here >= t1) continue;
+    if (!sure) {
+      if (g == 0) {
+        a.experts[t * a.k] = UNSURE;
+        *unsure = 1;
+      }
+      continue;
+    }
+#pragma unroll
+    for (int q = 0; q < P * EACH; ++q) {
+      const uint32_t j = q * W + g;
+      if (g < W && j < a.k) put(a, t, j, e[q], w[q], base);
     }
   }
 }
 
-constexpr uint32_t space_bytes(int G, uint32_t nodes) { return nodes > 1 ? WAVES * space_of_wave(G) : 0; }
+// Those of the tokens that are marked as unsure, each by a wavefront.
+template <class T, int EACH>
+__device__ void choose_exactly(const RouteArgs& a, int64_t t0, int64_t t1, uint32_t* base, double* d) {
+  const uint32_t lane = threadIdx.x & 63, each = (a.E + 63) / 64;
+  for (int64_t at = t0 + threadIdx.x / 64; at < t1; at += WAVES * 64) {  // neighbours to different wavefronts
+    const int64_t look = at + (int64_t)lane * WAVES;
+    uint64_t marked = __ballot(look < t1 && a.experts[look * a.k] == UNSURE);
+    for (; marked; marked &= marked - 1) {
+      const int64_t t = at + (int64_t)(__ffsll((unsigned long long)marked) - 1) * WAVES;
+      const int32_t e[1] = {pick_exactly<T, EACH>(a, t, d)};
+      float lc[1] = {e[0] < 0 ? -INFINITY : to_float(((const T*)a.logits)[t * a.ld + e[0]])}, w[1];
+      float big = -INFINITY, z = 0;
+      const bool full = !a.normalize && !a.sigmoid;
+      for (uint32_t i = 0; full && i < each; ++i) {
+        const uint32_t x = lane * each + i;
+        float l;
+        if (x < a.E && allowed_at<T>(a, t, x, l)) big = l != l || big != big ? NAN : fmaxf(big, l);
+      }
+      if (full) big = most<64>(big);
+      for (uint32_t i = 0; full && i < each; ++i) {
+        const uint32_t x = lane * each + i;
+        float l;
+        if (x < a.E && allowed_at<T>(a, t, x, l)) z += expf(l - big);
+      }
+      weigh<64>(a, lc, big, group_sum<64>(z), w);
+      if (lane < a.k) put(a, t, lane, e[0], w[0], base);
+    }
+  }
+}
 
-template <class T, int G, bool SCORES>
-__global__ void __launch_bounds__(THREADS) balanced_kernel(RouteArgs a) {
-  extern __shared__ __attribute__((aligned(16))) uint32_t lds[];
-  uint32_t* words = lds + space_bytes(G, a.nodes) / 4;
-  uint32_t *base = words, *counts = words + a.E + 1;
+constexpr int each_of(int G, int C) { return G * C < 8 ? 1 : G * C / 8; }  // experts of a lane of 64
+// LDS: the tokens' numbers in float, in whose place a wavefront of each 16 then has
+// E doubles of one token, the biases, the counts.
+template <int G, int C>
+constexpr uint32_t space_bytes() {
+  const uint32_t tokens = THREADS * lane_space(C) * 4, exact = WAVES * 64 * each_of(G, C) * 8;
+  return tokens > exact ? tokens : exact;
+}
+
+template <class T, int G, int C, int P>
+__global__ void __launch_bounds__(THREADS) balanced_kernel(RouteArgs a, int near_first) {
+  constexpr int EACH = each_of(G, C);
+  extern __shared__ __attribute__((aligned(16))) char lds[];
+  float* sbias = (float*)(lds + space_bytes<G, C>());
+  uint32_t *base = (uint32_t*)(sbias + 8 * G * C), *counts = base + a.E + 1;
+  __shared__ uint32_t unsure, size;
+  const int64_t t0 = (int64_t)blockIdx.x * a.chunk, t1 = min(t0 + (int64_t)a.chunk, a.T);
+  const Chunks ch = chunks_of(a.E, a.nodes);
+  // the first logits are on their way while the biases are laid out
+  float ahead = 0;
+  if (t0 < t1) ahead = to_float(((const T*)a.logits)[min(t0 + threadIdx.x / G, t1 - 1) * a.ld + min(threadIdx.x % G * 8, a.E - 1)]);
+  if (threadIdx.x == 0) unsure = size = 0;
   for (uint32_t i = threadIdx.x; i <= a.E; i += THREADS) base[i] = 0;
   __syncthreads();
-  const int64_t t0 = (int64_t)blockIdx.x * a.chunk, t1 = min(t0 + (int64_t)a.chunk, a.T);
-  choose_balanced<T, G, SCORES>(a, t0, t1, base, (char*)lds);
+  if (a.bias && threadIdx.x < 8 * G * C) {  // whole wavefronts
+    const uint32_t n = threadIdx.x / (ch.chunks_per * 8), in = threadIdx.x % (ch.chunks_per * 8);
+    const float b = n < a.nodes && in < ch.per ? a.bias[n * ch.per + in] : 0.0f;
+    sbias[threadIdx.x] = b;
+    const uint32_t most = most_key<G * C < 8 ? 8 * G * C : 64>(b == -INFINITY ? 0 : __float_as_uint(b) & 0x7fffffffu);
+    if (threadIdx.x % 64 == 0) atomicMax(&size, most);
+  } else if (threadIdx.x < 8 * G * C) {
+    sbias[threadIdx.x] = 0;
+  }
+  __syncthreads();
+  asm volatile("" ::"v"(ahead));
+  // How near two decisive numbers may come. A sigmoid is off by up to 2^-22, a
+  // softmax's share by 2^-20 (a sum 14 additions deep), a sum with the bias by
+  // 2^-24 of its size; a node's sum of two twice all that and 2^-24 of its own, and
+  // so does a difference. Near a bias that is NaN or infinite is everything.
+  const float near = !by_scores(a) ? 0 : (a.sigmoid ? 0x1p-20f : 0x1p-18f) + 0x1p-21f * (1 + __uint_as_float(size));
+  if (near_first) {
+    choose_balanced<T, G, C, P>(a, t0, t1, base, (float*)lds, sbias, near, &unsure);
+  } else {
+    for (int64_t t = t0 + threadIdx.x; t < t1; t += THREADS) a.experts[t * a.k] = UNSURE;
+    unsure = 1;
+  }
+  __threadfence_block();
+  __syncthreads();
+  if (unsure) choose_exactly<T, EACH>(a, t0, t1, base, (double*)lds + threadIdx.x / 64 * (64 * EACH));
   end_chunk(a, base, counts);
 }
 
@@ -540,25 +661,29 @@ __global__ void __launch_bounds__(256) balanced_backward_kernel(RouteArgs a, con
   }
 }
 
-template <class T, int G>
-hipError_t sized(const RouteArgs& a, uint32_t chunks, hipStream_t s) {
-  constexpr uint32_t most = space_bytes(G, 2) + group_lds(G * 8);
-  // the logits decide where they order the experts as their scores do
-  const bool scores = a.bias || (a.nodes > 1 && a.node_best == 2);
-  const uint32_t lds = space_bytes(G, a.nodes) + group_lds(a.E);
-  return scores ? launch<balanced_kernel<T, G, true>, most>(chunks, THREADS, lds, s, a)
-                : launch<balanced_kernel<T, G, false>, most>(chunks, THREADS, lds, s, a);
+template <class T, int G, int C>
+hipError_t sized(const RouteArgs& a, int near_first, uint32_t chunks, hipStream_t s) {
+  constexpr uint32_t more = space_bytes<G, C>() + 8 * G * C * 4, most = more + group_lds(8 * G * C);
+  const uint32_t lds = more + group_lds(a.E);
+  // further choices are further passes over the same numbers
+  return a.k <= 8 ? launch<balanced_kernel<T, G, C, 1>, most>(chunks, THREADS, lds, s, a, near_first)
+                  : launch<balanced_kernel<T, G, C, 4>, most>(chunks, THREADS, lds, s, a, near_first);
 }
 
 template <class T>
 hipError_t typed(const RouteArgs& a, uint32_t chunks, hipStream_t s) {
-  if (a.E <= 8) return sized<T, 1>(a, chunks, s);
-  if (a.E <= 16) return sized<T, 2>(a, chunks, s);
-  if (a.E <= 32) return sized<T, 4>(a, chunks, s);
-  if (a.E <= 64) return sized<T, 8>(a, chunks, s);
-  if (a.E <= 128) return sized<T, 16>(a, chunks, s);
-  if (a.E <= 256) return sized<T, 32>(a, chunks, s);
-  return sized<T, 64>(a, chunks, s);
+  // chunks of 8 that nodes have for themselves; more than the 64 of 512 experts (nodes
+  // of a few experts) are not laid out, and every token is decided in double
+  const uint64_t n = (uint64_t)chunks_of(a.E, a.nodes).chunks_per * a.nodes;
+  const int near_first = n <= 64;
+  const uint64_t m = near_first ? n : (a.E + 7) / 8;
+  if (m <= 1) return sized<T, 1, 1>(a, near_first, chunks, s);
+  if (m <= 2) return sized<T, 2, 1>(a, near_first, chunks, s);
+  if (m <= 4) return sized<T, 4, 1>(a, near_first, chunks, s);
+  if (m <= 8) return sized<T, 8, 1>(a, near_first, chunks, s);
+  if (m <= 16) return sized<T, 8, 2>(a, near_first, chunks, s);
+  if (m <= 32) return sized<T, 8, 4>(a, near_first, chunks, s);
+  return sized<T, 16, 4>(a, near_first, chunks, s);
 }
 
 }  // namespace

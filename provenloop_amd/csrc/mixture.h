@@ -59,6 +59,7 @@ struct RouteArgs {
   int sigmoid = 0;
   uint32_t nodes = 1, top_nodes = 1, node_best = 1;
 };
+inline bool balanced(const RouteArgs& a) { return a.sigmoid || a.bias || a.nodes > 1 || a.scale != 1.0f; }
 // 8 logits of a token, and their mask bytes, can be loaded at once.
 inline bool whole_loads(MixType type, const RouteArgs& a) {
   return (uintptr_t)a.logits % 16 == 0 && (a.T == 1 || a.ld * (type == MIX_F32 ? 4 : 2) % 16 == 0) &&

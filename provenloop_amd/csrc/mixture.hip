@@ -76,6 +76,12 @@ uint64_t hist_words(int64_t tokens, uint32_t experts, uint32_t choices) {
   return chunks > 1 ? chunks * (experts + 1) : 0;
 }
 
+// Of a gate: a balanced one has chunks of its own.
+uint64_t gate_words(const RouteArgs& a) {
+  const uint64_t chunks = balanced(a) ? th::gate_chunks(a.T, a.k) : th::group_chunks(a.T, a.k);
+  return chunks > 1 ? chunks * (a.E + 1) : 0;
+}
+
 uint32_t padded_rank(uint32_t r) { return (r + 3) & ~3u; }
 
 // Rows of 2-byte elements that all start on 16 bytes.
@@ -152,7 +158,7 @@ void gate_forward(const th_gate_args& d, float* weights, int32_t* experts, int32
                   size_t work_bytes, void* stream) {
   RouteArgs a = check_gate(d);
   need(offsets && (d.tokens == 0 || (weights && experts && order)), "null output");
-  need_work(work, work_bytes, hist_words(d.tokens, d.n_experts, d.choices) * 4);
+  need_work(work, work_bytes, gate_words(a) * 4);
   need_device();
   a.weights = weights;
   a.experts = experts;
@@ -591,6 +597,13 @@ int th_route(int dtype, const void* logits, int64_t ld, int64_t tokens, uint32_t
   return guarded([&] {
     const th_gate_args d = plain_gate(dtype, logits, ld, tokens, n_experts, mask, mask_ld, choices, normalize);
     gate_forward(d, weights, experts, order, offsets, work, work_bytes, stream);
+  });
+}
+int th_gate_workspace(const th_gate_args* d, size_t* bytes) {
+  return guarded([&] {
+    need(d != nullptr, "null descriptor");
+    need(bytes != nullptr, "null output");
+    *bytes = gate_words(check_gate(*d)) * 4;
   });
 }
 int th_gate(const th_gate_args* d, float* weights, int32_t* experts, int32_t* order, int32_t* offsets, void* work,

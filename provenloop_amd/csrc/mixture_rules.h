@@ -39,6 +39,16 @@ constexpr uint64_t group_chunk_tokens(uint64_t tokens, uint32_t k) {
   const uint64_t t = chunk / k;
   return t ? t : 1;
 }
+// The same for a balanced gate, which takes longer for a token than placing its
+// slots does: as few as give each of 256 workgroups some, down to 32 tokens, which
+// fill a wavefront on each SIMD.
+constexpr uint64_t gate_chunk_tokens(uint64_t tokens, uint32_t k) {
+  const uint64_t chunk = group_chunk_tokens(tokens, k), few = ceil_div(tokens, 256) < 32 ? 32 : ceil_div(tokens, 256);
+  return tokens * k <= 2048 || chunk < few ? chunk : few;
+}
+constexpr uint64_t gate_chunks(uint64_t tokens, uint32_t k) {
+  return tokens ? ceil_div(tokens, gate_chunk_tokens(tokens, k)) : 1;
+}
 constexpr uint64_t group_chunks(uint64_t tokens, uint32_t k) {
   return tokens ? ceil_div(tokens, group_chunk_tokens(tokens, k)) : 1;
 }

@@ -179,12 +179,12 @@ variable_list route_forward(const Gate& g) {
   Guard guard(logits.device());
   const int64_t t = logits.size(0), e = logits.size(1), k = g.k;
   NEED(k >= 1 && k <= e, "route: choices must be in [1, number of experts]");
+  const th_gate_args d = g.args();
   size_t bytes;
-  check(th_group_workspace(t, (uint32_t)e, (uint32_t)k, &bytes));
+  check(th_gate_workspace(&d, &bytes));
   Tensor weights = make({t, k}, at::kFloat, logits), experts = make({t, k}, at::kInt, logits);
   Tensor order = make({t * k}, at::kInt, logits), offsets = make({e + 1}, at::kInt, logits);
   const Work w = work(bytes, logits);
-  const th_gate_args d = g.args();
   check(th_gate(&d, ptr<float>(weights), ptr<int32_t>(experts), ptr<int32_t>(order), ptr<int32_t>(offsets), w.p, w.bytes,
                 stream(logits)));
   return {weights, experts, order, offsets};

@@ -283,13 +283,15 @@ hipError_t launch_place(const RouteArgs& a, uint32_t chunks, hipStream_t s) {
 }
 
 hipError_t launch_route(MixType type, RouteArgs a, hipStream_t s) {
-  const uint32_t chunks = (uint32_t)th::group_chunks(a.T, a.k);
-  a.chunk = (uint32_t)th::group_chunk_tokens(a.T, a.k);
   a.vector = whole_loads(type, a);
-  if (a.sigmoid || a.bias || a.nodes > 1 || a.scale != 1.0f) {
+  if (balanced(a)) {
+    const uint32_t chunks = (uint32_t)th::gate_chunks(a.T, a.k);
+    a.chunk = (uint32_t)th::gate_chunk_tokens(a.T, a.k);
     const hipError_t e = launch_balanced(type, a, chunks, s);
     return e != hipSuccess ? e : launch_place(a, chunks, s);
   }
+  const uint32_t chunks = (uint32_t)th::group_chunks(a.T, a.k);
+  a.chunk = (uint32_t)th::group_chunk_tokens(a.T, a.k);
   hipError_t e = type == MIX_BF16  ? route_typed<bf16_t>(a, chunks, group_lds(a.E), s)
                  : type == MIX_F16 ? route_typed<f16_t>(a, chunks, group_lds(a.E), s)
                                    : route_typed<float>(a, chunks, group_lds(a.E), s);

@@ -121,6 +121,7 @@ def test_gates(change, text):
     L = _lib.load()
     refused(L.th_gate(gate(**change), P, P, P, P, None, 0, None), text)
     refused(L.th_gate_backward(gate(**change), P, P, P, P, None), text)
+    refused(L.th_gate_workspace(gate(**change), C.byref(C.c_size_t())), text)
 
 
 def test_gate_outputs():
@@ -129,6 +130,12 @@ def test_gate_outputs():
     refused(L.th_gate(gate(), None, P, P, P, None, 0, None), "null output")
     refused(L.th_gate_backward(gate(), P, P, None, P, None), "null argument")
     refused(L.th_gate(gate(tokens=1 << 20), P, P, P, P, None, 0, None), "workspace")
+    size, plain = C.c_size_t(), C.c_size_t()
+    assert L.th_gate_workspace(gate(tokens=5000), C.byref(size)) == 0 and size.value > 0
+    refused(L.th_gate(gate(tokens=5000), P, P, P, P, P, size.value - 1, None), "bytes")
+    # without a bias, nodes or sigmoids it is the plain gate, with its workspace
+    assert L.th_gate_workspace(gate(tokens=5000, score=0, nodes=1, top_nodes=1), C.byref(size)) == 0
+    assert L.th_group_workspace(5000, 8, 2, C.byref(plain)) == 0 and size.value == plain.value
 
 
 def test_python_gate():
