@@ -33,66 +33,116 @@ __device__ inline float over_row(float v, bool most) {
   return v;
 }
 
+// Which strip of which matrix a workgroup takes, and its share of what lies along it.
+struct Share {
+  uint32_t strip, part, parts;
+  uint64_t e;
+};
+__device__ inline Share share_of(const FourRows& a, uint32_t parts) {
+  const uint32_t job = blockIdx.x / parts;
+  return Share{job % a.four.at.strips, blockIdx.x % parts, parts, job / a.four.at.strips};
+}
+
+// Codes of 8 values of a group, as their word. rint(v / s), ties to even, for v and s
+// of T with a quotient below 16: v / s is a tie, n + 1/2, or off any by more than
+// 2^-13 (both have 11 bits at most), and v times the rounded reciprocal is off by
+// less than 2^-18; rounded to a multiple of 2^-14 it is the tie, or on its own side
+// of it. That and the conversion of 8 values into bytes are 50 instructions, quotients
+// and shifts were 130.
+template <bool ZEROS>
+struct Coder {
+  float per, scale, zero;
+  bool small;  // the reciprocal would be infinite
+  __device__ inline Coder(float s, float z) : per(0x1p14f / s), scale(s), zero(z), small(s < 0x1p-100f) {}
+  template <class V>
+  __device__ inline uint32_t word(const V& v, bool slow) const {
+    uint32_t even = 0, odd = 0;  // a byte a code: columns 0, 4, 1, 5 and 2, 6, 3, 7
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float t = rintf(slow ? (float)v[i] / scale * 0x1p14f : (float)v[i] * per);
+      // 8 is even: rounding to a byte comes out the same with it added before
+      float c = ZEROS ? rintf(t * 0x1p-14f) + zero : fmaf(t, 0x1p-14f, 8.0f);
+      c = __builtin_amdgcn_fmed3f(c, ZEROS ? 0.0f : 1.0f, 15.0f);
+      uint32_t& w = i / 2 % 2 ? odd : even;
+      w = __builtin_amdgcn_cvt_pk_u8_f32(c, i % 2 * 2 + i / 4, w);
+    }
+    return even | odd << 4;
+  }
+};
+
 // A wavefront a group of columns of 16 rows. KEEP: steps of 32 columns whose
 // values stay in registers; longer groups are read again for their codes.
-template <class T, int KEEP>
-__global__ void __launch_bounds__(256) quantize4_kernel(FourRows a) {
+template <class T, int KEEP, bool ZEROS>
+__global__ void __launch_bounds__(256) quantize4_kernel(FourRows a, uint32_t parts) {
+  typedef __attribute__((ext_vector_type(8))) uint16_t u16x8;
   const uint32_t lane = threadIdx.x & 63;
   const th::FourLayout f = a.four.at;
-  const uint64_t jobs = (uint64_t)a.E * f.strips * f.groups;
-  for (uint64_t job = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); job < jobs; job += (uint64_t)gridDim.x * 4) {
-    const uint32_t g = job % f.groups, strip = job / f.groups % f.strips, e = job / f.groups / f.strips;
-    const uint32_t row = strip * 16 + lane % 16, k0 = g << f.shift;
+  const Share m = share_of(a, parts);
+  const uint32_t row = m.strip * 16 + lane % 16;
+  const T* in = (const T*)a.in + (int64_t)m.e * a.lde + (int64_t)min(row, a.rows - 1) * a.ld;
+  uint8_t* out = (uint8_t*)a.four.codes + m.e * f.codes() + (uint64_t)m.strip * f.blocks * 512 + lane * 8;
+  for (uint32_t g = m.part * 4 + (threadIdx.x >> 6); g < f.groups; g += parts * 4) {
+    const uint32_t k0 = g << f.shift;
     const uint32_t k1 = (uint32_t)min((uint64_t)k0 + (1ull << f.shift), (uint64_t)f.blocks * 64), steps = (k1 - k0) / 32;
-    const T* in = (const T*)a.in + (int64_t)e * a.lde + (int64_t)min(row, a.rows - 1) * a.ld;
     auto fetch = [&](uint32_t step) __attribute__((always_inline)) {
       const uint32_t k = k0 + step * 32 + lane / 16 * 8;
       const bool in_row = row < a.rows && k < a.cols;
       return load8<T>(in_row ? in + k : (const T*)&mix_zero16, in_row ? (int64_t)a.cols - k : 0);
     };
     vec8<T> kept[KEEP];
+    // without zeros, the largest magnitude as its bits, which order like it; NaN and infinity are above all
+    u16x8 size = 0;
     float low = 0, high = 0;
     bool bad = false;
     auto look = [&](const vec8<T>& v) __attribute__((always_inline)) {
-      bad |= !all_finite<T>(v);
+      if constexpr (!ZEROS) {
+        size = __builtin_elementwise_max(size, __builtin_bit_cast(u16x8, v) & (uint16_t)0x7fff);
+      } else {
+        bad |= !all_finite<T>(v);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        low = fminf(low, (float)v[i]);
-        high = fmaxf(high, (float)v[i]);
+        for (int i = 0; i < 8; ++i) {
+          low = fminf(low, (float)v[i]);
+          high = fmaxf(high, (float)v[i]);
+        }
       }
     };
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
-      if (i < (int)steps) {
-        kept[i] = fetch(i);
-        look(kept[i]);
-      }
+      if (i < (int)steps) kept[i] = fetch(i);
+#pragma unroll
+    for (int i = 0; i < KEEP; ++i)
+      if (i < (int)steps) look(kept[i]);
     for (uint32_t i = KEEP; i < steps; ++i) look(fetch(i));
-    low = over_row(low, false);
+    if constexpr (!ZEROS) {
+      uint16_t most = 0;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) most = most > size[i] ? most : size[i];
+      bad = most >= exponent_bits<T>();
+      high = (float)__builtin_bit_cast(T, bad ? (uint16_t)0 : most);
+    } else {
+      low = over_row(low, false);
+    }
     high = over_row(high, true);
     bad = over_row(bad ? 1.0f : 0.0f, true) != 0;
-    const bool zeros = a.four.zeros != nullptr;
-    const T scale = stored_scale((T)(bad ? NAN : zeros ? (high - low) / 15.0f : fmaxf(-low, high) / 7.0f));
+    const T scale = stored_scale((T)(bad ? NAN : ZEROS ? (high - low) / 15.0f : high / 7.0f));
     const float by = (float)scale > 0 ? (float)scale : 1.0f;
     const bool number = (float)scale == (float)scale;
-    const float zero = zeros && number ? fminf(rintf(-low / by), 15.0f) : 8.0f, least = zeros ? 0.0f : 1.0f;
+    const float zero = ZEROS && number ? fminf(rintf(-low / by), 15.0f) : 8.0f;
+    const Coder<ZEROS> coder(by, zero);
+    const bool slow = __any(coder.small);
     auto code = [&](const vec8<T>& v, uint32_t step) __attribute__((always_inline)) {
-      uint32_t c[8];
-#pragma unroll
-      for (int i = 0; i < 8; ++i)
-        c[i] = number ? (uint32_t)fminf(fmaxf(rintf((float)v[i] / by) + zero, least), 15.0f) : 8;
       const uint32_t k = k0 + step * 32;
-      uint8_t* out = (uint8_t*)a.four.codes + e * f.codes() + ((uint64_t)strip * f.blocks + k / 64) * 512;
-      *(uint32_t*)(out + lane * 8 + k / 32 % 2 * 4) = four_word(c);
+      const uint32_t w = slow ? coder.word(v, coder.small) : coder.word(v, false);
+      *(uint32_t*)(out + (uint64_t)(k / 64) * 512 + k / 32 % 2 * 4) = number ? w : 0x88888888u;
     };
 #pragma unroll
     for (int i = 0; i < KEEP; ++i)
       if (i < (int)steps) code(kept[i], i);
     for (uint32_t i = KEEP; i < steps; ++i) code(fetch(i), i);
     if (lane < 16) {
-      const uint64_t at = e * f.scales() + (uint64_t)g * f.strips * 16 + row;
+      const uint64_t at = m.e * f.scales() + (uint64_t)g * f.strips * 16 + row;
       ((T*)a.four.scales)[at] = row < a.rows ? scale : (T)0.0f;
-      if (zeros) ((uint8_t*)a.four.zeros)[at] = (uint8_t)zero;
+      if (ZEROS) ((uint8_t*)a.four.zeros)[at] = (uint8_t)zero;
     }
   }
 }
@@ -100,14 +150,14 @@ __global__ void __launch_bounds__(256) quantize4_kernel(FourRows a) {
 // A wavefront a block of 16 rows by 64 columns: codes, and the scales and zeros
 // of the groups that begin there.
 template <class T>
-__global__ void __launch_bounds__(256) pack4_kernel(FourRows a) {
+__global__ void __launch_bounds__(256) pack4_kernel(FourRows a, uint32_t parts) {
   const uint32_t lane = threadIdx.x & 63;
   const th::FourLayout f = a.four.at;
-  const uint64_t jobs = (uint64_t)a.E * f.strips * f.blocks;
-  for (uint64_t job = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); job < jobs; job += (uint64_t)gridDim.x * 4) {
-    const uint32_t block = job % f.blocks, strip = job / f.blocks % f.strips, e = job / f.blocks / f.strips;
-    const uint32_t row = strip * 16 + lane % 16;
-    const uint8_t* in = (const uint8_t*)a.in + (int64_t)e * a.lde + (int64_t)min(row, a.rows - 1) * a.ld;
+  const Share m = share_of(a, parts);
+  const uint32_t row = m.strip * 16 + lane % 16;
+  const uint8_t* in = (const uint8_t*)a.in + (int64_t)m.e * a.lde + (int64_t)min(row, a.rows - 1) * a.ld;
+  uint8_t* out = (uint8_t*)a.four.codes + m.e * f.codes() + (uint64_t)m.strip * f.blocks * 512 + lane * 8;
+  for (uint32_t block = m.part * 4 + (threadIdx.x >> 6); block < f.blocks; block += parts * 4) {
     uint32_t q[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -123,13 +173,13 @@ __global__ void __launch_bounds__(256) pack4_kernel(FourRows a) {
       }
       q[h] = four_word(c);
     }
-    *(uint2*)((uint8_t*)a.four.codes + job * 512 + lane * 8) = uint2{q[0], q[1]};
+    *(uint2*)(out + (uint64_t)block * 512) = uint2{q[0], q[1]};
     // group number h of the block, if it begins here
     const uint32_t h = lane / 16, k = block * 64 + h * 32, g = k >> f.shift;
     if (h < 2 && k == g << f.shift) {
       const bool in_rows = row < a.rows && g < a.scale_cols;
-      const uint64_t from = ((uint64_t)e * a.rows + row) * a.scale_cols + g;
-      const uint64_t to = e * f.scales() + (uint64_t)g * f.strips * 16 + row;
+      const uint64_t from = (m.e * a.rows + row) * a.scale_cols + g;
+      const uint64_t to = m.e * f.scales() + (uint64_t)g * f.strips * 16 + row;
       ((T*)a.four.scales)[to] = in_rows ? stored_scale(((const T*)a.scales)[from]) : (T)0.0f;
       if (a.four.zeros) ((uint8_t*)a.four.zeros)[to] = in_rows ? a.zeros[from] & 15 : 8;
     }
@@ -137,60 +187,68 @@ __global__ void __launch_bounds__(256) pack4_kernel(FourRows a) {
 }
 
 template <class T>
-__global__ void __launch_bounds__(256) dequantize4_kernel(FourRows a) {
+__global__ void __launch_bounds__(256) dequantize4_kernel(FourRows a, uint32_t parts) {
   const uint32_t lane = threadIdx.x & 63;
   const th::FourLayout f = a.four.at;
-  const uint64_t jobs = (uint64_t)a.E * f.strips * f.blocks;
+  const Share m = share_of(a, parts);
+  const uint32_t row = m.strip * 16 + lane % 16;
   const bool wide = ((uintptr_t)a.out & 15) == 0 && a.ld % 8 == 0 && a.lde % 8 == 0;
-  for (uint64_t job = (uint64_t)blockIdx.x * 4 + (threadIdx.x >> 6); job < jobs; job += (uint64_t)gridDim.x * 4) {
-    const uint32_t block = job % f.blocks, strip = job / f.blocks % f.strips, e = job / f.blocks / f.strips;
-    const uint32_t row = strip * 16 + lane % 16;
-    const uint2 q = *(const uint2*)(a.four.codes + job * 512 + lane * 8);
+  const uint8_t* in = a.four.codes + m.e * f.codes() + (uint64_t)m.strip * f.blocks * 512 + lane * 8;
+  const uint64_t scales = m.e * f.scales() + row, per = (uint64_t)f.strips * 16;
+  T* out = (T*)a.out + (int64_t)m.e * a.lde + (int64_t)row * a.ld;
+  for (uint32_t block = m.part * 4 + (threadIdx.x >> 6); block < f.blocks; block += parts * 4) {
+    const uint2 q = *(const uint2*)(in + (uint64_t)block * 512);
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
       const uint32_t k = block * 64 + h * 32 + lane / 16 * 8;
-      const uint64_t at = e * f.scales() + (uint64_t)(k >> f.shift) * f.strips * 16 + row;
+      const uint64_t at = scales + (k >> f.shift) * per;
       const FourScale<T> s(((const T*)a.four.scales)[at], a.four.zeros ? a.four.zeros[at] : 8);
       vec8<T> v = four_values(h ? q.y : q.x, s);
       if (row >= a.rows || k >= a.out_cols) continue;
-      T* out = (T*)a.out + (int64_t)e * a.lde + (int64_t)row * a.ld + k;
       if (k + 8 > a.cols)
         for (uint32_t i = 0; i < 8; ++i) v[i] = k + i < a.cols ? v[i] : (T)0.0f;
-      if (wide && k + 8 <= a.out_cols) *(vec8<T>*)out = v;
+      if (wide && k + 8 <= a.out_cols) *(vec8<T>*)(out + k) = v;
       else
         for (uint32_t i = 0; i < 8; ++i)
-          if (k + i < a.out_cols) out[i] = v[i];
+          if (k + i < a.out_cols) out[k + i] = v[i];
     }
   }
 }
 
-uint32_t blocks_for(uint64_t jobs) { return th::loop_blocks(th::ceil_div(jobs, 4)); }
+// Workgroups that share a strip's n blocks or groups, four of them at a time: enough
+// for 4096 in all, as far as there is that much to share.
+uint32_t parts_of(const FourRows& a, uint32_t n) {
+  const uint64_t strips = (uint64_t)a.E * a.four.at.strips, most = th::ceil_div(n, 4), want = th::ceil_div(4096, strips);
+  return (uint32_t)(want < most ? want : most);
+}
+template <auto Kernel>
+hipError_t go(const FourRows& a, uint32_t n, hipStream_t s) {
+  const uint32_t parts = parts_of(a, n);
+  return launch<Kernel>((uint64_t)a.E * a.four.at.strips * parts, 256, 0, s, a, parts);
+}
 
-template <class T>
+template <class T, bool ZEROS>
 hipError_t quantize(const FourRows& a, hipStream_t s) {
   const th::FourLayout& f = a.four.at;
-  const uint32_t blocks = blocks_for((uint64_t)a.E * f.strips * f.groups);
   switch (f.shift) {
-    case 5: return launch<quantize4_kernel<T, 1>>(blocks, 256, 0, s, a);
-    case 6: return launch<quantize4_kernel<T, 2>>(blocks, 256, 0, s, a);
-    default: return launch<quantize4_kernel<T, 4>>(blocks, 256, 0, s, a);
+    case 5: return go<quantize4_kernel<T, 1, ZEROS>>(a, f.groups, s);
+    case 6: return go<quantize4_kernel<T, 2, ZEROS>>(a, f.groups, s);
+    default: return go<quantize4_kernel<T, 4, ZEROS>>(a, f.groups, s);
   }
 }
 
 }  // namespace
 
 hipError_t launch_quantize4(MixType type, const FourRows& a, hipStream_t s) {
-  return type == MIX_BF16 ? quantize<bf16_t>(a, s) : quantize<f16_t>(a, s);
+  if (a.four.zeros) return type == MIX_BF16 ? quantize<bf16_t, true>(a, s) : quantize<f16_t, true>(a, s);
+  return type == MIX_BF16 ? quantize<bf16_t, false>(a, s) : quantize<f16_t, false>(a, s);
 }
 
 hipError_t launch_pack4(MixType type, const FourRows& a, hipStream_t s) {
-  const uint32_t blocks = blocks_for((uint64_t)a.E * a.four.at.strips * a.four.at.blocks);
-  return type == MIX_BF16 ? launch<pack4_kernel<bf16_t>>(blocks, 256, 0, s, a)
-                          : launch<pack4_kernel<f16_t>>(blocks, 256, 0, s, a);
+  return type == MIX_BF16 ? go<pack4_kernel<bf16_t>>(a, a.four.at.blocks, s) : go<pack4_kernel<f16_t>>(a, a.four.at.blocks, s);
 }
 
 hipError_t launch_dequantize4(MixType type, const FourRows& a, hipStream_t s) {
-  const uint32_t blocks = blocks_for((uint64_t)a.E * a.four.at.strips * a.four.at.blocks);
-  return type == MIX_BF16 ? launch<dequantize4_kernel<bf16_t>>(blocks, 256, 0, s, a)
-                          : launch<dequantize4_kernel<f16_t>>(blocks, 256, 0, s, a);
+  return type == MIX_BF16 ? go<dequantize4_kernel<bf16_t>>(a, a.four.at.blocks, s)
+                          : go<dequantize4_kernel<f16_t>>(a, a.four.at.blocks, s);
 }
