@@ -36,15 +36,20 @@ __device__ inline f16x8 four_values(uint32_t q, const FourScale<f16_t>& f) {
   return v;
 }
 __device__ inline bf16x8 four_values(uint32_t q, const FourScale<bf16_t>& f) {
-  // bytes: columns 0, 4, 1, 5 and 2, 6, 3, 7 of the word, after the masks
-  const uint32_t even = q & 0x0f0f0f0fu, odd = q >> 4 & 0x0f0f0f0fu;
+  typedef __attribute__((ext_vector_type(2))) float f32x2;
+  typedef __attribute__((ext_vector_type(2))) bf16_t bf16x2;
+  // bytes: columns 0, 4, 1, 5 and 2, 6, 3, 7 of the word
+  uint32_t even = q & 0x0f0f0f0fu, odd = q >> 4 & 0x0f0f0f0fu;
+  asm("" : "+v"(even), "+v"(odd));  // left as they are: a byte's conversion then needs no instruction to cut it out
   bf16x8 v;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const uint32_t w = i % 2 ? odd : even;
-    const uint32_t lo = w >> (8 * (i / 2)) & 0xff, hi = w >> (16 + 8 * (i / 2)) & 0xff;
-    v[2 * i] = (bf16_t)fmaf((float)lo, f.s, f.minus);
-    v[2 * i + 1] = (bf16_t)fmaf((float)hi, f.s, f.minus);
+    const f32x2 c = {fmaf((float)(w >> (8 * (i / 2)) & 0xff), f.s, f.minus),
+                     fmaf((float)(w >> (16 + 8 * (i / 2)) & 0xff), f.s, f.minus)};
+    const bf16x2 b = __builtin_convertvector(c, bf16x2);
+    v[2 * i] = b[0];
+    v[2 * i + 1] = b[1];
   }
   return v;
 }

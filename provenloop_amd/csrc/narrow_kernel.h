@@ -78,6 +78,7 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
   constexpr int OUTS = BM * BN / THREADS ? BM * BN / THREADS : 1;
   constexpr int LINE = FOUR ? 128 / NT : 64;       // contraction steps
   constexpr int LOADS = FOUR ? MT * 2 * (LINE / 64) + 2 : 2 * (MT + NT);  // of a line: 8 rows by 64 steps each
+  constexpr int FEWEST = LINE / 64 + 2;  // FOUR: of a line of at most 8 rows
   constexpr uint32_t STAGE = narrow_stage<MT, NT, FOUR>();
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   float* red = (float*)lds;                        // WAVES x BM x LD, after the rings
@@ -148,6 +149,10 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
       const th::FourLayout f = a.four.at;
       const uint32_t xk = ((lane % 8) ^ (lane / 8)) * 8;  // chunk c of row i lies at c ^ (i % 8)
       const T* p[2 * MT];
+      // only rows that exist are loaded, 8 at a time: with 4-bit weights a tile's x is
+      // the larger part. What else lies in their places gives columns of no output.
+      const uint32_t rows_left = (uint32_t)min(g.end - m0, (int64_t)BM);
+      const bool all_rows = rows_left > BM - 8;
 #pragma unroll
       for (int j = 0; j < 2 * MT; ++j) p[j] = (const T*)a.x + slot_of(m0 + j * 8 + lane / 8) / a.div * a.ldx + xk;
       const uint64_t e = grouped && has ? g.group : 0;
@@ -176,7 +181,8 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
         for (int h = 0; h < SUBS; ++h)
 #pragma unroll
           for (int j = 0; j < 2 * MT; ++j)
-            load_lds16(k0 + h * 64 + xk < a.k ? p[j] + k0 + h * 64 : zero, to + (h * 2 * MT + j) * 1024);
+            if (j * 8 + lane / 8 < rows_left)
+              load_lds16(k0 + h * 64 + xk < a.k ? p[j] + k0 + h * 64 : zero, to + (h * 2 * MT + j) * 1024);
         if (lane < fine_lanes) {
           const uint32_t k = k0 + part * 32;
           const bool in = in_rows && k < f.blocks * 64;
@@ -189,8 +195,9 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
       if (LR) lowrank_at<T, OUTS, THREADS, BN>(a, m0, g.end, n0, low);  // while the first lines are on their way
       uint32_t stage = 0;
       for (uint32_t i = 0; i < turns; ++i) {
-        if (i + S <= turns) arrived<(S - 1) * LOADS>();
-        else arrived<0>();
+        if (i + S > turns) arrived<0>();
+        else if (all_rows) arrived<(S - 1) * LOADS>();
+        else arrived<(S - 1) * FEWEST>();
         const char *xt = ring + stage * STAGE, *ct = xt + BM * LINE * 2, *st = ct + 1024;
         uint2 q[2];
         vec8<T> xf[STEPS][MT];
