@@ -141,10 +141,37 @@ constexpr uint64_t four_bytes(const FourLayout& f, uint32_t matrices, bool zeros
   return matrices * (f.codes() + f.scales() * (zeros ? 3 : 2));
 }
 
-// Whether a product with 4-bit weights goes by their codes in small tiles; a
-// larger one goes by their values, written to a workspace.
+// Whether a product with 4-bit weights goes by their codes in small tiles; a larger
+// one goes by their values, written to a workspace. Both times in ns, fitted to
+// measurements: a 32 x 32 tile takes 6 and 0.3 for each 64 steps; the large tiles 750
+// for each 64 steps of a round over the CUs, the values a 1900th a weight (tiles /
+// values in us: 512 rows of 3584 -> 3584 45 / 53, 768 rows 65 / 52; 1024 of 1536 ->
+// 1536 22 / 28; 8 groups of 100 rows, 3584 -> 1536 43 / 65, of 256 rows, 1536 -> 1536
+// 52 / 35; 64 groups of 24 rows, 1536 -> 1536 52 / 205).
 constexpr bool four_narrow(uint64_t rows, uint32_t n, uint32_t k, uint32_t groups) {
-  return narrow_product(rows, n, k, groups);
+  const uint64_t each = ceil_div(rows, groups), lines = ceil_div(k, 64);
+  const uint64_t tiles = groups * ceil_div(each, 32) * ceil_div(n, 32);
+  const uint64_t rounds = ceil_div(groups * ceil_div(each, 256) * ceil_div(n, 128), 256);
+  return 6000 + tiles * (60 + 3 * lines) / 10 <= 8000 + rounds * lines * 750 + (uint64_t)n * k * groups / 1900;
+}
+// The tile of such a small product, in rows x columns. 8 wavefronts are quicker
+// through a contraction, but a CU holds one or two such workgroups: they take the
+// products that are one round of them, in the fewest rows that make it one (us at 3584
+// -> 3584: 16 rows 7.8 with 16 x 16 and 9.1 with 16 x 32, 32 rows 12.5 and 9.3; 64
+// rows 12.3 with 16 x 32 and 10.7 with 32 x 32; 128 rows 20.4 with 32 x 32 and 14.8
+// with 64 x 32). Larger ones take 4 wavefronts, three workgroups a CU of 32 x 32 or two
+// of 64 x 32, which of them has fewer rounds (256 rows 29.8 and 23.7, 384 rows 38.5
+// and 39.2). Groups of up to 16 rows are weights to be read: 16 x 32 (8 groups of 4
+// rows 21.0, with 16 x 16 40.6).
+enum FourTile { FOUR_16x16, FOUR_16x32, FOUR_32x32_ONCE, FOUR_64x32_ONCE, FOUR_32x32, FOUR_64x32 };
+constexpr FourTile four_tile(uint64_t rows, uint32_t n, uint32_t groups) {
+  const uint64_t each = ceil_div(rows, groups), n32 = groups * ceil_div(n, 32);
+  const uint64_t c16 = ceil_div(each, 16) * n32, c32 = ceil_div(each, 32) * n32, c64 = ceil_div(each, 64) * n32;
+  if (groups * ceil_div(each, 16) * ceil_div(n, 16) <= 256) return FOUR_16x16;
+  if (each <= 16 || c16 <= 256) return FOUR_16x32;
+  if (c32 <= 256) return FOUR_32x32_ONCE;
+  if (c64 <= 256) return FOUR_64x32_ONCE;
+  return ceil_div(c32, 768) <= ceil_div(c64, 512) ? FOUR_32x32 : FOUR_64x32;
 }
 
 // Slots whose adapters a workgroup of the low-rank product looks through by

@@ -1,5 +1,14 @@
 // Products of few output tiles with 4-bit weights: y = x w^T for decodes and
-// small batches.
+// small batches, as narrow.hip's of 16-bit ones. A line of a wavefront is 1 KiB of
+// codes, contiguous in memory, the rows' values and up to 192 bytes of scales and
+// zeros, all by asynchronous loads into the wavefront's ring; a lane then has its
+// operands' codes in its own 16 bytes and makes their values in registers.
+//
+// A quarter of the weights' bytes leaves other things to wait for: x, which every
+// column tile reads from L2 again (8 groups of 4 rows, 3584 -> 3584: 24.8 us for 53 MB
+// with 16 columns a tile, 21.0 with 32), the 23 instructions a word, and for one row
+// the chain of steps before the first load (1536 -> 1536 5.0 us in a series of
+// launches, 3584 -> 3584 6.7).
 #include "narrow_kernel.h"
 
 using namespace mix;
@@ -18,11 +27,13 @@ hipError_t run(const MatArgs& a, hipStream_t s) {
 
 template <class T>
 hipError_t typed(const MatArgs& a, hipStream_t s) {
-  switch (th::narrow_tile(a.rows, a.n, a.offsets ? a.E : 1)) {
-    case th::NARROW_16x16: return run<T, 1, 1, 8, 2>(a, s);
-    case th::NARROW_16x16_MANY: return run<T, 1, 1, 4, 2>(a, s);
-    case th::NARROW_32x16: return run<T, 2, 1, 8, 2>(a, s);
-    default: return run<T, 2, 2, 4, 2>(a, s);
+  switch (th::four_tile(a.rows, a.n, a.offsets ? a.E : 1)) {
+    case th::FOUR_16x16: return run<T, 1, 1, 8, 2>(a, s);
+    case th::FOUR_16x32: return run<T, 1, 2, 8, 2>(a, s);
+    case th::FOUR_32x32_ONCE: return run<T, 2, 2, 8, 2>(a, s);
+    case th::FOUR_64x32_ONCE: return run<T, 4, 2, 8, 2>(a, s);
+    case th::FOUR_32x32: return run<T, 2, 2, 4, 2>(a, s);
+    default: return run<T, 4, 2, 4, 2>(a, s);
   }
 }
 
