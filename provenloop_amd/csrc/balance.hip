@@ -20,12 +20,12 @@
 // Up to 16 lanes take a token, several chunks of 8 experts a lane. Chunks are put in
 // order in a lane's registers and merged there and then across the lanes, 8 numbers
 // with 8: the fewer lanes a token has, the fewer steps go across lanes, which cost
-// most. 65536 tokens of 256 experts on 8 nodes, 8 chosen: 47 us where no two numbers
-// come near, with 16 for the places (32 lanes a token and rounds that take the
-// largest of the lanes' first: 87), 67 where a few tokens are decided again: one of
-// these takes some 12 us, waiting for one step after the other, and nearly every
-// workgroup has one. A copy's rate would be 8 us; about 1300 instructions a
-// wavefront's 8 tokens are 14. One token takes 9.5 us: the chain of its steps.
+// most. 65536 tokens of 256 experts on 8 nodes, 8 chosen, with the launch that places
+// their slots (16 us): 47 us where no two numbers come near (with 32 lanes a token and
+// rounds that take the largest of the lanes' first: 87), 65 where a few tokens of nearly
+// every workgroup are decided again: one of these takes 13 us and more, waiting for one
+// step after the other. A copy's rate would be 8 us; about 2100 vector instructions a
+// wavefront's 8 tokens are 33 of it. One token takes 9.3 us: the chain of its steps.
 #include "route_device.h"
 
 using namespace mix;
@@ -207,17 +207,25 @@ __device__ inline uint64_t most_key64(uint64_t v) {
   step(across<2>(v));
   step(across<4>(v));
   step(across<8>(v));
-  step(across<16>(v));
-  step(across<32>(v));
+  auto swapped = [&](auto lo, auto hi) __attribute__((always_inline)) {
+    const uint64_t x = (uint64_t)hi[0] << 32 | lo[0], y = (uint64_t)hi[1] << 32 | lo[1];
+    v = x > y ? x : y;
+  };
+  swapped(__builtin_amdgcn_permlane16_swap((uint32_t)v, (uint32_t)v, false, false),
+          __builtin_amdgcn_permlane16_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false));
+  swapped(__builtin_amdgcn_permlane32_swap((uint32_t)v, (uint32_t)v, false, false),
+          __builtin_amdgcn_permlane32_swap((uint32_t)(v >> 32), (uint32_t)(v >> 32), false, false));
   return v;
 }
 
 // The same choice of one token by a whole wavefront, EACH neighbouring experts a
-// lane; d: LDS for 64 EACH doubles. Lane j returns choice j. A few tokens go through
+// lane; d: LDS for 64 EACH doubles. Lane j returns choice j and its logit. A few tokens go through
 // it, each once in a while, so what it takes is fetching its code and waiting for
-// one step after the other: there is one exp and one quotient, in a loop.
+// one step after the other: exps and quotients go side by side (65.4 us against 67.2
+// in the case above with one after the other and shuffles through LDS).
 template <class T, int EACH>
-__device__ inline int32_t pick_exactly(const RouteArgs& a, int64_t t, double* d) {
+__device__ inline int32_t pick_exactly(const RouteArgs& a, int64_t t, double* d, float& lc) {
+  constexpr int SIDE = EACH < 4 ? EACH : 4;  // exps and quotients side by side
   const uint32_t lane = threadIdx.x & 63, e0 = lane * EACH;
   const bool scores = by_scores(a);
   float l[EACH], b[EACH], big = -INFINITY;
@@ -238,7 +246,7 @@ __device__ inline int32_t pick_exactly(const RouteArgs& a, int64_t t, double* d)
 #pragma unroll
     for (int i = 0; i < EACH; ++i) d[e0 + i] = a.sigmoid ? -(double)l[i] : (double)l[i] - (double)big;
     double z = 0;
-#pragma unroll 1
+#pragma unroll SIDE
     for (int i = 0; i < EACH; ++i) {
       const double v = exp(d[e0 + i]);
       d[e0 + i] = v;
@@ -247,7 +255,7 @@ __device__ inline int32_t pick_exactly(const RouteArgs& a, int64_t t, double* d)
     if (!a.sigmoid)
 #pragma unroll 1
       for (int m = 1; m < 64; m *= 2) z += __shfl_xor(z, m);
-#pragma unroll 1
+#pragma unroll SIDE
     for (int i = 0; i < EACH; ++i) {
       const double v = d[e0 + i];
       d[e0 + i] = (a.sigmoid ? 1.0 : v) / (a.sigmoid ? 1.0 + v : z);
@@ -309,16 +317,22 @@ __device__ inline int32_t pick_exactly(const RouteArgs& a, int64_t t, double* d)
   for (uint32_t j = 0; j < a.k; ++j) {
     uint64_t mine = 0;  // the largest of this lane's, the lowest of equals at `at`
     uint32_t at = 0;
+    float own = 0;
 #pragma unroll
     for (int i = 0; i < EACH; ++i) {
       at = key[i] > mine ? i : at;
+      own = key[i] > mine ? l[i] : own;
       mine = key[i] > mine ? key[i] : mine;
     }
     const uint64_t best = most_key64(mine);
     if (!best) break;
     const uint32_t from = __ffsll((unsigned long long)__ballot(mine == best)) - 1;
     at = __builtin_amdgcn_readlane(at, from);
-    if (lane == j) chosen = (int32_t)(from * EACH + at);
+    own = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(own), from));
+    if (lane == j) {
+      chosen = (int32_t)(from * EACH + at);
+      lc = own;
+    }
 #pragma unroll
     for (int i = 0; i < EACH; ++i) key[i] = lane == from && i == (int)at ? 0 : key[i];
   }
@@ -548,8 +562,8 @@ __device__ void choose_exactly(const RouteArgs& a, int64_t t0, int64_t t1, uint3
     uint64_t marked = __ballot(look < t1 && a.experts[look * a.k] == UNSURE);
     for (; marked; marked &= marked - 1) {
       const int64_t t = at + (int64_t)(__ffsll((unsigned long long)marked) - 1) * WAVES;
-      const int32_t e[1] = {pick_exactly<T, EACH>(a, t, d)};
-      float lc[1] = {e[0] < 0 ? -INFINITY : to_float(((const T*)a.logits)[t * a.ld + e[0]])}, w[1];
+      float lc[1] = {-INFINITY}, w[1];
+      const int32_t e[1] = {pick_exactly<T, EACH>(a, t, d, lc[0])};
       float big = -INFINITY, z = 0;
       const bool full = !a.normalize && !a.sigmoid;
       for (uint32_t i = 0; full && i < each; ++i) {
