@@ -172,9 +172,8 @@ def lora_linear(x, weight, lora_a, lora_b, experts, weights=None, scale=None, bi
                 groups: Optional[Groups] = None):
     """y[t] = weight @ x[t] + bias + sum_j weights[t, j] scale[e] B[e] @ (A[e] @ x[t]), e = experts[t, j].
 
-    x [T, d_in]; weight [d_out, d_in] (or a `Weight4` of it) and bias [d_out]
-    frozen; lora_a
-    [n, rank, d_in] and lora_b [n, d_out, rank] (PEFT's layout; rank <= 128,
+    x [T, d_in]; weight [d_out, d_in] (or a `Weight4` of that shape) and bias
+    [d_out] frozen; lora_a [n, rank, d_in] and lora_b [n, d_out, rank] (PEFT's layout; rank <= 128,
     shorter adapters padded with zeros); experts [T] or [T, k] int32, outside
     [0, n) none: each request's adapter, or `route`'s choice; weights [T, k]
     float32 or None (ones): `route`'s; scale [n] float32 or None (ones). The
