@@ -165,7 +165,12 @@ __global__ void __launch_bounds__(256) pack4_kernel(FourRows a, uint32_t parts) 
       uint32_t c[8];
       uint64_t w = 0x0808080808080808ull;
       const bool whole = row < a.rows && k + 8 <= a.cols;
-      if (whole) __builtin_memcpy(&w, in + k, 8);
+      if (whole) {
+        __builtin_memcpy(&w, in + k, 8);
+      } else if (a.four.zeros && row < a.rows && k >> f.shift < a.scale_cols) {
+        // behind the last column the value 0: another one's multiple of the scale may be infinite
+        w = 0x0101010101010101ull * (a.zeros[(m.e * a.rows + row) * a.scale_cols + (k >> f.shift)] & 15);
+      }
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
         c[i] = (uint32_t)(w >> (8 * i)) & 15;

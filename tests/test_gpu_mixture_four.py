@@ -196,6 +196,28 @@ def test_grouped_strides_and_alignment(t):
             near(torch.autograd.grad(y, xr, dy)[0], rdx, mdx, dout * k)
 
 
+@pytest.mark.parametrize("cols,size", [(33, 32), (40, 32), (40, 64), (130, 128)])
+@pytest.mark.parametrize("t", [1, 40])
+def test_columns_behind_the_last_have_no_value(t, cols, size):
+    """Scales at which a code that stands in their place would be an infinity, which times x's zeros is NaN."""
+    g = gen(cols + t)
+    codes = torch.randint(0, 6, (2, 24, cols), generator=g, device="cuda", dtype=torch.uint8)
+    scales = torch.full((2, 24, -(-cols // size)), 12288.0, dtype=torch.float16, device="cuda")
+    z = torch.zeros(scales.shape, dtype=torch.uint8, device="cuda")
+    x = normal(g, t, cols, dtype=torch.float16, std=2.0 ** -10)
+    v = values(codes, scales, z, size).double()
+    w = mixture.pack4(codes, scales, size, zeros=z)
+    groups = mixture.group(torch.zeros(t, 1, dtype=torch.int32, device="cuda"), 2)
+    w1 = mixture.pack4(codes[0], scales[0], size, zeros=z[0])
+    none = torch.full((t,), -1, dtype=torch.int32, device="cuda")
+    a, b = normal(g, 1, 8, cols, dtype=torch.float16), normal(g, 1, 24, 8, dtype=torch.float16)
+    want = x.cpu().double() @ v[0].T
+    # products of two f16 are exact in float; cols - 1 additions of them and one rounding to f16
+    bound = want.abs() * 2.0 ** -11 + (cols * 2.0 ** -23) * (x.cpu().double().abs() @ v[0].abs().T)
+    for y in (mixture.grouped_matmul(x, w, groups)[:, 0], mixture.lora_linear(x, w1, a, b, none)):
+        assert bool(((y.cpu().double() - want).abs() <= bound).all())
+
+
 @pytest.mark.parametrize("t", [20, 2500])
 def test_bad_values_stay_where_they_are(t):
     """A NaN scale shows in its row of its expert alone; a token's infinity in its own outputs, with the sign of its weight."""
