@@ -514,7 +514,7 @@ int th_lora_linear_backward(const th_lora_linear_args* d, const float* u, const 
  * above 2^120, makes its group's values NaN. */
 typedef struct th_weight4 {
   int dtype; /* TH_BF16 or TH_F16: scales and values */
-  uint32_t matrices, d_out, d_in;
+  uint32_t matrices, d_out, d_in; /* at most 2^30 columns; below 2^28 rows in all, each matrix's rounded up to 16 */
   uint32_t group; /* columns of a scale: a power of two, 32 to 2^30 */
   int zeros;      /* whether groups have zeros */
   void* data;

@@ -184,6 +184,8 @@ th::FourLayout check_weight4(const th_weight4* w, bool data = true) {
   mix_type(w->dtype, false);
   need(w->matrices >= 1 && w->d_in >= 1 && w->d_out >= 1, "matrices, d_in and d_out must be positive");
   need(w->d_in <= 1u << 30 && w->d_out <= 1u << 30, "d_in and d_out must be at most 2^30");
+  // a workgroup of 256 threads for 16 rows, below 2^32 threads in a launch
+  need(th::ceil_div(w->d_out, 16) * w->matrices < 1u << 24, "the matrices' rows in all must be below 2^28");
   need(w->group >= th::FOUR_MIN_GROUP && w->group <= th::FOUR_MAX_GROUP && (w->group & (w->group - 1)) == 0,
        "group must be a power of two from 32 to 2^30");
   if (data) {

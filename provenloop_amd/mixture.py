@@ -66,7 +66,8 @@ class Routing(NamedTuple):
 
 class Weight4(NamedTuple):
     """Frozen weights of 4 bits: the values scale * (code - zero), rounded to dtype,
-    with a scale (and a zero) for each row's group_size neighbouring columns.
+    with a scale (and a zero) for each row's group_size neighbouring columns. At
+    most 2^30 columns, below 2^28 rows in all.
 
     Made by `quantize4` and `pack4`; used in place of a weight by `grouped_matmul`
     and `lora_linear`. data is the layout that the kernels read, half a byte a

@@ -22,6 +22,7 @@ BAD_WEIGHTS = [(dict(dtype=3), "dtype"), (dict(dtype=0), "dtype"), (dict(matrice
                (dict(d_in=0), "positive"), (dict(d_in=(1 << 30) + 1), "2^30"), (dict(group=16), "power of two"),
                (dict(group=96), "power of two"), (dict(group=1 << 31), "power of two")]
 
+BAD_WEIGHTS += [(dict(d_out=1 << 28), "2^28"), (dict(matrices=1 << 24), "2^28"), (dict(matrices=0xffffffff, d_out=1 << 30, d_in=1 << 30), "2^28")]
 
 @pytest.mark.parametrize("change,text", BAD_WEIGHTS + [(dict(data=None), "null data"), (dict(data=P + 8), "multiple of 16")])
 def test_weights(change, text):
