@@ -481,13 +481,13 @@ __device__ void choose_balanced(const RouteArgs& a, int64_t t0, int64_t t1, uint
       if (!scores) clear = INFINITY;  // logits are what they are, and ties are in order
     }
 
-    int32_t e[P * EACH];
+    int32_t e[P * EACH];  // -1 also of the passes that k does not reach
+#pragma unroll
+    for (int q = 0; q < P * EACH; ++q) e[q] = -1;
     double limit = INFINITY;  // the last pass's least
     float last = INFINITY;
 #pragma unroll
     for (int p = 0; p < P; ++p) {
-#pragma unroll
-      for (int q = 0; q < EACH; ++q) e[p * EACH + q] = -1;
       if (p * 8 >= (int)a.k) break;
       const bool ask = scores && (int)a.k == 8 * (p + 1);
       double top[8], rest = -INFINITY;

@@ -191,6 +191,20 @@ def test_extremes_and_bad_values():
     torch.testing.assert_close(w, torch.tensor([[2 / 3, 1 / 3]]), rtol=2.0 ** -20, atol=0)
 
 
+@pytest.mark.parametrize("e", [16, 40, 64, 130, 256, 300, 512])
+def test_every_number_of_choices(e):
+    """1 to 32, each with weights that are its own sum's."""
+    g = gen(e)
+    logits = normal(g, 40, e)
+    bias = normal(g, e, std=0.1)
+    for k in range(1, min(e, 32) + 1):
+        for opts in (dict(score="sigmoid"), dict(bias=bias)):
+            r = mixture.route(logits, k, **opts)
+            w, ids, _, _ = oracle(logits, k, **opts)
+            assert np.array_equal(r.experts.cpu().numpy(), ids), k
+            np.testing.assert_allclose(r.weights.cpu().numpy(), w, rtol=2.0 ** -18, atol=2.0 ** -126)
+
+
 def test_strides_and_masks():
     g = gen(3)
     wide = normal(g, 50, 40, dtype=torch.bfloat16)
