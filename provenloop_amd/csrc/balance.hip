@@ -96,7 +96,7 @@ constexpr uint32_t lane_space(int C) { return 3 * C; }
 // ---------------------------------------------------------------- 8 numbers in falling order
 // A candidate is a double: its c, which float's 24 bits leave 29 bits of, and below
 // these the expert's number, so that of equal c the lowest expert's is the larger.
-// -inf: none.
+// -inf: none; c is not -0, whose expert would be read as another's.
 __device__ inline double candidate(float c, uint32_t e) {
   const uint64_t b = (uint64_t)__double_as_longlong((double)c);
   const uint32_t low = c == -INFINITY ? 0 : c < 0 ? e : 511 - e;
@@ -471,6 +471,10 @@ __device__ void choose_balanced(const RouteArgs& a, int64_t t0, int64_t t1, uint
         }
         __builtin_amdgcn_sched_barrier(0);
       }
+    } else {
+      // -0 is 0, and a candidate's sign is its number's; a score is never -0
+#pragma unroll
+      for (int i = 0; i < 8 * C; ++i) c[i] += 0.0f;
     }
     bool bad = false;  // a NaN or +inf, which the candidates cannot hold
 #pragma unroll
@@ -535,7 +539,7 @@ __device__ void choose_balanced(const RouteArgs& a, int64_t t0, int64_t t1, uint
 
     float lc[P * EACH], w[P * EACH];
 #pragma unroll
-    for (int q = 0; q < P * EACH; ++q) lc[q] = e[q] < 0 ? -INFINITY : (float)row[e[q]];
+    for (int q = 0; q < P * EACH; ++q) lc[q] = e[q] < 0 ? -INFINITY : (float)row[min((uint32_t)e[q], a.E - 1)];  // a NaN's number may be any
     weigh<G>(a, lc, big, z, w);
     if (here >= t1) continue;
     if (!sure) {
@@ -619,9 +623,10 @@ __global__ void __launch_bounds__(THREADS) balanced_kernel(RouteArgs a, int near
   __syncthreads();
   asm volatile("" ::"v"(ahead));
   // How near two decisive numbers may come. A sigmoid is off by up to 2^-22, a
-  // softmax's share by 2^-20 (a sum 14 additions deep), a sum with the bias by
-  // 2^-24 of its size; a node's sum of two twice all that and 2^-24 of its own, and
-  // so does a difference. Near a bias that is NaN or infinite is everything.
+  // softmax's share by 2^-22 and by its sum's error, up to 35 additions deep, 2^-18.8
+  // of the difference between two shares; a sum with the bias by 2^-24 of its size; a
+  // node's sum of two twice all that but the sum's and 2^-24 of its own, and so is a
+  // difference. Near a bias that is NaN or infinite is everything.
   const float near = !by_scores(a) ? 0 : (a.sigmoid ? 0x1p-20f : 0x1p-18f) + 0x1p-21f * (1 + __uint_as_float(size));
   if (near_first) {
     choose_balanced<T, G, C, P>(a, t0, t1, base, (float*)lds, sbias, near, &unsure);

@@ -191,6 +191,24 @@ def test_extremes_and_bad_values():
     torch.testing.assert_close(w, torch.tensor([[2 / 3, 1 / 3]]), rtol=2.0 ** -20, atol=0)
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("e,k,nodes,top,best", [(4, 2, 1, 1, 1), (13, 5, 1, 1, 1), (64, 8, 8, 2, 1), (200, 12, 1, 1, 1), (512, 8, 4, 2, 2)])
+def test_zeros_of_both_signs(dtype, e, k, nodes, top, best):
+    """-0 and 0 are equal, and go to the lowest index."""
+    g = gen(e)
+    logits = torch.randint(-1, 2, (300, e), generator=g, device="cuda").float()
+    logits = torch.where(torch.rand(300, e, generator=g, device="cuda") < 0.5, logits, -logits).to(TYPES[dtype])
+    assert bool((torch.signbit(logits) & (logits == 0)).any())
+    bias = torch.where(torch.rand(e, generator=g, device="cuda") < 0.5, 0.0, -0.0)
+    for opts in (dict(score="sigmoid"), dict(scale=2.0), dict(score="sigmoid", bias=bias)):
+        opts = dict(opts, nodes=nodes, top_nodes=top, node_best=best)
+        r = mixture.route(logits, k, **opts)
+        w, ids, _, _ = oracle(logits, k, **opts)
+        assert np.array_equal(r.experts.cpu().numpy(), ids)
+        np.testing.assert_allclose(r.weights.cpu().numpy(), w, rtol=2.0 ** -18, atol=0)
+        check_groups(r.groups, e)
+
+
 @pytest.mark.parametrize("e", [16, 40, 64, 130, 256, 300, 512])
 def test_every_number_of_choices(e):
     """1 to 32, each with weights that are its own sum's."""
