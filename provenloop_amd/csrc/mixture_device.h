@@ -192,6 +192,19 @@ struct GroupTile {
 __device__ inline int64_t group_begin(const int32_t* offsets, uint32_t g, uint32_t E, int64_t slots) {
   return g > E ? slots : min(max((int64_t)offsets[g], (int64_t)0), slots);
 }
+// Sum of a wavefront's words up to each lane's own, in registers: through LDS, as
+// shuffles go, the six steps take 0.4 us, which a decode waits for.
+__device__ inline uint32_t wave_prefix(uint32_t v) {
+  v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xf, 0xf, false);  // from 1, 2, 4, 8 lanes below in rows of 16
+  v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xf, 0xf, false);
+  v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xa, 0xf, false);  // rows 1 and 3: the last of the row below
+  v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xc, 0xf, false);  // rows 2 and 3: the last of row 1
+  return v;
+}
+__device__ inline uint32_t lane_word(uint32_t v, uint32_t lane) { return __builtin_amdgcn_readlane(v, lane); }
+
 // Tiles of all groups [0, groups); every lane of the calling wavefront gets the answer.
 __device__ inline uint32_t count_group_tiles(const int32_t* offsets, uint32_t E, uint32_t groups, int64_t slots,
                                              uint32_t bm, uint32_t lane) {
@@ -200,8 +213,7 @@ __device__ inline uint32_t count_group_tiles(const int32_t* offsets, uint32_t E,
     const int64_t c = group_begin(offsets, g + 1, E, slots) - group_begin(offsets, g, E, slots);
     if (c > 0) n += (uint32_t)((c + bm - 1) / bm);
   }
-  for (int d = 32; d; d >>= 1) n += __shfl_xor(n, d);
-  return n;
+  return lane_word(wave_prefix(n), 63);
 }
 __device__ inline GroupTile find_group_tile(const int32_t* offsets, uint32_t E, uint32_t groups, int64_t slots,
                                             uint32_t bm, uint32_t tile, uint32_t lane) {
@@ -215,21 +227,17 @@ __device__ inline GroupTile find_group_tile(const int32_t* offsets, uint32_t E, 
       c = group_begin(offsets, g + 1, E, slots) - lo;
     }
     const uint32_t n = c > 0 ? (uint32_t)((c + bm - 1) / bm) : 0;
-    uint32_t sum = n;
-    for (int d = 1; d < 64; d <<= 1) {
-      const uint32_t up = __shfl_up(sum, d);
-      if ((int)lane >= d) sum += up;
-    }
+    const uint32_t sum = wave_prefix(n);
     const uint32_t first = before + sum - n;
     const uint64_t here = __ballot(n && tile >= first && tile < first + n);
     if (here) {
       const int src = __ffsll((unsigned long long)here) - 1;
       t.group = at + src;
-      t.begin = __shfl((int)lo, src) + (int64_t)(tile - __shfl(first, src)) * bm;
-      t.end = min(t.begin + (int64_t)bm, (int64_t)__shfl((int)(lo + c), src));
+      t.begin = lane_word((uint32_t)lo, src) + (int64_t)(tile - lane_word(first, src)) * bm;
+      t.end = min(t.begin + (int64_t)bm, (int64_t)lane_word((uint32_t)(lo + c), src));
       return t;
     }
-    before += __shfl(sum, 63);
+    before += lane_word(sum, 63);
   }
   return t;
 }

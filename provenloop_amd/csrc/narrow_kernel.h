@@ -131,6 +131,7 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
     if (scan) return list[i];
     return a.order ? min((int64_t)(uint32_t)a.order[i], a.rows - 1) : i;
   };
+  auto row_of = [&](int64_t i) -> int64_t { return (uint32_t)slot_of(i) / a.div; };  // of x: slots are below 2^31
   const bool has = !grouped || g.group < a.E;
   const T* w = (const T*)a.w + (grouped || scan ? (int64_t)g.group * a.ldwe : 0);
   const T* zero = (const T*)&mix_zero16;
@@ -154,7 +155,7 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
       const uint32_t rows_left = (uint32_t)min(g.end - m0, (int64_t)BM);
       const bool all_rows = rows_left > BM - 8;
 #pragma unroll
-      for (int j = 0; j < 2 * MT; ++j) p[j] = (const T*)a.x + slot_of(m0 + j * 8 + lane / 8) / a.div * a.ldx + xk;
+      for (int j = 0; j < 2 * MT; ++j) p[j] = (const T*)a.x + row_of(m0 + j * 8 + lane / 8) * a.ldx + xk;
       const uint64_t e = grouped && has ? g.group : 0;
       const uint32_t rows = f.strips * 16;  // of the weights as they are stored
       const uint32_t strip = n0 / 16 + (NT == 2 ? lane / 32 : 0);
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
       for (int j = 0; j < LOADS; ++j) {
         const int jw = j - 2 * MT;
         if (j < 2 * MT) {
-          p[j] = (const T*)a.x + slot_of(m0 + j * 8 + lane / 8) / a.div * a.ldx + xk;
+          p[j] = (const T*)a.x + row_of(m0 + j * 8 + lane / 8) * a.ldx + xk;
         } else if constexpr (TR) {
           const uint32_t row = jw * (64 / CH) + lane / CH, col = n0 + ((lane % CH) ^ tr_swizzle<BN>(row)) * 8;
           p[j] = col < a.n ? w + (int64_t)row * a.ldw + col : nullptr;
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(64 * WAVES) narrow_kernel(MatArgs a, uint32_t 
       const uint32_t kl = lane / 16 * 16;  // this lane's 16 values of a line
       const T *xp[MT], *wp[NT];
 #pragma unroll
-      for (int mi = 0; mi < MT; ++mi) xp[mi] = (const T*)a.x + slot_of(m0 + mi * 16 + lane % 16) / a.div * a.ldx + kl;
+      for (int mi = 0; mi < MT; ++mi) xp[mi] = (const T*)a.x + row_of(m0 + mi * 16 + lane % 16) * a.ldx + kl;
 #pragma unroll
       for (int ni = 0; ni < NT; ++ni) wp[ni] = w + (int64_t)min(n0 + ni * 16 + lane % 16, a.n - 1) * a.ldw + kl;
       struct Line {
