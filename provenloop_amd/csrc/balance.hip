@@ -22,7 +22,7 @@
 // with 8: the fewer lanes a token has, the fewer steps go across lanes, which cost
 // most. 65536 tokens of 256 experts on 8 nodes, 8 chosen, with the launch that places
 // their slots (16 us): 47 us where no two numbers come near (with 32 lanes a token and
-// rounds that take the largest of the lanes' first: 87), 65 where a few tokens of nearly
+// rounds that take the largest of the lanes' first: 87), 64 where a few tokens of nearly
 // every workgroup are decided again: one of these takes 13 us and more, waiting for one
 // step after the other. A copy's rate would be 8 us; about 2100 vector instructions a
 // wavefront's 8 tokens are 33 of it. One token takes 9.3 us: the chain of its steps.

@@ -7,8 +7,9 @@
 // A quarter of the weights' bytes leaves other things to wait for: x, which every
 // column tile reads from L2 again (8 groups of 4 rows, 3584 -> 3584: 24.8 us for 53 MB
 // with 16 columns a tile, 21.0 with 32), the 23 instructions a word, and for one row
-// the chain of steps before the first load (1536 -> 1536 5.0 us in a series of
-// launches, 3584 -> 3584 6.7).
+// the chain of steps before the first load (1536 -> 1536 4.7 us in a series of
+// launches, 3584 -> 3584 6.2). More lines in the rings change nothing (16 x 32 with
+// 2, 3 and 4: 9.3, 9.3 and 9.4 us at 32 rows of 3584 -> 3584).
 #include "narrow_kernel.h"
 
 using namespace mix;
