@@ -260,8 +260,9 @@ __device__ inline int32_t pick_exactly(const RouteArgs& a, int64_t t, double* d,
       const double v = d[e0 + i];
       d[e0 + i] = (a.sigmoid ? 1.0 : v) / (a.sigmoid ? 1.0 + v : z);
     }
+    // a bias of -inf withholds its expert whatever the score, which may be NaN
 #pragma unroll
-    for (int i = 0; i < EACH; ++i) c[i] = l[i] == -INFINITY ? -INFINITY : d[e0 + i] + (double)b[i];
+    for (int i = 0; i < EACH; ++i) c[i] = l[i] == -INFINITY || b[i] == -INFINITY ? -INFINITY : d[e0 + i] + (double)b[i];
   }
   if (a.nodes > 1) {
     // a node's value and then whether it is kept are laid in its first expert's place
@@ -476,7 +477,7 @@ __device__ void choose_balanced(const RouteArgs& a, int64_t t0, int64_t t1, uint
 #pragma unroll
       for (int i = 0; i < 8 * C; ++i) c[i] += 0.0f;
     }
-    bool bad = false;  // a NaN or +inf, which the candidates cannot hold
+    bool bad = false;  // a NaN or +inf, which the candidates cannot hold: decided in double, also where its bias is -inf
 #pragma unroll
     for (int i = 0; i < 8 * C; ++i) bad |= !(c[i] < INFINITY);
     float clear = INFINITY;  // the least difference that decides something
