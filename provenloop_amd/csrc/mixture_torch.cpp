@@ -235,6 +235,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> route(const Tensor& given, int64_t k,
     NEED(bias.scalar_type() == at::kFloat && bias.dim() == 1 && bias.size(0) == e, "route: bias must be float32 [E]");
     NEED(!bias.requires_grad() || !at::GradMode::is_enabled(), "route: bias takes part in the choice alone and has no gradient");
   }
+  NEED(node_best == 1 || node_best == 2, "route: node_best must be 1 or 2");
   NEED(nodes >= 1 && nodes <= e && top_nodes >= 1 && top_nodes <= nodes, "route: top_nodes must be in [1, nodes], nodes in [1, number of experts]");
   on_gpu("route", given, {mask, bias});
   if (mask.defined()) {
