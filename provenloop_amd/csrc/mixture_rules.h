@@ -160,9 +160,10 @@ constexpr bool four_narrow(uint64_t rows, uint32_t n, uint32_t k, uint32_t group
 // -> 3584: 16 rows 7.8 with 16 x 16 and 9.1 with 16 x 32, 32 rows 12.5 and 9.3; 64
 // rows 12.3 with 16 x 32 and 10.7 with 32 x 32; 128 rows 20.4 with 32 x 32 and 14.8
 // with 64 x 32). Larger ones take 4 wavefronts, three workgroups a CU of 32 x 32 or two
-// of 64 x 32, which of them has fewer rounds (256 rows 29.8 and 23.7, 384 rows 38.5
-// and 39.2). Groups of up to 16 rows are weights to be read: 16 x 32 (8 groups of 4
-// rows 21.0, with 16 x 16 40.6).
+// of 64 x 32, with adapters and without, which of them has fewer rounds (without, 256
+// rows 29.8 and 23.7, 384 rows 38.5 and 39.2; with rank 32 and A x 39.3 and 34.3, 49.6
+// and 51.4, 512 rows 58.0 and 59.4). Groups of up to 16 rows are weights to be read:
+// 16 x 32 (8 groups of 4 rows 21.0, with 16 x 16 40.6).
 enum FourTile { FOUR_16x16, FOUR_16x32, FOUR_32x32_ONCE, FOUR_64x32_ONCE, FOUR_32x32, FOUR_64x32 };
 constexpr FourTile four_tile(uint64_t rows, uint32_t n, uint32_t groups) {
   const uint64_t each = ceil_div(rows, groups), n32 = groups * ceil_div(n, 32);
