@@ -421,10 +421,11 @@ int th_route_backward(int dtype, const void* logits, int64_t ld, int64_t tokens,
  * largest s + bias are chosen (bias NULL: of largest l; an expert whose bias is
  * -inf is not chosen). With nodes > 1 the experts lie on that many nodes, in
  * order and equally many each, and only those of the top_nodes nodes of largest
- * value may be chosen; a node's value is its largest s + bias, or the sum of its
- * node_best = 2 largest. Ties go to the lowest number. The choice is that of s
- * and s + bias in 64 bits. weights = scale s / sum of the chosen s (normalize), or
- * scale s. bias: a float per expert, which takes part in the choice alone. */
+ * value may be chosen; a node's value is its largest s + bias (bias NULL: largest
+ * l), or the sum of its node_best = 2 largest s + bias (bias NULL: s). Ties go to
+ * the lowest number. The choice is that of l, or of s and s + bias in 64 bits.
+ * weights = scale s / sum of the chosen s (normalize), or scale s. bias: a float
+ * per expert, which takes part in the choice alone. */
 enum { TH_SOFTMAX = 0, TH_SIGMOID = 1 };
 typedef struct th_gate_args {
   int dtype; /* of the logits: TH_BF16, TH_F16 or TH_F32 */

@@ -3,9 +3,10 @@
 // may use a few.
 //
 //   s_e = exp(l_e - max l) / sum over the allowed  or  1 / (1 + exp(-l_e))
-//   c_e = s_e + bias_e; without a bias, and with a node's value its largest c, the
-//         logits themselves, whose order is the scores'
-//   value of a node = its largest c, or the sum of its two largest
+//   c_e = s_e + bias_e; without a bias the logit l_e, whose order is the scores' and
+//         which tells apart what scores in 64 bits round to one number
+//   value of a node = its largest c, or the sum of its two largest (without a bias,
+//                     of its two largest s)
 // Of the nodes the top_nodes of largest value are kept, of their experts the k of
 // largest c, ties to the lowest number each, and
 //   w_j = scale s_j / (sum of the chosen s, or 1).
@@ -20,12 +21,18 @@
 // Up to 16 lanes take a token, several chunks of 8 experts a lane. Chunks are put in
 // order in a lane's registers and merged there and then across the lanes, 8 numbers
 // with 8: the fewer lanes a token has, the fewer steps go across lanes, which cost
-// most. 65536 tokens of 256 experts on 8 nodes, 8 chosen, with the launch that places
-// their slots (16 us): 47 us where no two numbers come near (with 32 lanes a token and
-// rounds that take the largest of the lanes' first: 87), 64 where a few tokens of nearly
-// every workgroup are decided again: one of these takes 13 us and more, waiting for one
-// step after the other. A copy's rate would be 8 us; about 2100 vector instructions a
-// wavefront's 8 tokens are 33 of it. One token takes 9.3 us: the chain of its steps.
+// most. 65536 tokens of 256 experts on 8 nodes, 8 chosen, bf16 logits, kernel times of
+// one trace: 44 us where no two numbers come near, 52 (57 on another card) where a few
+// tokens of nearly every workgroup are decided again, and 16 for the launch that places
+// their slots; 57 and 67 us a call in a series. A token that is decided again takes 13
+// us and more, waiting for one step after the other. Both launches' bytes are 8 us at a
+// copy's rate; about 2100 vector instructions a wavefront's 8 tokens are 33 of the 44.
+// One token takes 9.3 us of 64 experts and 20 of 256: the chain of its steps.
+//
+// A workgroup of 16 wavefronts has 128 registers a lane, and the forms for more than
+// 128 experts (more than 64 with more than 8 choices) need some more: 28 bytes a lane
+// are in scratch for 256 experts and 56 for 512, 44, 260 and 240 for 128, 256 and 512
+// with more than 8 choices.
 #include "route_device.h"
 
 using namespace mix;
@@ -405,7 +412,7 @@ __device__ void choose_balanced(const RouteArgs& a, int64_t t0, int64_t t1, uint
 #pragma unroll
     for (int i = 0; i < C; ++i) asm volatile("" : "+v"(first[i]), "+v"(count[i]));
     // the logits, -inf where the expert is not allowed; one chunk after the other
-    // here and below: several at once do not fit the registers
+    // here and below: several at once would put more of them into scratch
     float c[8 * C];
     if (whole) {
       T l[8 * C];
@@ -627,7 +634,9 @@ __global__ void __launch_bounds__(THREADS) balanced_kernel(RouteArgs a, int near
   // softmax's share by 2^-22 and by its sum's error, up to 35 additions deep, 2^-18.8
   // of the difference between two shares; a sum with the bias by 2^-24 of its size; a
   // node's sum of two twice all that but the sum's and 2^-24 of its own, and so is a
-  // difference. Near a bias that is NaN or infinite is everything.
+  // difference. Near a bias that is NaN or infinite is everything, and the more the
+  // larger it is: one of -1e4 or less that is to withhold an expert sends every token to
+  // be decided in double (65536 tokens as above: 229 us for 64), one of -inf none.
   const float near = !by_scores(a) ? 0 : (a.sigmoid ? 0x1p-20f : 0x1p-18f) + 0x1p-21f * (1 + __uint_as_float(size));
   if (near_first) {
     choose_balanced<T, G, C, P>(a, t0, t1, base, (float*)lds, sbias, near, &unsure);
@@ -644,7 +653,9 @@ __global__ void __launch_bounds__(THREADS) balanced_kernel(RouteArgs a, int near
 // With p the weights without their scale, P = sum p_i dw_i over the chosen:
 //   normalized    softmax  w_j (dw_j - P)             sigmoid  w_j (1 - s_j) (dw_j - P), at the chosen
 //   not           softmax  [chosen] w_e dw_e - scale s_e P     sigmoid  w_j (1 - s_j) dw_j
-// A wavefront a token.
+// A wavefront a token. 4099 tokens of 60 experts, 5 chosen, take 6.8 us; 65536 of 256,
+// 8 chosen, in bf16 138 us for 70 MB (14 at a copy's rate): every lane reads the
+// token's choices, weights and gradients again for each 64 experts.
 template <class T>
 __global__ void __launch_bounds__(256) balanced_backward_kernel(RouteArgs a, const float* dweights, T* dlogits) {
   const uint32_t lane = threadIdx.x & 63;
@@ -693,7 +704,8 @@ hipError_t sized(const RouteArgs& a, int near_first, uint32_t chunks, hipStream_
 template <class T>
 hipError_t typed(const RouteArgs& a, uint32_t chunks, hipStream_t s) {
   // chunks of 8 that nodes have for themselves; more than the 64 of 512 experts (nodes
-  // of a few experts) are not laid out, and every token is decided in double
+  // of a few experts) are not laid out, and every token is decided in double (65536
+  // tokens of 512 experts, 8 chosen: on 64 nodes 187 us, on 128 nodes 764, on 256 2260)
   const uint64_t n = (uint64_t)chunks_of(a.E, a.nodes).chunks_per * a.nodes;
   const int near_first = n <= 64;
   const uint64_t m = near_first ? n : (a.E + 7) / 8;

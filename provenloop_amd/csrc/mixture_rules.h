@@ -41,7 +41,10 @@ constexpr uint64_t group_chunk_tokens(uint64_t tokens, uint32_t k) {
 }
 // The same for a balanced gate, which takes longer for a token than placing its
 // slots does: as few as give each of 256 workgroups some, down to 32 tokens, which
-// fill a wavefront on each SIMD.
+// fill a wavefront on each SIMD. Up to 2048 slots stay one workgroup here too, which is
+// the quicker for few tokens only (us, 256 experts, 4 of 8 nodes: 128 tokens of 8
+// choices 28.6, 256 43.8, 257 in nine workgroups 31.9; of 1 choice 128 tokens 20, 512
+// 57, 2048 213, 2049 in 65 workgroups 34).
 constexpr uint64_t gate_chunk_tokens(uint64_t tokens, uint32_t k) {
   const uint64_t chunk = group_chunk_tokens(tokens, k), few = ceil_div(tokens, 256) < 32 ? 32 : ceil_div(tokens, 256);
   return tokens * k <= 2048 || chunk < few ? chunk : few;
@@ -121,9 +124,9 @@ constexpr uint32_t pad_blocks(uint64_t rows, uint32_t E, uint32_t cols) {
 //           4 i .. + 4 and 16 + 4 i .. + 4: a shift and a mask leave a pair.
 //   scales  of a group of columns for every row, rows rounded up to 16, group
 //           after group (2 bytes each); zeros the same (a byte each).
-// Rows and columns beyond the matrix's have code 8; its groups and rows beyond
-// have scale 0. The columns of a scale are a power of two, so that a group's
-// number is a shift.
+// Rows and groups beyond the matrix's have scale 0; columns behind a row's last have
+// the code whose value is 0 (8, or their group's zero). The columns of a scale are a
+// power of two, so that a group's number is a shift.
 constexpr uint32_t FOUR_MIN_GROUP = 32;       // the columns of a matrix instruction
 constexpr uint32_t FOUR_MAX_GROUP = 1u << 30;
 struct FourLayout {
@@ -147,7 +150,10 @@ constexpr uint64_t four_bytes(const FourLayout& f, uint32_t matrices, bool zeros
 // for each 64 steps of a round over the CUs, the values a 1900th a weight (tiles /
 // values in us: 512 rows of 3584 -> 3584 45 / 53, 768 rows 65 / 52; 1024 of 1536 ->
 // 1536 22 / 28; 8 groups of 100 rows, 3584 -> 1536 43 / 65, of 256 rows, 1536 -> 1536
-// 52 / 35; 64 groups of 24 rows, 1536 -> 1536 52 / 205).
+// 52 / 35; 64 groups of 24 rows, 1536 -> 1536 52 / 205). All without adapters. With them
+// the large tiles take the ranks of every adapter that a tile's rows use as further
+// steps, and codes are quicker for longer if these are many (3584 -> 3584, 32 adapters of
+// rank 32, with A x: 512 rows 59 / 117, 640 rows, which go by the values, 73 / 119).
 constexpr bool four_narrow(uint64_t rows, uint32_t n, uint32_t k, uint32_t groups) {
   const uint64_t each = ceil_div(rows, groups), lines = ceil_div(k, 64);
   const uint64_t tiles = groups * ceil_div(each, 32) * ceil_div(n, 32);

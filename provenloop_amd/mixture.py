@@ -94,7 +94,8 @@ def quantize4(weight, group_size: int = 128, zeros: bool = False) -> Weight4:
     codes stand for -7 .. 7 scales; with zeros, scale = (max - min) / 15 over the
     group's values and 0, and zero = -min / scale. Scales are rounded to the
     weight's type first, codes to the nearest value (ties to even). A group with
-    an infinity or NaN becomes NaN. Has no gradient.
+    an infinity or NaN becomes NaN, in bf16 also one whose scale is above 2^120.
+    Has no gradient.
     """
     return Weight4(_ext.quantize4(weight, group_size, zeros), tuple(weight.shape), weight.dtype, group_size, bool(zeros))
 
@@ -141,14 +142,17 @@ def route(logits, k: int, mask=None, normalize: bool = True, *, score: str = "so
     weight 0 there. Differentiable in the logits.
 
     score: "softmax" as above, or "sigmoid", s = 1 / (1 + exp(-l)) and weights s,
-    or s over the sum of the chosen ones (normalize=True). scale: a positive number
-    that multiplies the weights. bias [E] float32, which takes part in the choice
-    alone: the k largest s + bias are chosen (an expert whose bias is -inf never
-    is). Balancing raises it for experts with few slots and lowers it for those
-    with many, as groups.offsets counts them. nodes: the experts lie in order on
-    that many nodes, E / nodes each, and a token uses those of top_nodes nodes
-    alone: of the nodes whose largest s + bias, or sum of the two largest
-    (node_best=2), is largest. What is chosen is decided in 64 bits.
+    or s over the sum of the chosen ones (normalize=True). scale: a positive
+    number that multiplies the weights. bias [E] float32, which takes part in the
+    choice alone: the k largest s + bias are chosen in place of the k largest
+    logits (an expert whose bias is -inf never is; one of a large finite bias is
+    a last choice, and costs a prefill time). Balancing raises it for experts
+    with few slots and lowers it for those with many, as groups.offsets counts
+    them. nodes: the experts lie in order on that many nodes, E / nodes each, and
+    a token uses those of top_nodes nodes alone: of the nodes whose largest s +
+    bias (without a bias, largest logit), or sum of the two largest s + bias
+    (node_best=2; without a bias, of the two largest s), is largest. What scores
+    decide is decided in 64 bits.
     """
     weights, experts, order, offsets = _ext.route(logits, k, mask, normalize, score, bias, scale, nodes, top_nodes, node_best)
     return Routing(weights, experts, Groups(experts, order, offsets, logits.shape[1]))
