@@ -31,7 +31,7 @@
 //
 // A workgroup of 16 wavefronts has 128 registers a lane, and the forms for more than
 // 128 experts (more than 64 with more than 8 choices) need some more: 28 bytes a lane
-// are in scratch for 256 experts and 56 for 512, 44, 260 and 240 for 128, 256 and 512
+// are in scratch for 256 experts and 48 for 512, 44, 260 and 244 for 128, 256 and 512
 // with more than 8 choices.
 #include "route_device.h"
 
@@ -349,9 +349,11 @@ __device__ inline int32_t pick_exactly(const RouteArgs& a, int64_t t, double* d,
 
 // ---------------------------------------------------------------- weights
 // The weights of the choices of one token, which its G lanes keep, from their
-// logits lc (-inf: none): normalized ones from the largest chosen logit where they
-// are a softmax, or sigmoids so small that they are exp(l). z_all: sum of exp(l -
-// big) over the allowed, of a softmax that is not normalized.
+// logits lc (-inf: none). Normalized ones are taken from the largest chosen logit:
+// exp(l - top) of a softmax; of sigmoids, with `from` the largest or 0 if that is less,
+// s exp(-from) = exp(l - from) / (1 + exp(l)) for l <= 0, which is a float wherever the
+// weight is, though s itself may be none. z_all: sum of exp(l - big) over the allowed,
+// of a softmax that is not normalized.
 template <int G, int KEEP>
 __device__ inline void weigh(const RouteArgs& a, const float (&lc)[KEEP], float big, float z_all, float (&w)[KEEP]) {
   float top = -INFINITY;
@@ -360,13 +362,14 @@ __device__ inline void weigh(const RouteArgs& a, const float (&lc)[KEEP], float 
     for (int q = 0; q < KEEP; ++q) top = lc[q] != lc[q] || top != top ? NAN : fmaxf(top, lc[q]);
     top = most<G>(top);
   }
-  const bool by_exp = !a.sigmoid || (a.normalize && top < -40.0f);
-  const float from = a.normalize ? top : big;
+  const float from = !a.sigmoid ? a.normalize ? top : big : a.normalize ? fminf(top, 0.0f) : 0.0f;
   float z = a.normalize ? 0 : a.sigmoid ? 1 : z_all;
 #pragma unroll
   for (int q = 0; q < KEEP; ++q) {
-    const float x = expf(by_exp ? lc[q] - from : -lc[q]);
-    w[q] = lc[q] == -INFINITY ? 0.0f : by_exp ? x : 1.0f / (1.0f + x);
+    const bool small = lc[q] <= 0;
+    const float x = expf(!a.sigmoid || small ? lc[q] - from : -lc[q]);
+    const float y = a.sigmoid && from != 0 ? expf(lc[q]) : x;  // of a sigmoid: exp(-|l|)
+    w[q] = lc[q] == -INFINITY ? 0.0f : !a.sigmoid ? x : (small ? x : 1.0f) / (1.0f + y);
     if (a.normalize) z += w[q];
   }
   if (a.normalize) z = group_sum<G>(z);
